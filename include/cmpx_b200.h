@@ -43,7 +43,10 @@ extern "C" {
                                4: cmpx_attn_desc.mask / mask_kind (boolean or additive attention mask);
                                5: cmpx_bmm_small / cmpx_bmm_small_plan;
                                6: cmpx_bmm_rowstats(_plan), cmpx_softmax_product(_plan);
-                               7: cmpx_bmm_ws / cmpx_linear_ws and their workspace sizes */
+                               7: cmpx_bmm_ws / cmpx_linear_ws and their workspace sizes.
+                               The entry points of a served transformer's step (cmpx_rope,
+                               cmpx_kv_append, cmpx_paged_attn, cmpx_linear_w4) came with no change to
+                               what 7 declares: a caller finds them by symbol */
 
 /* Element type of every operand of one call (inputs and output share it, as in the reference:
  * dtype in == dtype out, src/main.cpp:1623-1627, :366-369). */
@@ -283,6 +286,154 @@ CMPX_API int cmpx_softmax_product(const cmpx_bmm_desc* desc, const float* stats,
 CMPX_API int cmpx_softmax_product_plan(const cmpx_bmm_desc* desc, const float* stats, const void* y, char* buf,
                                        size_t buf_len);
 
+/* ---------------------------------------------------------------------------------------------
+ * The step of a served transformer: rotary positions, the append to a paged key-value cache, the
+ * attention of one new token over that cache, and linear layers with 4-bit weights.  None has a
+ * counterpart among the reference's native ops; each stands beside an entry point above (the
+ * attentions beside cmpx_attn_fwd, cmpx_linear_w4 beside cmpx_linear).
+ * ------------------------------------------------------------------------------------------- */
+
+#define CMPX_ROPE_MAX_AXES 4
+
+typedef enum cmpx_pos_kind {
+  CMPX_POS_NONE = 0, /* cmpx_kv_append only: a token's position is its place in its sequence */
+  CMPX_POS_I32 = 1,
+  CMPX_POS_I64 = 2,
+  CMPX_POS_F32 = 3
+} cmpx_pos_kind;
+
+/* Rotary positions.  Pair j (0 <= j < pairs) of a row turns by position[axis(j)] * freqs[j] radians:
+ *   (a, b) -> (a cos - b sin, a sin + b cos).
+ * The pair is (x[j], x[j + pairs]), or (x[2j], x[2j + 1]) where interleaved is 1; values behind the
+ * first 2 * pairs of a row pass through.  Axis a takes the pairs section_end[a - 1] <= j <
+ * section_end[a] (section_end[axes - 1] == pairs).  positions holds one value per axis, batch item
+ * and token, pos_stride elements apart (0 = broadcast).  The angle is computed in 64 bits, so far
+ * positions keep their full precision; the products and the sum are fp32, rounded once. */
+typedef struct cmpx_rotation {
+  const void* positions;
+  const float* freqs;    /* [pairs] radians per position */
+  int64_t pos_stride[3]; /* axis, batch, token */
+  int32_t pos_kind;      /* cmpx_pos_kind */
+  int32_t pairs;         /* 0: no rotation */
+  int32_t axes;          /* 1 .. CMPX_ROPE_MAX_AXES */
+  int32_t interleaved;   /* 0 or 1 */
+  int32_t section_end[CMPX_ROPE_MAX_AXES];
+} cmpx_rotation;
+
+/* y = x turned (inverse = 1: by the negative angles, which is the gradient's rotation).
+ * x, y: [batch, heads, len, head_dim], head_dim <= 256, contiguous along head_dim, any strides
+ * otherwise (y's not 0 along a stepped dimension); y may be x. */
+typedef struct cmpx_rope_desc {
+  const void* x;
+  void* y;
+  int64_t batch, heads, len, head_dim;
+  int64_t x_stride[3]; /* batch, head, token (elements) */
+  int64_t y_stride[3];
+  cmpx_rotation rot;
+  int32_t dtype; /* cmpx_dtype */
+  int32_t inverse;
+} cmpx_rope_desc;
+
+CMPX_API int cmpx_rope(const cmpx_rope_desc* desc, void* stream);
+CMPX_API int cmpx_rope_plan(const cmpx_rope_desc* desc, char* buf, size_t buf_len);
+
+/* A paged key-value cache: k and v are [num_pages, heads_kv, page_size, head_dim] with any page,
+ * head and token strides (so [num_pages, page_size, heads_kv, head_dim] memory is a view of it) and
+ * a contiguous head_dim; rows start on 16-byte boundaries.  Token t of sequence b lies in page
+ * table[b * table_stride + t / page_size] at row t % page_size.  Entries behind a sequence's last
+ * page are never read. */
+typedef struct cmpx_paged_cache {
+  void* k;
+  void* v;
+  const int32_t* table;   /* [batch, table_width] */
+  const int32_t* lengths; /* [batch] tokens of each sequence, counting those appended by this step */
+  int64_t num_pages, page_size, heads_kv, head_dim;
+  int64_t k_stride[3];    /* page, head, token (elements) */
+  int64_t v_stride[3];
+  int64_t table_width, table_stride;
+} cmpx_paged_cache;
+
+/* Stores each sequence's new keys (turned, when rot.pairs > 0) and values in the cache, and writes
+ * the turned queries to q_out, in one launch.  k, v: [batch, heads_kv, len, head_dim]; q, q_out:
+ * [batch, heads, len, head_dim] or NULL with heads = 0.  Sequence b has new_lengths[b] new tokens (all
+ * len when NULL; values outside 0..len are clipped to it): its token i, i < new_lengths[b], goes to
+ * place lengths[b] - new_lengths[b] + i.  Rows i >= new_lengths[b] are padding: nothing is stored for
+ * them and q_out gets q as it is.  A token whose place is negative, behind the table, or in a page
+ * outside 0..num_pages-1 is not stored and raises CMPX_DEVFLAG_BAD_PAGE.  Two tokens of one call
+ * that share a slot (a page that two sequences both append to) leave either's values there. */
+typedef struct cmpx_kv_append_desc {
+  const void* k;
+  const void* v;
+  const void* q;
+  void* q_out;
+  const int32_t* new_lengths;
+  int64_t batch, heads, len;
+  int64_t k_in_stride[3]; /* batch, head, token (elements) */
+  int64_t v_in_stride[3];
+  int64_t q_stride[3];
+  int64_t q_out_stride[3];
+  cmpx_paged_cache cache;
+  cmpx_rotation rot;
+  int32_t dtype; /* cmpx_dtype, of the cache too */
+  int32_t reserved;
+} cmpx_kv_append_desc;
+
+CMPX_API int cmpx_kv_append(const cmpx_kv_append_desc* desc, void* stream);
+CMPX_API int cmpx_kv_append_plan(const cmpx_kv_append_desc* desc, char* buf, size_t buf_len);
+
+/* Attention of one query token per sequence over the paged cache:
+ *   o[b, h] = softmax(q[b, h] . K[b, h / (heads / heads_kv)] * scale) V,  keys 0 .. lengths[b] - 1.
+ * q, o: [batch, heads, head_dim], contiguous along head_dim, rows 16-byte aligned; head_dim <= 256,
+ * a multiple of 8 (fp32: 4).  A sequence of length 0 (or less) gets zeros.  A length beyond the table, or a page
+ * outside 0..num_pages-1 among a sequence's pages, makes that sequence's rows NaN and raises
+ * CMPX_DEVFLAG_BAD_PAGE; nothing outside the cache is read.
+ * The work is split over the sequences' lengths on the device (the lengths are read there, so a
+ * captured call serves any lengths); partial results go through the workspace
+ * (cmpx_paged_attn_workspace_size bytes, 16-byte aligned, no initial state, free again when the call's
+ * work is done) and are joined in a fixed order. */
+typedef struct cmpx_paged_attn_desc {
+  const void* q;
+  void* o;
+  int64_t batch, heads;
+  int64_t q_stride[2]; /* batch, head (elements) */
+  int64_t o_stride[2];
+  cmpx_paged_cache cache;
+  void* workspace;
+  size_t workspace_bytes;
+  double scale;
+  int32_t dtype; /* cmpx_dtype */
+  int32_t reserved;
+} cmpx_paged_attn_desc;
+
+CMPX_API size_t cmpx_paged_attn_workspace_size(const cmpx_paged_attn_desc* desc);
+CMPX_API int cmpx_paged_attn(const cmpx_paged_attn_desc* desc, void* stream);
+CMPX_API int cmpx_paged_attn_plan(const cmpx_paged_attn_desc* desc, char* buf, size_t buf_len);
+
+/* Linear layer with 4-bit weights for a few tokens:  y = x W^T (+ bias),
+ *   W[n, k] = (code[n, k] - zero[n, k / group]) * scale[n, k / group].
+ * w: [n, k / 2] bytes, two codes (0..15) a byte, the even k in the low half; scales [n, k / group] in
+ * x's type; zeros [n, k / group] bytes (0..15) or NULL (8).  group is a multiple of 32 and
+ * divides k.  The differences code - zero are exact in every type, their products with x are summed
+ * in fp32 and multiplied by the fp32 value of the scale group by group; the bias is added before the
+ * one rounding.  Rows of x and w start on 16-byte boundaries. */
+typedef struct cmpx_linear_w4_desc {
+  const void* x;
+  const uint8_t* w;
+  const void* scales;
+  const uint8_t* zeros; /* NULL: 8 */
+  const void* bias;     /* NULL: no bias */
+  void* y;
+  int64_t m, n, k, group;
+  int64_t x_row_stride, y_row_stride; /* elements */
+  int64_t w_row_stride;               /* bytes */
+  int64_t scales_row_stride, zeros_row_stride;
+  int32_t dtype; /* cmpx_dtype of x, scales, bias and y */
+  int32_t reserved;
+} cmpx_linear_w4_desc;
+
+CMPX_API int cmpx_linear_w4(const cmpx_linear_w4_desc* desc, void* stream);
+CMPX_API int cmpx_linear_w4_plan(const cmpx_linear_w4_desc* desc, char* buf, size_t buf_len);
+
 /* Name of the tile-table entry a call would use, written into buf (NUL-terminated).
  * Returns CMPX_OK or the status the call itself would return.  Replaces the per-signature
  * decision record of the reference's runtime autoselect (cmpext3/autoselect.py:290-364),
@@ -299,6 +450,7 @@ CMPX_API const char* cmpx_status_str(int status);
  * No reference counterpart (the reference's kernels have no bounded waits). */
 #define CMPX_DEVFLAG_WAIT_TIMEOUT 1u   /* an mbarrier / pipeline wait ran out */
 #define CMPX_DEVFLAG_BAD_ARGS 2u       /* a kernel rejected its own launch arguments */
+#define CMPX_DEVFLAG_BAD_PAGE 4u       /* a length or page number outside the paged cache */
 CMPX_API int cmpx_device_status(unsigned int* flags);
 
 /* Self-test of the bounded-wait path: launches one CTA that waits on an mbarrier nothing ever

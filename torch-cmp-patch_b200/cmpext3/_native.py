@@ -23,7 +23,8 @@ from pathlib import Path
 import torch
 
 __all__ = ["attention", "bmm", "attention_plan", "bmm_plan", "device_status", "LIBRARY_PATH",
-           "lib", "CmpxError"]
+           "lib", "CmpxError", "rope", "rope_plan", "kv_append", "kv_append_plan", "paged_attention",
+           "paged_attention_plan", "linear_w4", "linear_w4_plan"]
 
 LIBRARY_PATH = Path(os.environ.get("CMPX_LIBRARY", Path(__file__).with_name("libcmpx_b200.so")))
 
@@ -40,6 +41,7 @@ ERR_DEVICE_TIMEOUT = 8
 
 DEVFLAG_WAIT_TIMEOUT = 1
 DEVFLAG_BAD_ARGS = 2
+DEVFLAG_BAD_PAGE = 4
 
 _DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
@@ -771,3 +773,9 @@ def selftest_wait_timeout(timeout_ns: int, device=None) -> None:
         st = lib.cmpx_selftest_wait_timeout(int(timeout_ns), _stream_handle(dev))
     if st != OK:
         raise CmpxError("selftest", st)
+
+
+# The step of a served transformer (rotary positions, paged cache, 4-bit linear): bound in its own module,
+# which builds on this one.
+from ._serving import (kv_append, kv_append_plan, linear_w4, linear_w4_plan, paged_attention,  # noqa: E402
+                       paged_attention_plan, rope, rope_plan)

@@ -412,6 +412,82 @@ int cmpx_softmax_product_plan(const cmpx_bmm_desc* desc, const float* stats, con
   return st;
 }
 
+int cmpx_rope(const cmpx_rope_desc* desc, void* stream) {
+  int st = CMPX_OK;
+  rope_plan(desc, &st);
+  if (st != CMPX_OK) return st;
+  if (desc->batch == 0 || desc->heads == 0 || desc->len == 0) return CMPX_OK;
+  LaunchCtx ctx;
+  st = device_ctx(&ctx, static_cast<cudaStream_t>(stream));
+  if (st != CMPX_OK) return st;
+  return launch_rope(desc, ctx);
+}
+
+int cmpx_rope_plan(const cmpx_rope_desc* desc, char* buf, size_t buf_len) {
+  int st = CMPX_OK;
+  const char* name = rope_plan(desc, &st);
+  copy_name(st == CMPX_OK ? name : "none", buf, buf_len);
+  return st;
+}
+
+int cmpx_kv_append(const cmpx_kv_append_desc* desc, void* stream) {
+  int st = CMPX_OK;
+  kv_append_plan(desc, &st);
+  if (st != CMPX_OK) return st;
+  if (desc->batch == 0 || desc->len == 0) return CMPX_OK;
+  LaunchCtx ctx;
+  st = device_ctx(&ctx, static_cast<cudaStream_t>(stream));
+  if (st != CMPX_OK) return st;
+  return launch_kv_append(desc, ctx);
+}
+
+int cmpx_kv_append_plan(const cmpx_kv_append_desc* desc, char* buf, size_t buf_len) {
+  int st = CMPX_OK;
+  const char* name = kv_append_plan(desc, &st);
+  copy_name(st == CMPX_OK ? name : "none", buf, buf_len);
+  return st;
+}
+
+size_t cmpx_paged_attn_workspace_size(const cmpx_paged_attn_desc* desc) {
+  return paged_attn_workspace_bytes(desc, current_num_sms());
+}
+
+int cmpx_paged_attn(const cmpx_paged_attn_desc* desc, void* stream) {
+  int st = CMPX_OK;
+  paged_attn_plan(desc, &st);
+  if (st != CMPX_OK) return st;
+  if (desc->batch == 0 || desc->heads == 0) return CMPX_OK;
+  LaunchCtx ctx;
+  st = device_ctx(&ctx, static_cast<cudaStream_t>(stream));
+  if (st != CMPX_OK) return st;
+  return launch_paged_attn(desc, ctx);
+}
+
+int cmpx_paged_attn_plan(const cmpx_paged_attn_desc* desc, char* buf, size_t buf_len) {
+  int st = CMPX_OK;
+  const char* name = paged_attn_plan(desc, &st);
+  copy_name(st == CMPX_OK ? name : "none", buf, buf_len);
+  return st;
+}
+
+int cmpx_linear_w4(const cmpx_linear_w4_desc* desc, void* stream) {
+  int st = CMPX_OK;
+  linear_w4_plan(desc, &st);
+  if (st != CMPX_OK) return st;
+  if (desc->m == 0 || desc->n == 0) return CMPX_OK;
+  LaunchCtx ctx;
+  st = device_ctx(&ctx, static_cast<cudaStream_t>(stream));
+  if (st != CMPX_OK) return st;
+  return launch_linear_w4(desc, ctx);
+}
+
+int cmpx_linear_w4_plan(const cmpx_linear_w4_desc* desc, char* buf, size_t buf_len) {
+  int st = CMPX_OK;
+  const char* name = linear_w4_plan(desc, &st);
+  copy_name(st == CMPX_OK ? name : "none", buf, buf_len);
+  return st;
+}
+
 int cmpx_device_status(unsigned int* flags) {
   if (!flags) return CMPX_ERR_INVALID_ARGUMENT;
   LaunchCtx ctx;

@@ -98,6 +98,23 @@ int launch_bmm_rowstats(const cmpx_bmm_desc* d, float* stats, const LaunchCtx& c
 const char* softmax_product_plan(const cmpx_bmm_desc* d, const void* stats, const void* y, int* status);
 int launch_softmax_product(const cmpx_bmm_desc* d, const float* stats, void* y, const LaunchCtx& ctx);
 
+// ---- the step of a served transformer ----
+// Rotary positions and the append to a paged cache (one kernel).
+const char* rope_plan(const cmpx_rope_desc* d, int* status);
+int launch_rope(const cmpx_rope_desc* d, const LaunchCtx& ctx);
+const char* kv_append_plan(const cmpx_kv_append_desc* d, int* status);
+int launch_kv_append(const cmpx_kv_append_desc* d, const LaunchCtx& ctx);
+// The paged cache's own checks: arguments, then sizes and alignment (a status).
+bool paged_cache_ok(const cmpx_paged_cache& c, int64_t batch);
+int paged_cache_limits(const cmpx_paged_cache& c, int dtype);
+// Attention of one new token per sequence over the paged cache.
+const char* paged_attn_plan(const cmpx_paged_attn_desc* d, int* status);
+size_t paged_attn_workspace_bytes(const cmpx_paged_attn_desc* d, int num_sms);
+int launch_paged_attn(const cmpx_paged_attn_desc* d, const LaunchCtx& ctx);
+// Linear layer with 4-bit weights for a few tokens.
+const char* linear_w4_plan(const cmpx_linear_w4_desc* d, int* status);
+int launch_linear_w4(const cmpx_linear_w4_desc* d, const LaunchCtx& ctx);
+
 // ---- self test ----
 int launch_wait_selftest(uint64_t timeout_ns, const LaunchCtx& ctx);
 

@@ -1,0 +1,429 @@
+// paged_attn.cu -- attention of one new token per sequence over a paged key-value cache,
+// fp16 / bf16 / fp32, B200 sm_100a.
+//
+//   o[b, h] = sum_t p_t V[t] / sum_t p_t,   p_t = exp(q[b, h] . K[t] * scale - m),  t < lengths[b],
+// with the maximum m and both sums carried along (one pass over the keys).
+//
+// Each key and value is read once from memory for all the query heads that share it, and that read is the
+// whole cost: 4 flops per element of K or V and head.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "cmpx_internal.h"
+#include "paged_schedule.cuh"
+
+namespace cmpx {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kJoinThreads = 256;
+
+// Group of LPT lanes per key; a lane holds NV vectors of 4 values of the key's row.  Each lane group
+// runs its own online softmax over its keys; groups and warps are joined at the end of a stretch.
+template <int DT, int LPT, int HG>
+struct Ffma {
+  static constexpr int NV = 2;
+  static constexpr int KEYS = 32 / LPT;  // keys per warp and step
+  static constexpr int STEPS = 2;        // steps whose loads are issued together
+  static constexpr int VB = 4 * elt_size(DT);
+};
+
+template <int DT, int LPT, int HG>
+__global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_constant__ PagedArgs a) {
+  using C = Ffma<DT, LPT, HG>;
+  constexpr int NV = C::NV, KEYS = C::KEYS, STEPS = C::STEPS, VB = C::VB;
+  __shared__ int64_t scratch[36];
+  __shared__ float sm_ml[kWarps][HG][2];
+  extern __shared__ float sm_o[];  // [kWarps][HG][head_dim]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sub = lane % LPT, slot = lane / LPT;
+  pdl_allow_dependents();
+
+  Share share{};
+  bool more = true;
+  Stretch st;
+  if (a.whole_items) {
+    st = whole_item(a, blockIdx.x);
+  } else {
+    share = find_share(a, scratch);
+    more = next_stretch(a, share, st);
+  }
+  int col[NV];
+  bool in[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    col[i] = 4 * (sub + LPT * i);
+    in[i] = col[i] < a.head_dim;
+  }
+  while (more) {
+    float q[HG][NV][4], o[HG][NV][4], m[HG], l[HG];
+#pragma unroll
+    for (int h = 0; h < HG; ++h) {
+      m[h] = -INFINITY;
+      l[h] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[h][i][e] = o[h][i][e] = 0.f;
+        if (h < st.nh && in[i]) {
+          const uint8_t* p = a.q + st.b * a.q_sb + (st.h0 + h) * a.q_sh + col[i] * elt_size(DT);
+          unpack_vec<DT, VB>(*reinterpret_cast<const RawVec<VB>*>(p), q[h][i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[h][i][e] *= a.scale_log2;
+        }
+      }
+    }
+    bool bad = st.bad;
+    const int32_t* table = a.table + st.b * a.table_stride;
+    const uint8_t* kb = a.kc + st.kvh * a.kc_sh;
+    const uint8_t* vb = a.vc + st.kvh * a.vc_sh;
+    for (int t0 = st.key0 + warp * KEYS * STEPS; t0 < st.key1; t0 += kWarps * KEYS * STEPS) {
+      RawVec<VB> kr[STEPS][NV], vr[STEPS][NV];
+      bool valid[STEPS];
+#pragma unroll
+      for (int u = 0; u < STEPS; ++u) {
+        const int t = t0 + u * KEYS + slot;
+        valid[u] = t < st.key1;
+        int id = 0, row = 0;
+        if (valid[u]) {
+          const uint32_t page = fast_div(t, a.page);
+          row = t - page * a.page.d;
+          id = __ldg(table + page);
+          if (id < 0 || id >= a.num_pages) {
+            bad = true;
+            valid[u] = false;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          kr[u][i] = RawVec<VB>{};
+          vr[u][i] = RawVec<VB>{};
+          if (valid[u] && in[i]) {
+            kr[u][i] = *reinterpret_cast<const RawVec<VB>*>(kb + id * a.kc_sp + row * a.kc_st + col[i] * elt_size(DT));
+            vr[u][i] = *reinterpret_cast<const RawVec<VB>*>(vb + id * a.vc_sp + row * a.vc_st + col[i] * elt_size(DT));
+          }
+        }
+      }
+      float s[STEPS][HG];
+#pragma unroll
+      for (int u = 0; u < STEPS; ++u) {
+        float k[NV][4];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) unpack_vec<DT, VB>(kr[u][i], k[i]);
+#pragma unroll
+        for (int h = 0; h < HG; ++h) {
+          float x = 0.f;
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x = fmaf(q[h][i][e], k[i][e], x);
+#pragma unroll
+          for (int off = LPT / 2; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+          s[u][h] = valid[u] ? x : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < HG; ++h) {
+        float top = m[h];
+#pragma unroll
+        for (int u = 0; u < STEPS; ++u) top = fmaxf(top, s[u][h]);
+        const float base = top == -INFINITY ? 0.f : top;  // no key yet: exp2(-inf - 0) = 0
+        const float keep = ex2_approx(m[h] - base);
+        m[h] = top;
+        l[h] *= keep;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[h][i][e] *= keep;
+#pragma unroll
+        for (int u = 0; u < STEPS; ++u) {
+          s[u][h] = ex2_approx(s[u][h] - base);
+          l[h] += s[u][h];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < STEPS; ++u) {
+        float v[NV][4];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) unpack_vec<DT, VB>(vr[u][i], v[i]);
+#pragma unroll
+        for (int h = 0; h < HG; ++h)
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[h][i][e] = fmaf(s[u][h], v[i][e], o[h][i][e]);
+      }
+    }
+    // the warp's lane groups, then the warps
+    bad = __syncthreads_or(bad);
+    if (bad && threadIdx.x == 0) atomicOr(a.flags, CMPX_DEVFLAG_BAD_PAGE);
+#pragma unroll
+    for (int h = 0; h < HG; ++h) {
+#pragma unroll
+      for (int off = LPT; off < 32; off <<= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m[h], off);
+        const float top = fmaxf(m[h], m2), base = top == -INFINITY ? 0.f : top;
+        const float w1 = ex2_approx(m[h] - base), w2 = ex2_approx(m2 - base);
+        l[h] = l[h] * w1 + __shfl_xor_sync(0xffffffffu, l[h], off) * w2;
+        m[h] = top;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[h][i][e] = o[h][i][e] * w1 + __shfl_xor_sync(0xffffffffu, o[h][i][e], off) * w2;
+      }
+      if (lane == 0) {
+        sm_ml[warp][h][0] = m[h];
+        sm_ml[warp][h][1] = l[h];
+      }
+      if (slot == 0)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (in[i])
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sm_o[(warp * HG + h) * a.head_dim + col[i] + e] = o[h][i][e];
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < st.nh * a.head_dim; x += kThreads) {
+      const int h = x / a.head_dim, d = x - h * a.head_dim;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_ml[w][h][0]);
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, acc = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float weight = ex2_approx(sm_ml[w][h][0] - base);
+        sum = fmaf(weight, sm_ml[w][h][1], sum);
+        acc = fmaf(weight, sm_o[(w * HG + h) * a.head_dim + d], acc);
+      }
+      if (bad) sum = __int_as_float(0x7fffffff);
+      if (st.slot < 0) {
+        const float r = sum == 0.f ? 0.f : acc / sum;
+        constexpr int ES = elt_size(DT);
+        *reinterpret_cast<RawVec<ES>*>(a.o + st.b * a.o_sb + (st.h0 + h) * a.o_sh + d * ES) = pack_vec<DT, ES>(&r);
+      } else {
+        const int64_t row = st.slot * a.item_heads + h;
+        a.part_o[row * a.head_dim + d] = acc;
+        if (d == 0) {
+          a.part_ml[2 * row] = top;
+          a.part_ml[2 * row + 1] = sum;
+        }
+      }
+    }
+    if (a.whole_items) break;
+    more = next_stretch(a, share, st);
+    __syncthreads();
+  }
+}
+
+// Joins the partial results of one (sequence, query head): a block per row, a warp per partial result
+// in turn, lanes along the head.
+template <int DT>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a, int ctas) {
+  constexpr int W = kJoinThreads / 32, MAXV = 8;
+  constexpr int ES = elt_size(DT);
+  __shared__ int64_t scratch[36];
+  __shared__ float sm_ml[W][2];
+  __shared__ float sm_o[W][256];
+  const int b = blockIdx.x / a.heads, h = blockIdx.x - b * a.heads;
+  const int64_t items = static_cast<int64_t>(a.heads_kv) * a.items_per_head;
+  int64_t first = 0, rest = 0, unused;
+  for (int i = threadIdx.x; i < a.batch; i += kJoinThreads) {
+    const int64_t n = seq_tiles(a, i) * items;
+    (i < b ? first : rest) += n;
+  }
+  first = block_scan(first, scratch, &unused);
+  const int64_t total = first + block_scan(rest, scratch, &unused);
+  const int64_t share = share_tiles(total, ctas);
+  const int tiles = seq_tiles(a, b);
+  const int kvh = h / a.group, g = h - kvh * a.group, part = g / a.item_heads;
+  const int64_t begin = first + (static_cast<int64_t>(kvh) * a.items_per_head + part) * tiles;
+  const int64_t c0 = begin / share, c1 = (begin + tiles - 1) / share;
+  pdl_wait();  // every block: this kernel is not done before the main one is
+  if (c0 == c1) return;  // written by its CTA
+  const int hh = g - part * a.item_heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float m = -INFINITY, l = 0.f, o[MAXV];
+#pragma unroll
+  for (int i = 0; i < MAXV; ++i) o[i] = 0.f;
+  for (int64_t c = c0 + warp; c <= c1; c += W) {
+    const int64_t row = (2 * c + (c == c0 ? 1 : 0)) * a.item_heads + hh;
+    const float m2 = __ldcg(a.part_ml + 2 * row), l2 = __ldcg(a.part_ml + 2 * row + 1);
+    float p[MAXV];
+#pragma unroll
+    for (int i = 0; i < MAXV; ++i)
+      p[i] = lane + 32 * i < a.head_dim ? __ldcg(a.part_o + row * a.head_dim + lane + 32 * i) : 0.f;
+    const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
+    const float w1 = ex2_approx(m - base), w2 = ex2_approx(m2 - base);
+    m = top;
+    l = l * w1 + l2 * w2;
+#pragma unroll
+    for (int i = 0; i < MAXV; ++i) o[i] = o[i] * w1 + p[i] * w2;
+  }
+  if (lane == 0) {
+    sm_ml[warp][0] = m;
+    sm_ml[warp][1] = l;
+  }
+#pragma unroll
+  for (int i = 0; i < MAXV; ++i)
+    if (lane + 32 * i < a.head_dim) sm_o[warp][lane + 32 * i] = o[i];
+  __syncthreads();
+  for (int d = threadIdx.x; d < a.head_dim; d += kJoinThreads) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) top = fmaxf(top, sm_ml[w][0]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float weight = ex2_approx(sm_ml[w][0] - base);
+      sum = fmaf(weight, sm_ml[w][1], sum);
+      acc = fmaf(weight, sm_o[w][d], acc);
+    }
+    const float r = sum == 0.f ? 0.f : acc / sum;
+    *reinterpret_cast<RawVec<ES>*>(a.o + b * a.o_sb + h * a.o_sh + d * ES) = pack_vec<DT, ES>(&r);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------
+
+struct Schedule {
+  int item_heads, items_per_head;
+  int64_t items;
+  bool whole_items;
+  int ctas;
+};
+
+constexpr int kCtasPerSm = 2;
+
+Schedule schedule(const cmpx_paged_attn_desc* d, int num_sms) {
+  Schedule s;
+  const int64_t group = d->heads / d->cache.heads_kv;
+  s.item_heads = group == 1 ? 1 : 4;
+  s.items_per_head = static_cast<int>((group + s.item_heads - 1) / s.item_heads);
+  s.items = d->batch * d->cache.heads_kv * s.items_per_head;
+  // No table longer than a CTA's least share: one CTA per item, no join.
+  const int64_t most = std::max<int64_t>(1, (d->cache.table_width * d->cache.page_size + kTile - 1) / kTile);
+  s.whole_items = most <= kShareMin;
+  const int64_t tiles = s.items * most;
+  s.ctas = static_cast<int>(s.whole_items
+                                ? s.items
+                                : std::max<int64_t>(1, std::min<int64_t>(static_cast<int64_t>(kCtasPerSm) * num_sms,
+                                                                         (tiles + kShareMin - 1) / kShareMin)));
+  return s;
+}
+
+size_t part_floats(const cmpx_paged_attn_desc* d, const Schedule& s) {
+  return s.whole_items ? 0 : 2ull * s.ctas * s.item_heads * (d->cache.head_dim + 2);
+}
+
+template <int DT, int LPT, int HG>
+int launch_main(const PagedArgs& a, int ctas, const LaunchCtx& ctx) {
+  const int smem = kWarps * HG * a.head_dim * static_cast<int>(sizeof(float));
+  paged_attn_kernel<DT, LPT, HG><<<ctas, kThreads, smem, ctx.stream>>>(a);
+  return cudaGetLastError() == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
+}
+
+template <int DT>
+int launch_dt(const PagedArgs& a, int ctas, const LaunchCtx& ctx) {
+  const int vectors = (a.head_dim + 3) / 4;
+#define CMPX_PAGED(LPT) (a.item_heads == 1 ? launch_main<DT, LPT, 1>(a, ctas, ctx) : launch_main<DT, LPT, 4>(a, ctas, ctx))
+  const int st = vectors <= 16 ? CMPX_PAGED(8) : vectors <= 32 ? CMPX_PAGED(16) : CMPX_PAGED(32);
+#undef CMPX_PAGED
+  if (st != CMPX_OK || a.whole_items) return st;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.heads));
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = ctx.stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<DT>, a, ctas) == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
+}
+
+}  // namespace
+
+const char* paged_attn_plan(const cmpx_paged_attn_desc* d, int* status) {
+  *status = CMPX_ERR_INVALID_ARGUMENT;
+  if (!d || !d->q || !d->o || d->batch < 0 || d->heads < 0 || !std::isfinite(d->scale)) return "none";
+  if (!paged_cache_ok(d->cache, d->batch) || d->heads % d->cache.heads_kv != 0) return "none";
+  *status = CMPX_ERR_UNSUPPORTED_DTYPE;
+  if (d->dtype != CMPX_F32 && d->dtype != CMPX_F16 && d->dtype != CMPX_BF16) return "none";
+  *status = paged_cache_limits(d->cache, d->dtype);
+  if (*status != CMPX_OK) return "none";
+  const int64_t es = elt_size(d->dtype);
+  *status = CMPX_ERR_MISALIGNED;
+  if (reinterpret_cast<uintptr_t>(d->q) % 16 || reinterpret_cast<uintptr_t>(d->o) % 16) return "none";
+  for (int i = 0; i < 2; ++i)
+    if ((d->q_stride[i] * es) % 16 || (d->o_stride[i] * es) % 16) return "none";
+  *status = CMPX_ERR_UNSUPPORTED_SHAPE;
+  if (d->heads > (1 << 20) || d->batch > (1 << 20) || d->batch * d->heads > (1ll << 31) - 65536) return "none";
+  *status = CMPX_OK;
+  return schedule(d, 148).whole_items ? "paged_attn<one CTA per item>" : "paged_attn<equal shares, join>";
+}
+
+size_t paged_attn_workspace_bytes(const cmpx_paged_attn_desc* d, int num_sms) {
+  int st;
+  paged_attn_plan(d, &st);
+  if (st != CMPX_OK || d->batch == 0 || d->heads == 0) return 0;
+  return part_floats(d, schedule(d, num_sms)) * sizeof(float);
+}
+
+int launch_paged_attn(const cmpx_paged_attn_desc* d, const LaunchCtx& ctx) {
+  const int es = elt_size(d->dtype);
+  const cmpx_paged_cache& c = d->cache;
+  const Schedule s = schedule(d, ctx.num_sms);
+  const size_t floats = part_floats(d, s);
+  if (floats && (!d->workspace || d->workspace_bytes < floats * sizeof(float) ||
+                 reinterpret_cast<uintptr_t>(d->workspace) % 16 != 0))
+    return CMPX_ERR_WORKSPACE;
+  PagedArgs a{};
+  a.q = static_cast<const uint8_t*>(d->q);
+  a.o = static_cast<uint8_t*>(d->o);
+  a.q_sb = d->q_stride[0] * es;
+  a.q_sh = d->q_stride[1] * es;
+  a.o_sb = d->o_stride[0] * es;
+  a.o_sh = d->o_stride[1] * es;
+  a.kc = static_cast<const uint8_t*>(c.k);
+  a.vc = static_cast<const uint8_t*>(c.v);
+  a.kc_sp = c.k_stride[0] * es;
+  a.kc_sh = c.k_stride[1] * es;
+  a.kc_st = c.k_stride[2] * es;
+  a.vc_sp = c.v_stride[0] * es;
+  a.vc_sh = c.v_stride[1] * es;
+  a.vc_st = c.v_stride[2] * es;
+  a.table = c.table;
+  a.lengths = c.lengths;
+  a.table_stride = c.table_stride;
+  a.capacity = static_cast<int>(c.table_width * c.page_size);
+  a.num_pages = static_cast<int>(c.num_pages);
+  a.page = make_fast_div(static_cast<uint32_t>(c.page_size));
+  a.batch = static_cast<int>(d->batch);
+  a.heads = static_cast<int>(d->heads);
+  a.heads_kv = static_cast<int>(c.heads_kv);
+  a.group = a.heads / a.heads_kv;
+  a.item_heads = s.item_heads;
+  a.items_per_head = s.items_per_head;
+  a.head_dim = static_cast<int>(c.head_dim);
+  a.scale_log2 = static_cast<float>(d->scale * 1.4426950408889634074);
+  a.whole_items = s.whole_items ? 1 : 0;
+  a.flags = ctx.dev_flags;
+  if (floats) {
+    a.part_o = static_cast<float*>(d->workspace);
+    a.part_ml = a.part_o + 2ull * s.ctas * s.item_heads * c.head_dim;
+  }
+  if (d->dtype == CMPX_F32) return launch_dt<CMPX_F32>(a, s.ctas, ctx);
+  if (d->dtype == CMPX_F16) return launch_dt<CMPX_F16>(a, s.ctas, ctx);
+  return launch_dt<CMPX_BF16>(a, s.ctas, ctx);
+}
+
+}  // namespace cmpx
