@@ -1,5 +1,5 @@
-// paged_attn.cu -- attention of one new token per sequence over a paged key-value cache,
-// fp16 / bf16 / fp32, B200 sm_100a.
+// paged_attn.cu -- attention of one new token per sequence over a paged key-value cache, B200 sm_100a:
+// the choice of schedule, the fp32 kernel over the keys (fp16 / bf16: paged_attn_mma.cu) and the join.
 //
 //   o[b, h] = sum_t p_t V[t] / sum_t p_t,   p_t = exp(q[b, h] . K[t] * scale - m),  t < lengths[b],
 // with the maximum m and both sums carried along (one pass over the keys).
@@ -23,20 +23,22 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kJoinThreads = 256;
 
 // Group of LPT lanes per key; a lane holds NV vectors of 4 values of the key's row.  Each lane group
-// runs its own online softmax over its keys; groups and warps are joined at the end of a stretch.
-template <int DT, int LPT, int HG>
+// runs its own online softmax over its keys; the groups are joined at the end of a stretch, and with
+// WHOLE (a CTA per item, its keys shared by the warps) the warps, too.
+template <int LPT, int HG>
 struct Ffma {
   static constexpr int NV = 2;
   static constexpr int KEYS = 32 / LPT;  // keys per warp and step
   static constexpr int STEPS = 2;        // steps whose loads are issued together
-  static constexpr int VB = 4 * elt_size(DT);
+  static constexpr int VB = 16;
 };
 
-template <int DT, int LPT, int HG>
+template <int LPT, int HG, bool WHOLE>
 __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_constant__ PagedArgs a) {
-  using C = Ffma<DT, LPT, HG>;
+  using C = Ffma<LPT, HG>;
+  constexpr int DT = CMPX_F32;
   constexpr int NV = C::NV, KEYS = C::KEYS, STEPS = C::STEPS, VB = C::VB;
-  __shared__ int64_t scratch[36];
+  __shared__ int64_t scratch[33 + 2 * kWarps];
   __shared__ float sm_ml[kWarps][HG][2];
   extern __shared__ float sm_o[];  // [kWarps][HG][head_dim]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -46,12 +48,13 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
   Share share{};
   bool more = true;
   Stretch st;
-  if (a.whole_items) {
+  if (WHOLE) {
     st = whole_item(a, blockIdx.x);
   } else {
-    share = find_share(a, scratch);
+    share = find_share<kWarps>(a, scratch);
     more = next_stretch(a, share, st);
   }
+  constexpr int kStep = (WHOLE ? kWarps : 1) * KEYS * STEPS;
   int col[NV];
   bool in[NV];
 #pragma unroll
@@ -81,7 +84,7 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
     const int32_t* table = a.table + st.b * a.table_stride;
     const uint8_t* kb = a.kc + st.kvh * a.kc_sh;
     const uint8_t* vb = a.vc + st.kvh * a.vc_sh;
-    for (int t0 = st.key0 + warp * KEYS * STEPS; t0 < st.key1; t0 += kWarps * KEYS * STEPS) {
+    for (int t0 = st.key0 + (WHOLE ? warp * KEYS * STEPS : 0); t0 < st.key1; t0 += kStep) {
       RawVec<VB> kr[STEPS][NV], vr[STEPS][NV];
       bool valid[STEPS];
 #pragma unroll
@@ -158,9 +161,6 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
             for (int e = 0; e < 4; ++e) o[h][i][e] = fmaf(s[u][h], v[i][e], o[h][i][e]);
       }
     }
-    // the warp's lane groups, then the warps
-    bad = __syncthreads_or(bad);
-    if (bad && threadIdx.x == 0) atomicOr(a.flags, CMPX_DEVFLAG_BAD_PAGE);
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
 #pragma unroll
@@ -176,76 +176,85 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
           for (int e = 0; e < 4; ++e)
             o[h][i][e] = o[h][i][e] * w1 + __shfl_xor_sync(0xffffffffu, o[h][i][e], off) * w2;
       }
-      if (lane == 0) {
-        sm_ml[warp][h][0] = m[h];
-        sm_ml[warp][h][1] = l[h];
-      }
-      if (slot == 0)
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (in[i])
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sm_o[(warp * HG + h) * a.head_dim + col[i] + e] = o[h][i][e];
     }
-    __syncthreads();
-    for (int x = threadIdx.x; x < st.nh * a.head_dim; x += kThreads) {
-      const int h = x / a.head_dim, d = x - h * a.head_dim;
-      float top = -INFINITY;
+    if constexpr (WHOLE) {
+      bad = __syncthreads_or(bad);
+      if (bad && threadIdx.x == 0) atomicOr(a.flags, CMPX_DEVFLAG_BAD_PAGE);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_ml[w][h][0]);
-      const float base = top == -INFINITY ? 0.f : top;
-      float sum = 0.f, acc = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float weight = ex2_approx(sm_ml[w][h][0] - base);
-        sum = fmaf(weight, sm_ml[w][h][1], sum);
-        acc = fmaf(weight, sm_o[(w * HG + h) * a.head_dim + d], acc);
-      }
-      if (bad) sum = __int_as_float(0x7fffffff);
-      if (st.slot < 0) {
-        const float r = sum == 0.f ? 0.f : acc / sum;
-        constexpr int ES = elt_size(DT);
-        *reinterpret_cast<RawVec<ES>*>(a.o + st.b * a.o_sb + (st.h0 + h) * a.o_sh + d * ES) = pack_vec<DT, ES>(&r);
-      } else {
-        const int64_t row = st.slot * a.item_heads + h;
-        a.part_o[row * a.head_dim + d] = acc;
-        if (d == 0) {
-          a.part_ml[2 * row] = top;
-          a.part_ml[2 * row + 1] = sum;
+      for (int h = 0; h < HG; ++h) {
+        if (lane == 0) {
+          sm_ml[warp][h][0] = m[h];
+          sm_ml[warp][h][1] = l[h];
         }
+        if (slot == 0)
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+            if (in[i])
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sm_o[(warp * HG + h) * a.head_dim + col[i] + e] = o[h][i][e];
+      }
+      __syncthreads();
+      for (int x = threadIdx.x; x < st.nh * a.head_dim; x += kThreads) {
+        const int h = x / a.head_dim, d = x - h * a.head_dim;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_ml[w][h][0]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, acc = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float weight = ex2_approx(sm_ml[w][h][0] - base);
+          sum = fmaf(weight, sm_ml[w][h][1], sum);
+          acc = fmaf(weight, sm_o[(w * HG + h) * a.head_dim + d], acc);
+        }
+        if (bad) sum = __int_as_float(0x7fffffff);
+        *reinterpret_cast<float*>(a.o + st.b * a.o_sb + (st.h0 + h) * a.o_sh + d * 4) = sum == 0.f ? 0.f : acc / sum;
+      }
+      break;
+    }
+    bad = __any_sync(0xffffffffu, bad);
+    if (bad && lane == 0) atomicOr(a.flags, CMPX_DEVFLAG_BAD_PAGE);
+#pragma unroll
+    for (int h = 0; h < HG; ++h) {
+      if (h >= st.nh || slot != 0) continue;
+      const float sum = bad ? __int_as_float(0x7fffffff) : l[h];
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int64_t row = st.slot * a.item_heads + h;
+      if (st.slot >= 0 && sub == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * row) = make_float2(m[h], sum);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (!in[i]) continue;
+        float* p = st.slot < 0 ? reinterpret_cast<float*>(a.o + st.b * a.o_sb + (st.h0 + h) * a.o_sh) + col[i]
+                               : a.part_o + row * a.head_dim + col[i];
+        const float f = st.slot < 0 ? inv : 1.f;
+        *reinterpret_cast<float4*>(p) = make_float4(o[h][i][0] * f, o[h][i][1] * f, o[h][i][2] * f, o[h][i][3] * f);
       }
     }
-    if (a.whole_items) break;
     more = next_stretch(a, share, st);
-    __syncthreads();
   }
 }
 
 // Joins the partial results of one (sequence, query head): a block per row, a warp per partial result
 // in turn, lanes along the head.
 template <int DT>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a, int ctas) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a) {
   constexpr int W = kJoinThreads / 32, MAXV = 8;
   constexpr int ES = elt_size(DT);
   __shared__ int64_t scratch[36];
   __shared__ float sm_ml[W][2];
   __shared__ float sm_o[W][256];
   const int b = blockIdx.x / a.heads, h = blockIdx.x - b * a.heads;
-  const int64_t items = static_cast<int64_t>(a.heads_kv) * a.items_per_head;
   int64_t first = 0, rest = 0, unused;
-  for (int i = threadIdx.x; i < a.batch; i += kJoinThreads) {
-    const int64_t n = seq_tiles(a, i) * items;
-    (i < b ? first : rest) += n;
-  }
+  for (int i = threadIdx.x; i < a.batch; i += kJoinThreads) (i < b ? first : rest) += seq_units(a, i);
   first = block_scan(first, scratch, &unused);
   const int64_t total = first + block_scan(rest, scratch, &unused);
-  const int64_t share = share_tiles(total, ctas);
+  const int64_t share = share_units(total, a.workers);
   const int tiles = seq_tiles(a, b);
   const int kvh = h / a.group, g = h - kvh * a.group, part = g / a.item_heads;
-  const int64_t begin = first + (static_cast<int64_t>(kvh) * a.items_per_head + part) * tiles;
+  const int64_t begin = first + (static_cast<int64_t>(kvh) * a.items_per_head + part) * (tiles + kItemCost) + kItemCost;
   const int64_t c0 = begin / share, c1 = (begin + tiles - 1) / share;
   pdl_wait();  // every block: this kernel is not done before the main one is
-  if (c0 == c1) return;  // written by its CTA
+  if (c0 == c1) return;  // written by its warp
   const int hh = g - part * a.item_heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float m = -INFINITY, l = 0.f, o[MAXV];
@@ -297,47 +306,55 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
 struct Schedule {
   int item_heads, items_per_head;
   int64_t items;
-  bool whole_items;
+  bool whole_items;  // a CTA per item, no join
   int ctas;
+  int64_t workers;
 };
 
-constexpr int kCtasPerSm = 2;
+constexpr int kF32CtasPerSm = 2;
+constexpr int kWholeKeys = 256;  // longest table of which a CTA takes an item alone
 
 Schedule schedule(const cmpx_paged_attn_desc* d, int num_sms) {
   Schedule s;
-  const int64_t group = d->heads / d->cache.heads_kv;
-  s.item_heads = group == 1 ? 1 : 4;
-  s.items_per_head = static_cast<int>((group + s.item_heads - 1) / s.item_heads);
+  const bool f32 = d->dtype == CMPX_F32;
+  const int64_t group = d->heads / d->cache.heads_kv, most_heads = f32 ? 4 : 16;
+  // the fewest items of at most most_heads heads, and their heads shared out evenly
+  s.items_per_head = static_cast<int>(std::max<int64_t>(1, (group + most_heads - 1) / most_heads));
+  s.item_heads = static_cast<int>((group + s.items_per_head - 1) / s.items_per_head);
   s.items = d->batch * d->cache.heads_kv * s.items_per_head;
-  // No table longer than a CTA's least share: one CTA per item, no join.
-  const int64_t most = std::max<int64_t>(1, (d->cache.table_width * d->cache.page_size + kTile - 1) / kTile);
-  s.whole_items = most <= kShareMin;
-  const int64_t tiles = s.items * most;
-  s.ctas = static_cast<int>(s.whole_items
-                                ? s.items
-                                : std::max<int64_t>(1, std::min<int64_t>(static_cast<int64_t>(kCtasPerSm) * num_sms,
-                                                                         (tiles + kShareMin - 1) / kShareMin)));
+  const int64_t keys = d->cache.table_width * d->cache.page_size;
+  s.whole_items = keys <= kWholeKeys;
+  const int64_t slots = static_cast<int64_t>(num_sms) * (f32 ? kF32CtasPerSm : paged_mma_ctas_per_sm(d->cache.head_dim));
+  const int64_t units = s.items * (std::max<int64_t>(1, (keys + kTile - 1) / kTile) + kItemCost);
+  s.ctas = static_cast<int>(s.whole_items ? s.items
+                                          : std::max<int64_t>(1, std::min(slots, (units + kShareMin - 1) / kShareMin)));
+  s.workers = static_cast<int64_t>(s.ctas) * (f32 ? kWarps : kPagedMmaWarps);
   return s;
 }
 
 size_t part_floats(const cmpx_paged_attn_desc* d, const Schedule& s) {
-  return s.whole_items ? 0 : 2ull * s.ctas * s.item_heads * (d->cache.head_dim + 2);
+  return s.whole_items ? 0 : 2ull * s.workers * s.item_heads * (d->cache.head_dim + 2);
 }
 
-template <int DT, int LPT, int HG>
-int launch_main(const PagedArgs& a, int ctas, const LaunchCtx& ctx) {
+template <int LPT, int HG>
+int launch_f32(const PagedArgs& a, int ctas, bool whole_items, const LaunchCtx& ctx) {
   const int smem = kWarps * HG * a.head_dim * static_cast<int>(sizeof(float));
-  paged_attn_kernel<DT, LPT, HG><<<ctas, kThreads, smem, ctx.stream>>>(a);
+  if (whole_items)
+    paged_attn_kernel<LPT, HG, true><<<ctas, kThreads, smem, ctx.stream>>>(a);
+  else
+    paged_attn_kernel<LPT, HG, false><<<ctas, kThreads, 0, ctx.stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
 }
 
-template <int DT>
-int launch_dt(const PagedArgs& a, int ctas, const LaunchCtx& ctx) {
-  const int vectors = (a.head_dim + 3) / 4;
-#define CMPX_PAGED(LPT) (a.item_heads == 1 ? launch_main<DT, LPT, 1>(a, ctas, ctx) : launch_main<DT, LPT, 4>(a, ctas, ctx))
-  const int st = vectors <= 16 ? CMPX_PAGED(8) : vectors <= 32 ? CMPX_PAGED(16) : CMPX_PAGED(32);
+int launch_f32(const PagedArgs& a, int ctas, bool whole, const LaunchCtx& ctx) {
+#define CMPX_PAGED(LPT) \
+  (a.item_heads == 1 ? launch_f32<LPT, 1>(a, ctas, whole, ctx) : launch_f32<LPT, 4>(a, ctas, whole, ctx))
+  return a.head_dim <= 64 ? CMPX_PAGED(8) : a.head_dim <= 128 ? CMPX_PAGED(16) : CMPX_PAGED(32);
 #undef CMPX_PAGED
-  if (st != CMPX_OK || a.whole_items) return st;
+}
+
+template <int DT>
+int launch_join(const PagedArgs& a, const LaunchCtx& ctx) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.heads));
   cfg.blockDim = dim3(kJoinThreads);
@@ -347,7 +364,7 @@ int launch_dt(const PagedArgs& a, int ctas, const LaunchCtx& ctx) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<DT>, a, ctas) == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<DT>, a) == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -415,15 +432,18 @@ int launch_paged_attn(const cmpx_paged_attn_desc* d, const LaunchCtx& ctx) {
   a.items_per_head = s.items_per_head;
   a.head_dim = static_cast<int>(c.head_dim);
   a.scale_log2 = static_cast<float>(d->scale * 1.4426950408889634074);
-  a.whole_items = s.whole_items ? 1 : 0;
+  a.workers = s.workers;
   a.flags = ctx.dev_flags;
   if (floats) {
     a.part_o = static_cast<float*>(d->workspace);
-    a.part_ml = a.part_o + 2ull * s.ctas * s.item_heads * c.head_dim;
+    a.part_ml = a.part_o + 2ull * s.workers * s.item_heads * c.head_dim;
   }
-  if (d->dtype == CMPX_F32) return launch_dt<CMPX_F32>(a, s.ctas, ctx);
-  if (d->dtype == CMPX_F16) return launch_dt<CMPX_F16>(a, s.ctas, ctx);
-  return launch_dt<CMPX_BF16>(a, s.ctas, ctx);
+  const int st = d->dtype == CMPX_F32 ? launch_f32(a, s.ctas, s.whole_items, ctx)
+                                        : launch_paged_mma(a, d->dtype, s.ctas, s.whole_items, ctx);
+  if (st != CMPX_OK || s.whole_items) return st;
+  if (d->dtype == CMPX_F32) return launch_join<CMPX_F32>(a, ctx);
+  if (d->dtype == CMPX_F16) return launch_join<CMPX_F16>(a, ctx);
+  return launch_join<CMPX_BF16>(a, ctx);
 }
 
 }  // namespace cmpx

@@ -1,16 +1,16 @@
 // paged_schedule.cuh -- how the one-token attention over a paged cache is cut into equal shares, and
-// what its kernels share: arguments, the walk over a share, and the partial results' places.
+// what its kernels have in common: arguments, the walk over a share, and the partial results' places.
 //
-// An item is one sequence's keys for one group of query heads that share a key head.  Items are
-// cut into tiles of kTile keys and laid end to end (sequence, then item in the sequence); an empty
-// sequence counts one tile, so that somebody writes its zeros.  CTA c takes the tiles
-// [c * share, (c + 1) * share), whatever items they belong to: every CTA has the same work, whether
-// the lengths are alike or one sequence is a thousand times as long as the others, and the lengths
-// are only read on the device.  A CTA that has all of an item writes its output; otherwise
-// it leaves a partial result (running maximum, sum and unnormalised output) in the workspace: slot
-// 2c for an item that began before the CTA's share, slot 2c + 1 for one that begins in it.  The join
-// kernel finds an item's slots by the same arithmetic and adds them in the order of the CTAs, so the
-// result does not depend on timing.
+// An item is one sequence's keys for one group of query heads that share a key head.  Its keys are
+// cut into tiles of kTile; an empty sequence counts one tile, so that somebody writes its zeros.  All items
+// laid end to end, each with kItemCost units before its tiles for what an item costs whatever its
+// length (the first loads' latency, the output), are cut into equal shares, one per warp: every
+// warp has the same work, whether the lengths are alike or one sequence is a thousand times as long as
+// the others, and the lengths are only read on the device.  A warp that has all of an item writes
+// its output; otherwise it leaves a partial result (running maximum, sum and unnormalised output) in the
+// workspace: slot 2w for an item that began before warp w's share, slot 2w + 1 for one that begins in
+// it.  The join kernel finds an item's slots by the same arithmetic and adds them in a fixed order, so
+// the result does not depend on timing.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -20,8 +20,9 @@
 
 namespace cmpx {
 
-constexpr int kTile = 64;        // keys per tile
-constexpr int kShareMin = 2;     // tiles per CTA at least, where there are more CTAs than work
+constexpr int kTile = 16;      // keys per tile
+constexpr int kItemCost = 2;   // an item's fixed cost, in tiles
+constexpr int kShareMin = 6;   // units per warp at least, where there are more warps than work
 
 struct PagedArgs {
   const uint8_t* q;
@@ -38,7 +39,7 @@ struct PagedArgs {
   int item_heads, items_per_head;     // query heads per item, items per key head
   int head_dim;
   float scale_log2;      // softmax scale * log2(e)
-  int whole_items;       // 1: CTA c has item c and there is no join
+  int64_t workers;       // warps that have shares
   float* part_o;         // [slot][item_heads][head_dim]
   float* part_ml;        // [slot][item_heads][2]: maximum (in log2 units), sum
   unsigned int* flags;
@@ -79,43 +80,55 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* scratch, int64
   return total;
 }
 
-// A CTA's share: tiles [cur, end) and the sequence that cur lies in, with the tiles before it.
+// A warp's share: units [cur, end), the sequence that cur lies in and the units before that sequence.
 struct Share {
-  int64_t cur, end, before;
+  int64_t cur, end, before, slot;
   int b;
 };
 
-__device__ __forceinline__ int64_t share_tiles(int64_t total, int ctas) {
-  const int64_t s = (total + ctas - 1) / ctas;
+__device__ __forceinline__ int64_t share_units(int64_t total, int64_t workers) {
+  const int64_t s = (total + workers - 1) / workers;
   return s < kShareMin ? kShareMin : s;
 }
+__device__ __forceinline__ int64_t seq_units(const PagedArgs& a, int b) {
+  return static_cast<int64_t>(seq_tiles(a, b) + kItemCost) * (a.heads_kv * a.items_per_head);
+}
 
-// Finds CTA blockIdx.x's share.  scratch: 33 + 2 values of shared memory.
+// The share of this warp: worker warp * gridDim.x + blockIdx.x, so that little work spreads over the CTAs
+// first.  scratch: 33 + 2 WARPS values of shared memory.
+template <int WARPS>
 __device__ __forceinline__ Share find_share(const PagedArgs& a, int64_t* scratch) {
   const int per = (a.batch + blockDim.x - 1) / blockDim.x;  // sequences per thread
-  const int64_t items = static_cast<int64_t>(a.heads_kv) * a.items_per_head;
-  const int b0 = threadIdx.x * per, b1 = min(a.batch, b0 + per);
+  const int b0 = min(a.batch, static_cast<int>(threadIdx.x) * per), b1 = min(a.batch, b0 + per);
   int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += seq_tiles(a, b) * items;
+  for (int b = b0; b < b1; ++b) mine += seq_units(a, b);
   int64_t before;
   const int64_t total = block_scan(mine, scratch, &before);
-  const int64_t share = share_tiles(total, gridDim.x);
-  Share s;
-  s.cur = blockIdx.x * share;
-  s.end = min(total, s.cur + share);
-  if (s.cur >= before && s.cur < before + mine) {
-    int b = b0;
-    for (; b < b1 - 1; ++b) {
-      const int64_t n = seq_tiles(a, b) * items;
-      if (s.cur < before + n) break;
-      before += n;
+  const int64_t share = share_units(total, a.workers);
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    const int64_t cur = (static_cast<int64_t>(w) * gridDim.x + blockIdx.x) * share;
+    if (cur >= before && cur < before + mine) {
+      int64_t at = before;
+      int b = b0;
+      for (; b < b1 - 1; ++b) {
+        const int64_t n = seq_units(a, b);
+        if (cur < at + n) break;
+        at += n;
+      }
+      scratch[33 + 2 * w] = at;
+      scratch[34 + 2 * w] = b;
     }
-    scratch[33] = before;
-    scratch[34] = b;
   }
   __syncthreads();
-  s.before = scratch[33];
-  s.b = static_cast<int>(scratch[34]);
+  const int warp = threadIdx.x >> 5;
+  const int64_t worker = static_cast<int64_t>(warp) * gridDim.x + blockIdx.x;
+  Share s;
+  s.cur = worker * share;
+  s.end = min(total, s.cur + share);
+  s.slot = 2 * worker;
+  s.before = scratch[33 + 2 * warp];
+  s.b = static_cast<int>(scratch[34 + 2 * warp]);
   return s;
 }
 
@@ -134,30 +147,35 @@ __device__ __forceinline__ void stretch_heads(const PagedArgs& a, int item, Stre
   st.nh = min(a.item_heads, a.group - g);
 }
 
-// The stretch that begins at s.cur; moves s behind it.  False when the share is done.
+// The next stretch of s; moves s behind it.  False when the share is done.
 __device__ __forceinline__ bool next_stretch(const PagedArgs& a, Share& s, Stretch& st) {
-  if (s.cur >= s.end) return false;
-  const int64_t items = static_cast<int64_t>(a.heads_kv) * a.items_per_head;
-  int tiles = seq_tiles(a, s.b);
-  while (s.cur >= s.before + tiles * items) {
-    s.before += tiles * items;
-    tiles = seq_tiles(a, ++s.b);
+  const int items = a.heads_kv * a.items_per_head;
+  while (s.cur < s.end) {
+    int units = seq_tiles(a, s.b) + kItemCost;
+    while (s.cur >= s.before + static_cast<int64_t>(units) * items) {
+      s.before += static_cast<int64_t>(units) * items;
+      units = seq_tiles(a, ++s.b) + kItemCost;
+    }
+    const int64_t off = s.cur - s.before;
+    const int item = static_cast<int>(off / units);
+    const int unit0 = static_cast<int>(off - static_cast<int64_t>(item) * units);
+    const int unit1 = static_cast<int>(min(static_cast<int64_t>(units), unit0 + (s.end - s.cur)));
+    s.cur += unit1 - unit0;
+    const int tiles = units - kItemCost;
+    const int tile0 = max(unit0 - kItemCost, 0), tile1 = unit1 - kItemCost;
+    if (tile1 <= tile0) continue;  // the share ends before the item's first tile
+    st.b = s.b;
+    stretch_heads(a, item, st);
+    const int n = seq_len(a, st.b, st.bad);
+    st.key0 = min(n, tile0 * kTile);
+    st.key1 = tile1 == tiles ? n : tile1 * kTile;
+    st.slot = tile0 == 0 && tile1 == tiles ? -1 : s.slot + (tile0 == 0 ? 1 : 0);
+    return true;
   }
-  const int64_t off = s.cur - s.before;
-  const int item = static_cast<int>(off / tiles);
-  const int tile0 = static_cast<int>(off - static_cast<int64_t>(item) * tiles);
-  const int tile1 = static_cast<int>(min(static_cast<int64_t>(tiles), tile0 + (s.end - s.cur)));
-  s.cur += tile1 - tile0;
-  st.b = s.b;
-  stretch_heads(a, item, st);
-  const int n = seq_len(a, st.b, st.bad);
-  st.key0 = min(n, tile0 * kTile);
-  st.key1 = tile1 == tiles ? n : tile1 * kTile;
-  st.slot = tile0 == 0 && tile1 == tiles ? -1 : 2 * static_cast<int64_t>(blockIdx.x) + (tile0 == 0 ? 1 : 0);
-  return true;
+  return false;
 }
 
-// Item blockIdx.x as one stretch (whole_items).
+// An item as one stretch (a CTA for each, no join).
 __device__ __forceinline__ Stretch whole_item(const PagedArgs& a, int64_t index) {
   const int items = a.heads_kv * a.items_per_head;
   Stretch st;
@@ -168,6 +186,11 @@ __device__ __forceinline__ Stretch whole_item(const PagedArgs& a, int64_t index)
   st.slot = -1;
   return st;
 }
+
+// The kernel over the keys for fp16 / bf16 (paged_attn_mma.cu): items of up to 16 heads.
+constexpr int kPagedMmaWarps = 4;
+int paged_mma_ctas_per_sm(int64_t head_dim);
+int launch_paged_mma(const PagedArgs& a, int dtype, int ctas, bool whole_items, const LaunchCtx& ctx);
 
 // Programmatic dependent launch: the join kernel starts while the main kernel runs, reads the
 // lengths, and waits here for the main kernel's results.
