@@ -326,10 +326,10 @@ typedef struct cmpx_rotation {
 typedef struct cmpx_rope_desc {
   const void* x;
   void* y;
+  cmpx_rotation rot;
   int64_t batch, heads, len, head_dim;
   int64_t x_stride[3]; /* batch, head, token (elements) */
   int64_t y_stride[3];
-  cmpx_rotation rot;
   int32_t dtype; /* cmpx_dtype */
   int32_t inverse;
 } cmpx_rope_desc;
@@ -367,13 +367,13 @@ typedef struct cmpx_kv_append_desc {
   const void* q;
   void* q_out;
   const int32_t* new_lengths;
+  cmpx_paged_cache cache;
+  cmpx_rotation rot;
   int64_t batch, heads, len;
   int64_t k_in_stride[3]; /* batch, head, token (elements) */
   int64_t v_in_stride[3];
   int64_t q_stride[3];
   int64_t q_out_stride[3];
-  cmpx_paged_cache cache;
-  cmpx_rotation rot;
   int32_t dtype; /* cmpx_dtype, of the cache too */
   int32_t reserved;
 } cmpx_kv_append_desc;
@@ -394,12 +394,12 @@ CMPX_API int cmpx_kv_append_plan(const cmpx_kv_append_desc* desc, char* buf, siz
 typedef struct cmpx_paged_attn_desc {
   const void* q;
   void* o;
+  void* workspace;
+  cmpx_paged_cache cache;
+  size_t workspace_bytes;
   int64_t batch, heads;
   int64_t q_stride[2]; /* batch, head (elements) */
   int64_t o_stride[2];
-  cmpx_paged_cache cache;
-  void* workspace;
-  size_t workspace_bytes;
   double scale;
   int32_t dtype; /* cmpx_dtype */
   int32_t reserved;

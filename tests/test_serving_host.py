@@ -89,6 +89,8 @@ def test_rope_refusals(cpu):
     refused("add up to 4", ops.rope, x, torch.zeros(2, 5), f, (5, -1))
     refused("sections must be 1 to 4", ops.rope, x, torch.zeros(5, 5), f, (1, 1, 1, 1, 0))
     refused("sections must be 1 to 4", ops.rope, x, torch.zeros(0, 5), f, ())
+    refused("whole numbers", ops.rope, x, torch.zeros(2, 5), f, (2.0, 2.0), error=TypeError)
+    refused("whole numbers", ops.rope, x, torch.zeros(2, 5), f, (torch.tensor(2), 2), error=TypeError)
     refused("no gradient", ops.rope, x, p, f.clone().requires_grad_())
     refused("no gradient", ops.rope, x, p.float().requires_grad_(), f)
 
@@ -187,8 +189,8 @@ def _rotation(pairs=32, axes=1, kind=1, ends=None):
 
 
 def _rope(dtype=2, D=64, ptr=PTR, stride=64, **rot):
-    return S.RopeDesc(ptr, PTR, 2, 3, 5, D, S._I64x3(15 * stride, 5 * stride, stride),
-                      S._I64x3(15 * D, 5 * D, D), _rotation(**rot), dtype, 0)
+    return S.RopeDesc(ptr, PTR, _rotation(**rot), 2, 3, 5, D, S._I64x3(15 * stride, 5 * stride, stride),
+                      S._I64x3(15 * D, 5 * D, D), dtype, 0)
 
 
 def test_rope_plans_and_statuses():
@@ -216,8 +218,8 @@ def _cache(D=64, page=16, pages=100, Hkv=2, width=8, ptr=PTR):
 
 def _attn(dtype=2, H=8, B=3, scale=0.1, **cache):
     c = _cache(**cache)
-    return S.PagedAttnDesc(PTR, PTR, B, H, S._I64x2(H * c.head_dim, c.head_dim), S._I64x2(H * c.head_dim, c.head_dim), c,
-                           None, 0, scale, dtype, 0)
+    st = S._I64x2(H * c.head_dim, c.head_dim)
+    return S.PagedAttnDesc(PTR, PTR, None, c, 0, B, H, st, st, scale, dtype, 0)
 
 
 def test_paged_attention_plans_and_statuses():
@@ -243,8 +245,8 @@ def test_paged_attention_plans_and_statuses():
 def _append(dtype=2, H=4, **cache):
     c = _cache(**cache)
     st = S._I64x3(c.heads_kv * 5 * c.head_dim, 5 * c.head_dim, c.head_dim)
-    return S.KvAppendDesc(PTR, PTR, PTR if H else None, PTR if H else None, None, 2, H, 5, st, st, st, st, c,
-                          _rotation(kind=0), dtype, 0)
+    return S.KvAppendDesc(PTR, PTR, PTR if H else None, PTR if H else None, None, c, _rotation(kind=0), 2, H, 5,
+                          st, st, st, st, dtype, 0)
 
 
 def test_kv_append_plans_and_statuses():

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -36,9 +37,9 @@ class Rotation(ctypes.Structure):
 
 
 class RopeDesc(ctypes.Structure):
-    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p),
+    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p), ("rot", Rotation),
                 ("batch", ctypes.c_int64), ("heads", ctypes.c_int64), ("len", ctypes.c_int64),
-                ("head_dim", ctypes.c_int64), ("x_stride", _I64x3), ("y_stride", _I64x3), ("rot", Rotation),
+                ("head_dim", ctypes.c_int64), ("x_stride", _I64x3), ("y_stride", _I64x3),
                 ("dtype", ctypes.c_int32), ("inverse", ctypes.c_int32)]
 
 
@@ -51,16 +52,16 @@ class PagedCache(ctypes.Structure):
 
 class KvAppendDesc(ctypes.Structure):
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q", ctypes.c_void_p), ("q_out", ctypes.c_void_p),
-                ("new_lengths", ctypes.c_void_p), ("batch", ctypes.c_int64), ("heads", ctypes.c_int64),
-                ("len", ctypes.c_int64), ("k_in_stride", _I64x3), ("v_in_stride", _I64x3), ("q_stride", _I64x3),
-                ("q_out_stride", _I64x3), ("cache", PagedCache), ("rot", Rotation),
+                ("new_lengths", ctypes.c_void_p), ("cache", PagedCache), ("rot", Rotation),
+                ("batch", ctypes.c_int64), ("heads", ctypes.c_int64), ("len", ctypes.c_int64),
+                ("k_in_stride", _I64x3), ("v_in_stride", _I64x3), ("q_stride", _I64x3), ("q_out_stride", _I64x3),
                 ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
 class PagedAttnDesc(ctypes.Structure):
-    _fields_ = [("q", ctypes.c_void_p), ("o", ctypes.c_void_p), ("batch", ctypes.c_int64), ("heads", ctypes.c_int64),
-                ("q_stride", _I64x2), ("o_stride", _I64x2), ("cache", PagedCache),
-                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("scale", ctypes.c_double),
+    _fields_ = [("q", ctypes.c_void_p), ("o", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("cache", PagedCache),
+                ("workspace_bytes", ctypes.c_size_t), ("batch", ctypes.c_int64), ("heads", ctypes.c_int64),
+                ("q_stride", _I64x2), ("o_stride", _I64x2), ("scale", ctypes.c_double),
                 ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
@@ -81,6 +82,33 @@ for _name, _desc in (("rope", RopeDesc), ("kv_append", KvAppendDesc), ("paged_at
     _fn.argtypes, _fn.restype = [ctypes.POINTER(_desc), ctypes.c_char_p, ctypes.c_size_t], ctypes.c_int
 lib.cmpx_paged_attn_workspace_size.argtypes = [ctypes.POINTER(PagedAttnDesc)]
 lib.cmpx_paged_attn_workspace_size.restype = ctypes.c_size_t
+
+
+# The checks, the descriptor and the output's layout of a call depend on its arguments' shapes, strides, types
+# and devices alone; only the pointers differ from call to call.  What a signature came to the first time
+# (the descriptor's bytes behind its pointers) is kept, so that a decoding loop's calls cost a lookup instead
+# of the checks.  A call whose pointers the kernel declines (misaligned ones) goes the long way again.
+_SIGNATURES: dict = {}
+_SIGNATURES_MOST = 4096
+_DIRECT = {}
+for _name in ("rope", "kv_append", "paged_attn", "linear_w4"):
+    _fn = lib[f"cmpx_{_name}"]  # the same entry point, taking the descriptor as bytes
+    _fn.argtypes, _fn.restype = [ctypes.c_char_p, ctypes.c_void_p], ctypes.c_int
+    _DIRECT[_name] = _fn
+_pack2, _pack4, _pack6, _pack7, _pack9 = (struct.Struct(f"={n}Q").pack for n in (2, 4, 6, 7, 9))
+
+
+def _keep(key, value) -> None:
+    if len(_SIGNATURES) >= _SIGNATURES_MOST:
+        _SIGNATURES.clear()
+    _SIGNATURES[key] = value
+
+
+def _direct(fn, data: bytes, index: int) -> int:
+    if index == torch._C._cuda_getDevice():
+        return fn(data, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(data, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _run(what: str, fn, desc, device: torch.device) -> None:
@@ -153,12 +181,14 @@ def _rotation(positions, freqs, sections, interleaved, batch: int, tokens: int, 
     axes = 1
     ends = (pairs, 0, 0, 0)
     if sections is not None:
+        if not all(type(n) is int for n in sections):
+            raise TypeError("sections must be whole numbers")
         axes = len(sections)
-        if not 1 <= axes <= _MAX_AXES or any(int(n) != n or n < 0 for n in sections) or sum(sections) != pairs:
+        if not 1 <= axes <= _MAX_AXES or min(sections) < 0 or sum(sections) != pairs:
             raise RuntimeError(f"sections must be 1 to {_MAX_AXES} counts of pairs that add up to {pairs}, got {sections}")
         at, out = 0, []
         for n in sections:
-            at += int(n)
+            at += n
             out.append(at)
         ends = tuple(out) + (0,) * (_MAX_AXES - axes)
     if positions is None:
@@ -196,17 +226,33 @@ def _rope_desc(x, positions, freqs, sections, interleaved, inverse):
     rot, keep = _rotation(positions, freqs, sections, interleaved, b, n, d, device)
     x = _unit(x)
     y = torch.empty_like(x)
-    if y.stride(3) != 1 and d != 1:
+    alike = y.stride(3) == 1 or d == 1
+    if not alike:
         y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    desc = RopeDesc(x.data_ptr(), y.data_ptr(), b, h, n, d, _I64x3(*x.stride()[:3]), _I64x3(*y.stride()[:3]), rot,
+    desc = RopeDesc(x.data_ptr(), y.data_ptr(), rot, b, h, n, d, _I64x3(*x.stride()[:3]), _I64x3(*y.stride()[:3]),
                     _DTYPE[x.dtype], 1 if inverse else 0)
-    return desc, y, (x, keep)
+    return desc, y, (x, keep, alike)
 
 
 def _rope_call(x, positions, freqs, sections, interleaved, inverse):
-    desc, y, _keep = _rope_desc(x, positions, freqs, sections, interleaved, inverse)
+    try:
+        key = ("rope", x.shape, x.stride(), x.dtype, x.device, positions.shape, positions.stride(), positions.dtype,
+               positions.device, freqs.shape, freqs.stride(), freqs.dtype, freqs.device, sections, interleaved, inverse)
+        how = _SIGNATURES.get(key)
+    except (AttributeError, TypeError):  # no tensors: the checks below name them
+        key = how = None
+    if how is not None:
+        tail, index = how
+        y = torch.empty_like(x)
+        if _direct(_DIRECT["rope"], _pack4(x.data_ptr(), y.data_ptr(), positions.data_ptr(), freqs.data_ptr()) + tail,
+                   index) == OK:
+            _post_check()
+            return y
+    desc, y, used = _rope_desc(x, positions, freqs, sections, interleaved, inverse)
     if y.numel():
         _run("rope", lib.cmpx_rope, desc, y.device)
+        if key is not None and used[0] is x and used[1][1] is freqs and used[2]:
+            _keep(key, (bytes(desc)[32:], y.device.index))
     return y
 
 
@@ -242,17 +288,17 @@ def rope(input, positions, freqs, sections=None, interleaved=False):
     ...): the first sections[0] pairs turn by positions[0], the next by positions[1], and so on.
     Angles are computed in 64 bits; the result, a new tensor, is rounded once.  Differentiable in
     ``input``; positions and freqs have no gradient.  head_dim <= 256."""
+    sections, interleaved = None if sections is None else tuple(sections), bool(interleaved)
     if torch.is_grad_enabled():
         _no_grad_only("rope in positions and freqs", positions, freqs)
         if isinstance(input, torch.Tensor) and input.requires_grad:
-            return _Rope.apply(input, positions, freqs, None if sections is None else tuple(sections),
-                               bool(interleaved), False)
+            return _Rope.apply(input, positions, freqs, sections, interleaved, False)
     return _rope_call(input, positions, freqs, sections, interleaved, False)
 
 
 def rope_plan(input, positions, freqs, sections=None, interleaved=False) -> str:
     """Name of the kernel ``rope`` runs for these arguments."""
-    desc, _y, _keep = _rope_desc(input, positions, freqs, sections, interleaved, False)
+    desc, _y, _used = _rope_desc(input, positions, freqs, sections, interleaved, False)
     return _plan("rope", lib.cmpx_rope_plan, desc)
 
 
@@ -311,7 +357,7 @@ def _append_desc(key, value, k_cache, v_cache, page_table, lengths, new_lengths,
             raise RuntimeError(f"query {tuple(query.shape)} does not match key {tuple(key.shape)}")
         query = _unit(query)
         # [batch, tokens, heads, head_dim] memory, as attention's output
-        out = torch.empty((b, n, heads, d), dtype=key.dtype, device=device).transpose(1, 2)
+        out = torch.empty_strided((b, heads, n, d), (n * heads * d, d, heads * d, 1), dtype=key.dtype, device=device)
         qp, qs, op, os_ = query.data_ptr(), query.stride()[:3], out.data_ptr(), out.stride()[:3]
     keep = ()
     if freqs is None:
@@ -323,8 +369,8 @@ def _append_desc(key, value, k_cache, v_cache, page_table, lengths, new_lengths,
             raise RuntimeError("sections need positions")
         rot, keep = _rotation(positions, freqs, sections, interleaved, b, n, d, device)
     desc = KvAppendDesc(key.data_ptr(), value.data_ptr(), qp, op,
-                        None if new_lengths is None else new_lengths.data_ptr(), b, heads, n,
-                        _I64x3(*key.stride()[:3]), _I64x3(*value.stride()[:3]), _I64x3(*qs), _I64x3(*os_), cache, rot,
+                        None if new_lengths is None else new_lengths.data_ptr(), cache, rot, b, heads, n,
+                        _I64x3(*key.stride()[:3]), _I64x3(*value.stride()[:3]), _I64x3(*qs), _I64x3(*os_),
                         _DTYPE[key.dtype], 0)
     return desc, out, (key, value, query, keep)
 
@@ -348,19 +394,54 @@ def kv_append(key, value, k_cache, v_cache, page_table, lengths, new_lengths=Non
 
     A token whose place is negative, behind the table or in a page that does not exist is not stored and
     sets a bit of ``device_status()``.  Which of two tokens that share a slot stays is not defined."""
-    _no_grad_only("kv_append", key, value, k_cache, v_cache, query, positions, freqs)
-    desc, out, _keep = _append_desc(key, value, k_cache, v_cache, page_table, lengths, new_lengths, query, positions,
-                                    freqs, sections, interleaved)
+    sections, interleaved = None if sections is None else tuple(sections), bool(interleaved)
+    if torch.is_grad_enabled():
+        _no_grad_only("kv_append", key, value, k_cache, v_cache, query, positions, freqs)
+    try:
+        sig = ("kv_append", key.shape, key.stride(), key.dtype, key.device, value.shape, value.stride(), value.dtype,
+               value.device, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device, v_cache.shape,
+               v_cache.stride(), v_cache.dtype, v_cache.device, page_table.shape, page_table.stride(), page_table.dtype,
+               page_table.device, lengths.shape, lengths.stride(), lengths.dtype, lengths.device, sections, interleaved)
+        for t in (new_lengths, query, positions, freqs):
+            sig += (None,) if t is None else (t.shape, t.stride(), t.dtype, t.device)
+        how = _SIGNATURES.get(sig)
+    except (AttributeError, TypeError):
+        sig = how = None
+    if how is not None:
+        middle, tail, shape, stride, index = how
+        out = None if shape is None else torch.empty_strided(shape, stride, dtype=key.dtype, device=key.device)
+        data = b"".join((
+            _pack9(key.data_ptr(), value.data_ptr(), 0 if out is None else query.data_ptr(),
+                   0 if out is None else out.data_ptr(), 0 if new_lengths is None else new_lengths.data_ptr(),
+                   k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), lengths.data_ptr()),
+            middle, _pack2(0 if positions is None else positions.data_ptr(), 0 if freqs is None else freqs.data_ptr()),
+            tail))
+        if _direct(_DIRECT["kv_append"], data, index) == OK:
+            _post_check()
+            _changed(k_cache, v_cache)
+            return out
+    desc, out, used = _append_desc(key, value, k_cache, v_cache, page_table, lengths, new_lengths, query, positions,
+                                   freqs, sections, interleaved)
     if desc.batch and desc.len:
         _run("kv_append", lib.cmpx_kv_append, desc, key.device)
-        torch.autograd.graph.increment_version([t for t in (k_cache, v_cache) if not t.is_inference()])
+        _changed(k_cache, v_cache)
+        if (sig is not None and used[0] is key and used[1] is value and used[2] is query
+                and (freqs is None or used[3][-1] is freqs)):
+            data, at = bytes(desc), KvAppendDesc.rot.offset
+            _keep(sig, (data[72:at], data[at + 16:], None if out is None else tuple(out.shape),
+                        None if out is None else out.stride(), key.device.index))
     return out
+
+
+def _changed(*caches) -> None:
+    """Counts the caches as written in place, for autograd's check of saved tensors."""
+    torch.autograd.graph.increment_version([t for t in caches if not t.is_inference()])
 
 
 def kv_append_plan(key, value, k_cache, v_cache, page_table, lengths, new_lengths=None, query=None, positions=None,
                    freqs=None, sections=None, interleaved=False) -> str:
     """Name of the kernel ``kv_append`` runs for these arguments."""
-    desc, _out, _keep = _append_desc(key, value, k_cache, v_cache, page_table, lengths, new_lengths, query, positions,
+    desc, _out, _used = _append_desc(key, value, k_cache, v_cache, page_table, lengths, new_lengths, query, positions,
                                      freqs, sections, interleaved)
     return _plan("kv_append", lib.cmpx_kv_append_plan, desc)
 
@@ -383,9 +464,9 @@ def _paged_attn_desc(query, k_cache, v_cache, page_table, lengths, scale):
         if query.data_ptr() % 16:
             query = query.clone()
         st = query.stride()
-    out = torch.empty((b, 1, heads, d), dtype=query.dtype, device=device).transpose(1, 2)
-    desc = PagedAttnDesc(query.data_ptr(), out.data_ptr(), b, heads, _I64x2(st[0], st[1]), _I64x2(heads * d, d), cache,
-                         None, 0, scale, _DTYPE[query.dtype], 0)
+    out = torch.empty((b, heads, 1, d), dtype=query.dtype, device=device)
+    desc = PagedAttnDesc(query.data_ptr(), out.data_ptr(), None, cache, 0, b, heads, _I64x2(st[0], st[1]),
+                         _I64x2(heads * d, d), scale, _DTYPE[query.dtype], 0)
     return desc, out, query
 
 
@@ -399,25 +480,43 @@ def paged_attention(query, k_cache, v_cache, page_table, lengths, scale=None):
     A sequence of length 0 gets zeros.  A length beyond the table, or a page that does not exist among a
     sequence's pages, makes that sequence's rows NaN and sets a bit of ``device_status()``.  The lengths
     are read on the device: a captured call can be replayed with other ones."""
-    _no_grad_only("paged_attention", query, k_cache, v_cache)
-    desc, out, _keep = _paged_attn_desc(query, k_cache, v_cache, page_table, lengths, scale)
+    scale = None if scale is None else float(scale)
+    if torch.is_grad_enabled():
+        _no_grad_only("paged_attention", query, k_cache, v_cache)
+    try:
+        sig = ("paged_attention", query.shape, query.stride(), query.dtype, query.device, k_cache.shape, k_cache.stride(),
+               k_cache.dtype, k_cache.device, v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device,
+               page_table.shape, page_table.stride(), page_table.dtype, page_table.device, lengths.shape,
+               lengths.stride(), lengths.dtype, lengths.device, scale)
+        how = _SIGNATURES.get(sig)
+    except (AttributeError, TypeError):
+        sig = how = None
+    if how is not None:
+        tail, nbytes, index = how
+        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
+        data = _pack7(query.data_ptr(), out.data_ptr(), 0 if ws is None else ws.data_ptr(), k_cache.data_ptr(),
+                      v_cache.data_ptr(), page_table.data_ptr(), lengths.data_ptr()) + tail
+        if _direct(_DIRECT["paged_attn"], data, index) == OK:
+            _post_check()
+            return out
+    desc, out, used = _paged_attn_desc(query, k_cache, v_cache, page_table, lengths, scale)
     if out.numel():
         dev = out.device
-        if dev.index == torch.cuda.current_device():
+        with torch.cuda.device(dev):
             nbytes = lib.cmpx_paged_attn_workspace_size(ctypes.byref(desc))
-        else:
-            with torch.cuda.device(dev):
-                nbytes = lib.cmpx_paged_attn_workspace_size(ctypes.byref(desc))
         if nbytes:  # this call's own: concurrent calls and captured graphs share none
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             desc.workspace, desc.workspace_bytes = ws.data_ptr(), nbytes
         _run("paged_attention", lib.cmpx_paged_attn, desc, dev)
+        if sig is not None and used is query:
+            _keep(sig, (bytes(desc)[56:], nbytes, dev.index))
     return out
 
 
 def paged_attention_plan(query, k_cache, v_cache, page_table, lengths, scale=None) -> str:
     """Name of the schedule ``paged_attention`` runs for these arguments."""
-    desc, _out, _keep = _paged_attn_desc(query, k_cache, v_cache, page_table, lengths, scale)
+    desc, _out, _used = _paged_attn_desc(query, k_cache, v_cache, page_table, lengths, scale)
     return _plan("paged_attention", lib.cmpx_paged_attn_plan, desc)
 
 
@@ -479,14 +578,35 @@ def linear_w4(input, weight, scales, zeros=None, bias=None):
     weights are not rounded (whole-number differences, fp32 sums, one product with the scale a group)
     and the result is rounded once.  The weights are read once per 8 tokens: with many tokens a
     dequantised weight and ``linear`` are the faster way."""
-    _no_grad_only("linear_w4", input, scales, bias)
-    desc, y, _keep = _linear_w4_desc(input, weight, scales, zeros, bias)
+    if torch.is_grad_enabled():
+        _no_grad_only("linear_w4", input, scales, bias)
+    try:
+        sig = ("linear_w4", input.shape, input.stride(), input.dtype, input.device, weight.shape, weight.stride(),
+               weight.dtype, weight.device, scales.shape, scales.stride(), scales.dtype, scales.device)
+        for t in (zeros, bias):
+            sig += (None,) if t is None else (t.shape, t.stride(), t.dtype, t.device)
+        how = _SIGNATURES.get(sig)
+    except (AttributeError, TypeError):
+        sig = how = None
+    if how is not None:
+        tail, shape, index = how
+        y = torch.empty(shape, dtype=input.dtype, device=input.device)
+        data = _pack6(input.data_ptr(), weight.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(),
+                      0 if bias is None else bias.data_ptr(), y.data_ptr()) + tail
+        if _direct(_DIRECT["linear_w4"], data, index) == OK:
+            _post_check()
+            return y
+    desc, y, used = _linear_w4_desc(input, weight, scales, zeros, bias)
+    shape = tuple(input.shape[:-1]) + (y.shape[1],)
     if y.numel():
         _run("linear_w4", lib.cmpx_linear_w4, desc, y.device)
-    return y.view(input.shape[:-1] + (y.shape[1],))
+        if (sig is not None and used[0].data_ptr() == input.data_ptr()
+                and all(a is b for a, b in zip(used[1:], (weight, scales, zeros, bias)))):
+            _keep(sig, (bytes(desc)[48:], shape, y.device.index))
+    return y.view(shape)
 
 
 def linear_w4_plan(input, weight, scales, zeros=None, bias=None) -> str:
     """Name of the kernel ``linear_w4`` runs for these arguments."""
-    desc, _y, _keep = _linear_w4_desc(input, weight, scales, zeros, bias)
+    desc, _y, _used = _linear_w4_desc(input, weight, scales, zeros, bias)
     return _plan("linear_w4", lib.cmpx_linear_w4_plan, desc)

@@ -234,20 +234,41 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_const
   }
 }
 
-// Joins the partial results of one (sequence, query head): a block per row, a warp per partial result
-// in turn, lanes along the head.
-template <int DT>
+// Loads of what the main kernel wrote: from L2, and, being volatile, never moved above pdl_wait().
+__device__ __forceinline__ float2 load_part2(const float* p) {
+  float2 v;
+  asm volatile("ld.global.cg.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 load_part4(const float* p) {
+  float4 v;
+  asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
+// Joins the partial results of one (sequence, query head): a block per row.  A warp takes every
+// kJoinWarps'th partial result: up to 32 at a time, a lane each for the maxima and sums, all lanes along
+// the head for the outputs, whose loads do not wait for the weights.
+template <int DT, int V>  // V: float4 vectors per lane and row (head_dim <= 128 V)
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a) {
-  constexpr int W = kJoinThreads / 32, MAXV = 8;
+  constexpr int W = kJoinThreads / 32;
+  constexpr int AHEAD = 8;
   constexpr int ES = elt_size(DT);
-  __shared__ int64_t scratch[36];
   __shared__ float sm_ml[W][2];
-  __shared__ float sm_o[W][256];
+  __shared__ float4 sm_o[W][32 * V];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / a.heads, h = blockIdx.x - b * a.heads;
-  int64_t first = 0, rest = 0, unused;
-  for (int i = threadIdx.x; i < a.batch; i += kJoinThreads) (i < b ? first : rest) += seq_units(a, i);
-  first = block_scan(first, scratch, &unused);
-  const int64_t total = first + block_scan(rest, scratch, &unused);
+  int64_t first = 0, total = 0;  // units before sequence b, and in all
+  for (int i = lane; i < a.batch; i += 32) {
+    const int64_t n = seq_units(a, i);
+    total += n;
+    if (i < b) first += n;
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    first += __shfl_xor_sync(0xffffffffu, first, off);
+    total += __shfl_xor_sync(0xffffffffu, total, off);
+  }
   const int64_t share = share_units(total, a.workers);
   const int tiles = seq_tiles(a, b);
   const int kvh = h / a.group, g = h - kvh * a.group, part = g / a.item_heads;
@@ -256,31 +277,60 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   pdl_wait();  // every block: this kernel is not done before the main one is
   if (c0 == c1) return;  // written by its warp
   const int hh = g - part * a.item_heads;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float m = -INFINITY, l = 0.f, o[MAXV];
+  float m = -INFINITY, l = 0.f;
+  float4 o[V];
 #pragma unroll
-  for (int i = 0; i < MAXV; ++i) o[i] = 0.f;
-  for (int64_t c = c0 + warp; c <= c1; c += W) {
-    const int64_t row = (2 * c + (c == c0 ? 1 : 0)) * a.item_heads + hh;
-    const float m2 = __ldcg(a.part_ml + 2 * row), l2 = __ldcg(a.part_ml + 2 * row + 1);
-    float p[MAXV];
+  for (int v = 0; v < V; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto row_of = [&](int64_t c) { return (2 * c + (c == c0 ? 1 : 0)) * a.item_heads + hh; };
+  for (int64_t cb = c0 + warp; cb <= c1; cb += 32 * W) {
+    const int64_t mine = cb + static_cast<int64_t>(lane) * W;
+    const int count = static_cast<int>(min(static_cast<int64_t>(32), (c1 - cb) / W + 1));
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < count) ml = load_part2(a.part_ml + 2 * row_of(mine));
+    float top = ml.x;
 #pragma unroll
-    for (int i = 0; i < MAXV; ++i)
-      p[i] = lane + 32 * i < a.head_dim ? __ldcg(a.part_o + row * a.head_dim + lane + 32 * i) : 0.f;
-    const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
-    const float w1 = ex2_approx(m - base), w2 = ex2_approx(m2 - base);
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    top = fmaxf(top, m);
+    const float base = top == -INFINITY ? 0.f : top;
+    const float keep = ex2_approx(m - base), weight = lane < count ? ex2_approx(ml.x - base) : 0.f;
+    float sum = lane < count ? weight * ml.y : 0.f;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
     m = top;
-    l = l * w1 + l2 * w2;
+    l = l * keep + sum;
 #pragma unroll
-    for (int i = 0; i < MAXV; ++i) o[i] = o[i] * w1 + p[i] * w2;
+    for (int v = 0; v < V; ++v) o[v] = make_float4(o[v].x * keep, o[v].y * keep, o[v].z * keep, o[v].w * keep);
+    for (int k0 = 0; k0 < count; k0 += AHEAD) {
+      float4 p[AHEAD][V];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          p[k][v] = make_float4(0.f, 0.f, 0.f, 0.f);
+          const int d = 4 * (lane + 32 * v);
+          if (k0 + k < count && d < a.head_dim)
+            p[k][v] = load_part4(a.part_o + row_of(cb + static_cast<int64_t>(k0 + k) * W) * a.head_dim + d);
+        }
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const float w = __shfl_sync(0xffffffffu, weight, (k0 + k) & 31);
+        if (k0 + k < count)
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            o[v].x = fmaf(w, p[k][v].x, o[v].x);
+            o[v].y = fmaf(w, p[k][v].y, o[v].y);
+            o[v].z = fmaf(w, p[k][v].z, o[v].z);
+            o[v].w = fmaf(w, p[k][v].w, o[v].w);
+          }
+      }
+    }
   }
   if (lane == 0) {
     sm_ml[warp][0] = m;
     sm_ml[warp][1] = l;
   }
 #pragma unroll
-  for (int i = 0; i < MAXV; ++i)
-    if (lane + 32 * i < a.head_dim) sm_o[warp][lane + 32 * i] = o[i];
+  for (int v = 0; v < V; ++v) sm_o[warp][lane + 32 * v] = o[v];
   __syncthreads();
   for (int d = threadIdx.x; d < a.head_dim; d += kJoinThreads) {
     float top = -INFINITY;
@@ -292,7 +342,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     for (int w = 0; w < W; ++w) {
       const float weight = ex2_approx(sm_ml[w][0] - base);
       sum = fmaf(weight, sm_ml[w][1], sum);
-      acc = fmaf(weight, sm_o[w][d], acc);
+      acc = fmaf(weight, reinterpret_cast<const float*>(sm_o[w])[d], acc);
     }
     const float r = sum == 0.f ? 0.f : acc / sum;
     *reinterpret_cast<RawVec<ES>*>(a.o + b * a.o_sb + h * a.o_sh + d * ES) = pack_vec<DT, ES>(&r);
@@ -364,7 +414,9 @@ int launch_join(const PagedArgs& a, const LaunchCtx& ctx) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<DT>, a) == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
+  const cudaError_t err = a.head_dim <= 128 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<DT, 1>, a)
+                                            : cudaLaunchKernelEx(&cfg, paged_join_kernel<DT, 2>, a);
+  return err == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
 }
 
 }  // namespace
