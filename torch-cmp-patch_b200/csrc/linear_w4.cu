@@ -7,18 +7,25 @@
 // go in as three bf16 parts (the leading, next and last 8 bits of the fraction: an exact sum), three
 // products each.
 //
-// The weights are read once, n k / 2 bytes, and that read bounds it while the tokens are few.  A CTA has 16
-// rows of W, its warps take turns at chunks of 128 k, and mma.m16n8k16 multiplies the 16 rows with up to
-// 8 NT tokens.  A lane loads 8 bytes of a row, 16 k that lie side by side (a quad: one 32-byte sector),
-// and the products run over k in the order that falls out of it: word j of the lanes tq = 0..3 holds k =
-// 16 tq + 8 j .. + 7, and nibbles e and e + 4 of a word, which one mask isolates as the halves of a
-// register, are a pair.  x follows that order with one byte permutation a register.  Chunks are loaded DEPTH ahead
-// into registers.  What it costs beside the loads is instructions: for eight weights 3 shifts, 4 masks, 4
-// subtractions (fp16: 1, 4, 4).
+// The weights are read once, n k / 2 bytes, and that read bounds it while the tokens are few.  One CTA per SM
+// has a run of tiles of 16 rows of W, and its warps have equal runs of the tiles' turns of 256 k laid
+// end to end; mma.m16n8k16 multiplies the 16 rows with 8 NT tokens.  Every warp has its own pipeline
+// of turns (2 KB each, cp.async) that runs on across tiles.  A tile that one warp has to itself is written from
+// its registers; the others' parts are summed once, at the CTA's end, in a fixed order.  (A tile
+// shared by all warps and summed before the next one took twice the instructions and 22 us for 8 x 16384 x 4096
+// in fp16, whose bytes take 5.7.)
+// A lane takes 16 k of a row that lie side by side, and the products run over k in the order that falls out
+// of it: word j of the lanes tq = 0..3 holds k = 16 tq + 8 j .. + 7, and nibbles e and e + 4 of a word, which
+// one mask isolates as the halves of a register, are a pair.  x follows that order with one byte
+// permutation a register.  Scales and zero points pass through a table in shared memory that holds them
+// as the products take them.  Instructions come next to the bytes: for eight weights 3 shifts, 4
+// masks and 4 subtractions (fp16: 1, 4, 4), and as many again for the rest.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <mutex>
+#include <type_traits>
 
 #include "cmpx_internal.h"
 #include "rowvec.cuh"
@@ -26,10 +33,13 @@
 namespace cmpx {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
-constexpr int kRows = 16;    // rows of W per CTA
-constexpr int kChunk = 128;  // k per warp and turn
+constexpr int kRows = 16;    // rows of W per tile
+constexpr int kChunk = 256;  // k per turn
+constexpr int kStages = 4;   // turns in a warp's pipeline
+constexpr int kHeld = kStages - 1;  // turns between the load of a scale and its entry in the table: turn u's
+                                    // scales are entered by the push that comes before its products
 
 struct W4Args {
   const uint8_t* x;
@@ -41,58 +51,59 @@ struct W4Args {
   int64_t xs, ws, ss, zs, ys;  // row strides in bytes
   int m, n, k;
   FastDiv group;
+  int tiles, chunks;  // row tiles, turns per tile
 };
 
-// Where the groups end: at every chunk's end or rarer, inside it at 64 k, or at 32 k.
+// Where groups may end: at multiples of 128 k, of 64 k, or of 32 k.
 enum GroupKind { kGroup128 = 0, kGroup64 = 1, kGroup32 = 2 };
 
-__device__ __forceinline__ uint2 load_w(const uint8_t* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-
-template <int DT>
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// c = (FIRST ? 0 : c) + A B
+template <int DT, bool FIRST>
 __device__ __forceinline__ void mma_w4(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
+  const float i0 = FIRST ? 0.f : c[0], i1 = FIRST ? 0.f : c[1], i2 = FIRST ? 0.f : c[2], i3 = FIRST ? 0.f : c[3];
   if constexpr (DT == CMPX_F16)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(i0), "f"(i1), "f"(i2), "f"(i3));
   else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(i0), "f"(i1), "f"(i2), "f"(i3));
 }
 
 // The eight codes of a word minus a zero point as four 16-bit pairs: pair e = codes e and e + 4.  A code
 // placed under the exponent of 128 (bf16) or 1024 (fp16) is that number plus the code; zp holds the number
 // plus the zero point, twice.  fp16 has room for a nibble four bits higher, which saves shifts: 1024 + 16 c
-// times 1/16 minus (64 + zero), one exact fma (zp16).
+// times 1/16 minus (64 + zero), one exact fma.
 template <int DT>
-struct Zero {
-  uint32_t zp, zp16;
-  __device__ __forceinline__ explicit Zero(uint32_t z) {
-    if constexpr (DT == CMPX_F16) {
-      zp = (0x6400u + z) * 0x10001u;
-      const __half2 v = __float2half2_rn(-64.f - static_cast<float>(z));
-      zp16 = *reinterpret_cast<const uint32_t*>(&v);
-    } else {
-      zp = (0x4300u + z) * 0x10001u;
-      zp16 = 0;
-    }
-  }
-};
+__device__ __forceinline__ uint32_t zero_pair(uint32_t z) {
+  return ((DT == CMPX_F16 ? 0x6400u : 0x4300u) + z) * 0x10001u;
+}
+
+// (w & mask) | base as one instruction: given two constants the compiler takes two.
+__device__ __forceinline__ uint32_t mask_or(uint32_t w, uint32_t mask, uint32_t base) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(w), "r"(mask), "r"(base));
+  return d;
+}
 
 template <int DT>
-__device__ __forceinline__ void codes_minus_zero(uint32_t w, const Zero<DT>& z, uint32_t (&out)[4]) {
+__device__ __forceinline__ void codes_minus_zero(uint32_t w, uint32_t zero, uint32_t (&out)[4]) {
   if constexpr (DT == CMPX_F16) {
     const uint32_t v = w >> 8;
-    const uint32_t c[4] = {(w & 0x000F000Fu) | 0x64006400u, (w & 0x00F000F0u) | 0x64006400u,
-                           (v & 0x000F000Fu) | 0x64006400u, (v & 0x00F000F0u) | 0x64006400u};
-    const __half2 zp = *reinterpret_cast<const __half2*>(&z.zp), zp16 = *reinterpret_cast<const __half2*>(&z.zp16);
+    const uint32_t c[4] = {mask_or(w, 0x000F000Fu, 0x64006400u), mask_or(w, 0x00F000F0u, 0x64006400u),
+                           mask_or(v, 0x000F000Fu, 0x64006400u), mask_or(v, 0x00F000F0u, 0x64006400u)};
+    const __half2 zp = *reinterpret_cast<const __half2*>(&zero);
+    const __half2 zp16 = __hsub2(__half2half2(__ushort_as_half(0x6380)), zp);  // 960 - (1024 + z)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const __half2 h = *reinterpret_cast<const __half2*>(&c[e]);
@@ -100,228 +111,354 @@ __device__ __forceinline__ void codes_minus_zero(uint32_t w, const Zero<DT>& z, 
       out[e] = *reinterpret_cast<const uint32_t*>(&d);
     }
   } else {
-    const __nv_bfloat162 zp = *reinterpret_cast<const __nv_bfloat162*>(&z.zp);
+    const __nv_bfloat162 zp = *reinterpret_cast<const __nv_bfloat162*>(&zero);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const uint32_t c = ((w >> (4 * e)) & 0x000F000Fu) | 0x43004300u;
+      const uint32_t c = mask_or(w >> (4 * e), 0x000F000Fu, 0x43004300u);
       const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&c), zp);
       out[e] = *reinterpret_cast<const uint32_t*>(&d);
     }
   }
 }
 
-// 8 activations as PARTS sets of four pairs (e, e + 4).
+// 8 activations: as loaded, and as PARTS sets of four pairs (e, e + 4).
 template <int DT>
-struct XParts {
+struct Activations {
   static constexpr int PARTS = DT == CMPX_F32 ? 3 : 1;
-  uint32_t p[PARTS][4];
+  static constexpr int VECS = DT == CMPX_F32 ? 2 : 1;
+  uint4 v[VECS];
+
+  __device__ __forceinline__ void load(const uint8_t* p) {
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < VECS; ++i) v[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void pairs(uint32_t (&p)[PARTS][4]) const {
+    if constexpr (DT == CMPX_F32) {
+      const uint32_t x[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+      uint32_t part[8][3];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        // cut off, not rounded, so that the largest values do not become infinite (the permutation below
+        // takes the upper halves); an infinite value has no rest
+        const float f = __uint_as_float(x[e]);
+        const float rest = fabsf(f) == INFINITY ? 0.f : f - __uint_as_float(x[e] & 0xFFFF0000u);
+        part[e][0] = x[e];
+        part[e][1] = __float_as_uint(rest);
+        part[e][2] = __float_as_uint(rest - __uint_as_float(part[e][1] & 0xFFFF0000u));
+      }
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[i][e] = __byte_perm(part[e][i], part[e + 4][i], 0x7632);
+    } else {
+      p[0][0] = __byte_perm(v[0].x, v[0].z, 0x5410);
+      p[0][1] = __byte_perm(v[0].x, v[0].z, 0x7632);
+      p[0][2] = __byte_perm(v[0].y, v[0].w, 0x5410);
+      p[0][3] = __byte_perm(v[0].y, v[0].w, 0x7632);
+    }
+  }
 };
 
-template <int DT>
-__device__ __forceinline__ XParts<DT> load_x(const uint8_t* p, bool there) {
-  XParts<DT> r;
-  if constexpr (DT == CMPX_F32) {
-    uint4 u = make_uint4(0, 0, 0, 0), v = u;
-    if (there) {
-      u = __ldg(reinterpret_cast<const uint4*>(p));
-      v = __ldg(reinterpret_cast<const uint4*>(p) + 1);
-    }
-    const uint32_t x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-    uint32_t part[8][3];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float f = __uint_as_float(x[e]);
-      const bool finite = fabsf(f) <= 3.402823466e38f;
-      // cut off, not rounded, so that the largest values do not become infinite; NaN stays NaN
-      part[e][0] = finite ? x[e] & 0xFFFF0000u : f != f ? 0x7FC00000u : x[e];
-      const float rest = finite ? f - __uint_as_float(part[e][0]) : 0.f;
-      part[e][1] = __float_as_uint(rest) & 0xFFFF0000u;
-      part[e][2] = __float_as_uint(rest - __uint_as_float(part[e][1]));
-    }
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r.p[i][e] = __byte_perm(part[e][i], part[e + 4][i], 0x7632);
-  } else {
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (there) u = __ldg(reinterpret_cast<const uint4*>(p));
-    r.p[0][0] = __byte_perm(u.x, u.z, 0x5410);
-    r.p[0][1] = __byte_perm(u.x, u.z, 0x7632);
-    r.p[0][2] = __byte_perm(u.y, u.w, 0x5410);
-    r.p[0][3] = __byte_perm(u.y, u.w, 0x7632);
-  }
-  return r;
-}
+template <int NT, int GK>
+struct W4Cfg {
+  static constexpr int GROUPS = GK == kGroup128 ? 2 : GK == kGroup64 ? 4 : 8;  // columns of the table per turn
+  static constexpr int ENTRIES = GROUPS * kRows / 32;                          // per lane
+  static constexpr int STAGE = kRows * kChunk / 2;
+  static constexpr int TABLE = GROUPS * (kRows + 1) * 8;                       // bytes
+  static constexpr int WARP = kStages * STAGE + TABLE;
+  static constexpr int RED = NT * 8 * (kRows + 1);                             // floats of a part
+  static constexpr int SMEM = kWarps * (WARP + 2 * RED * 4);
+};
 
 template <int DT, int NT, int GK>
-__global__ void __launch_bounds__(kThreads) linear_w4_kernel(const __grid_constant__ W4Args a) {
-  constexpr int ES = elt_size(DT);
-  constexpr int GROUPS = GK == kGroup128 ? 1 : GK == kGroup64 ? 2 : 4;  // scales per row and chunk
-  constexpr int DEPTH = GK == kGroup128 ? 4 : GK == kGroup64 ? 3 : 2;
-  __shared__ float red[kWarps][NT * 8][kRows + 1];
+__global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_constant__ W4Args a) {
+  using C = W4Cfg<NT, GK>;
+  constexpr int ES = elt_size(DT), GROUPS = C::GROUPS;
+  // Where registers allow it, the next quarter turn's activations are loaded before this one's products, and
+  // the two words of a quarter have sums of their own (8 x 131072 x 4096 fp16: 113 us without, 98 with).
+  constexpr bool AHEAD = DT != CMPX_F32 && NT == 1 && GK != kGroup32;
+  extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, tq = lane & 3;
-  const int n0 = blockIdx.x * kRows, m0 = blockIdx.y * (8 * NT);
-  // rows behind the last read the last one; their results are not written
-  const int row[2] = {min(n0 + gr, a.n - 1), min(n0 + gr + 8, a.n - 1)};
-  const uint8_t* wp[2] = {a.w + row[0] * a.ws + tq * 8, a.w + row[1] * a.ws + tq * 8};
-  const uint8_t* sp[2] = {a.scales + row[0] * a.ss, a.scales + row[1] * a.ss};
-  const uint8_t* zp[2] = {a.zeros + row[0] * a.zs, a.zeros + row[1] * a.zs};
-  const int chunks = (a.k + kChunk - 1) / kChunk;
+  const int m0 = blockIdx.y * (8 * NT);
+  uint8_t* const mine = smem + warp * C::WARP;
+  const uint32_t buf = smem_u32(mine);
+  float2* const table = reinterpret_cast<float2*>(mine + kStages * C::STAGE);
+  float* const red = reinterpret_cast<float*>(smem + kWarps * C::WARP);  // [warp][first or later tile][token][kRows + 1]
 
-  struct Chunk {
-    uint2 w[2][2];             // [half of the chunk][row]
-    RawVec<ES> s[GROUPS][2];   // [group][row]
-    uint32_t z[GROUPS][2];
-  };
-  auto fetch = [&](int c, Chunk& q) {
-    if (c >= chunks) return;
-    const int k0 = c * kChunk;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const bool there = k0 + h * 64 + tq * 16 < a.k;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) q.w[h][r] = there ? load_w(wp[r] + (k0 >> 1) + h * 32) : make_uint2(0, 0);
-    }
-#pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-      const int at = fast_div(min(k0 + g * (kChunk / GROUPS), a.k - 1), a.group);
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        q.s[g][r] = *reinterpret_cast<const RawVec<ES>*>(sp[r] + at * ES);
-        q.z[g][r] = a.zeros ? __ldg(zp[r] + at) : 8u;
-      }
-    }
-  };
+  const int chunks = a.chunks;
+  const int tile0 = static_cast<int>(static_cast<int64_t>(a.tiles) * blockIdx.x / gridDim.x);
+  const int tile1 = static_cast<int>(static_cast<int64_t>(a.tiles) * (blockIdx.x + 1) / gridDim.x);
+  const int run = ((tile1 - tile0) * chunks + kWarps - 1) / kWarps;  // turns per warp
+  const int u0 = min(warp * run, (tile1 - tile0) * chunks), u1 = min(u0 + run, (tile1 - tile0) * chunks);
 
-  float acc[NT][4];
+  const uint8_t* xp[NT];  // tokens behind the last read the last one; their results are not written
 #pragma unroll
   for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+    xp[t] = a.x + static_cast<int64_t>(min(m0 + t * 8 + gr, a.m - 1)) * a.xs + tq * 16 * ES;
 
-  auto compute = [&](int c, const Chunk& q) {
-    const int k0 = c * kChunk;
-    float part[GK == kGroup32 ? 2 : 1][NT][4];
-    auto clear = [&] {
+  // ---- loads: a cursor over this warp's turns, kStages - 1 ahead of the products
+  int f_left = u1 - u0, f_tile = tile0 + u0 / chunks, f_chunk = u0 % chunks, f_stage = 0;
+  const uint8_t *f_w[2], *f_s[C::ENTRIES], *f_z[C::ENTRIES];
+  auto f_rows = [&] {  // rows behind the last read the last one; their results are not written
+    const int n0 = f_tile * kRows;
 #pragma unroll
-      for (int i = 0; i < (GK == kGroup32 ? 2 : 1); ++i)
+    for (int i = 0; i < 2; ++i) f_w[i] = a.w + static_cast<int64_t>(min(n0 + 8 * i + gr, a.n - 1)) * a.ws + tq * 16;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+    for (int i = 0; i < C::ENTRIES; ++i) {
+      const int64_t r = min(n0 + (lane + 32 * i) / GROUPS, a.n - 1);
+      f_s[i] = a.scales + r * a.ss;
+      f_z[i] = a.zeros + r * a.zs;
+    }
+  };
+  f_rows();
+  RawVec<ES> s_raw[kHeld][C::ENTRIES];
+  uint32_t z_raw[kHeld][C::ENTRIES];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) part[i][t][e] = 0.f;
-    };
-    auto add = [&](int i, int g) {  // acc += scale[g] * part[i]
-      float s[2];
-      unpack_vec<DT, ES>(q.s[g][0], &s[0]);
-      unpack_vec<DT, ES>(q.s[g][1], &s[1]);
+  for (int q = 0; q < kHeld; ++q)
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+    for (int i = 0; i < C::ENTRIES; ++i) {
+      s_raw[q][i] = RawVec<ES>{};
+      z_raw[q][i] = 0;
+    }
+  // where this lane's 16 bytes of a row go: halves of 64 k of odd row pairs change places, so that a
+  // quad's 32 bytes of 4 rows fill the banks once
+  const uint32_t put = buf + gr * (kChunk / 2) + ((tq * 16) ^ (((gr >> 1) & 1) << 5));
+  // Starts the loads of the cursor's turn and enters the scales of the turn kHeld before it in the table.
+  auto push = [&] {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(s[e >> 1], part[i][t][e], acc[t][e]);
-    };
-    clear();
+    for (int i = 0; i < C::ENTRIES; ++i) {
+      const int e = lane + 32 * i, g = e % GROUPS, r = e / GROUPS;
+      float s;
+      unpack_vec<DT, ES>(s_raw[kHeld - 1][i], &s);
+      table[g * (kRows + 1) + r] = make_float2(s, __uint_as_float(zero_pair<DT>(z_raw[kHeld - 1][i])));
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = k0 + h * 64 + tq * 16;
-      // this lane's 16 k lie in one group
-      const int g = GK == kGroup128 ? 0 : GK == kGroup64 ? h : 0;
-      uint32_t z0, z1;
-      if (GK == kGroup32) {
-        z0 = tq < 2 ? q.z[(2 * h) % GROUPS][0] : q.z[(2 * h + 1) % GROUPS][0];
-        z1 = tq < 2 ? q.z[(2 * h) % GROUPS][1] : q.z[(2 * h + 1) % GROUPS][1];
-      } else {
-        z0 = q.z[g][0];
-        z1 = q.z[g][1];
+      for (int q = kHeld - 1; q > 0; --q) {
+        s_raw[q][i] = s_raw[q - 1][i];
+        z_raw[q][i] = z_raw[q - 1][i];
       }
-      const Zero<DT> zero0(z0), zero1(z1);
+    }
+    if (f_left > 0) {
+      --f_left;
+      const int k0 = f_chunk * kChunk;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int there = k0 + h * 128 + tq * 32 < a.k ? 16 : 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          cp_async16(put + f_stage * C::STAGE + i * 8 * (kChunk / 2) + h * 64, there ? f_w[i] + (k0 >> 1) + h * 64 : a.w, there);
+      }
+#pragma unroll
+      for (int i = 0; i < C::ENTRIES; ++i) {
+        const int g = (lane + 32 * i) % GROUPS;
+        const int at = fast_div(min(k0 + g * (kChunk / GROUPS), a.k - 1), a.group);
+        s_raw[0][i] = *reinterpret_cast<const RawVec<ES>*>(f_s[i] + at * ES);
+        z_raw[0][i] = a.zeros ? __ldg(f_z[i] + at) : 8u;
+      }
+      if (++f_chunk == chunks) {
+        f_chunk = 0;
+        ++f_tile;
+        f_rows();
+      }
+    }
+    cp_async_commit();
+    f_stage = f_stage + 1 == kStages ? 0 : f_stage + 1;
+  };
+
+  // ---- products
+  float acc[NT][4];
+  Activations<DT> x_ahead[2][NT];  // of the next full quarter turn
+  auto load_ahead = [&](int k) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) x_ahead[j][t].load(xp[t] + (k + 8 * j) * ES);
+  };
+  auto compute = [&](auto full, int c, int next, const uint8_t* stage) {  // full: the turn has all its 256 k
+    constexpr bool FULL = decltype(full)::value;
+    constexpr int SETS = GK == kGroup32 ? 2 : 1;  // sums of a quarter that have scales of their own
+    constexpr int CHAINS = AHEAD ? 2 : 1;
+    float part[CHAINS][SETS][NT][4];
+    float2 col[2], other[2];  // this lane's k's column, and (groups of 32) the quad's other one
+#pragma unroll
+    for (int h = 0; h < kChunk / 64; ++h) {
+      const int k = c * kChunk + h * 64;
+      if (!FULL && k >= a.k) break;
+      Activations<DT> x[2][NT];
+      if (AHEAD && FULL) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) x[j][t] = x_ahead[j][t];
+        load_ahead(h + 1 < kChunk / 64 ? k + 64 : next);
+      } else if (FULL || k + 64 <= a.k || tq < 2) {  // (the last quarter may have 32 k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) x[j][t].load(xp[t] + (k + 8 * j) * ES);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) x[j][t].zero();
+      }
+      uint2 w[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        w[r] = *reinterpret_cast<const uint2*>(stage + (8 * r + gr) * (kChunk / 2) + (((h & 1) ^ ((gr >> 1) & 1)) << 5) +
+                                               (h >> 1) * 64 + tq * 8);
+      const bool first = GK != kGroup128 || (h & 1) == 0;  // of the products that share a scale
+      if (first) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int g = GK == kGroup128 ? h >> 1 : GK == kGroup64 ? h : 2 * h + (tq >> 1);
+          col[r] = table[g * (kRows + 1) + 8 * r + gr];
+          if (GK == kGroup32) other[r] = table[(g ^ 1) * (kRows + 1) + 8 * r + gr];
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         uint32_t d0[4], d1[4];
-        codes_minus_zero<DT>(j ? q.w[h][0].y : q.w[h][0].x, zero0, d0);
-        codes_minus_zero<DT>(j ? q.w[h][1].y : q.w[h][1].x, zero1, d1);
+        codes_minus_zero<DT>(j ? w[0].y : w[0].x, __float_as_uint(col[0].y), d0);
+        codes_minus_zero<DT>(j ? w[1].y : w[1].x, __float_as_uint(col[1].y), d1);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const int m = m0 + t * 8 + gr;
-          const XParts<DT> x = load_x<DT>(a.x + m * a.xs + (k + 8 * j) * ES, m < a.m && k < a.k);
+          uint32_t p[Activations<DT>::PARTS][4];
+          x[j][t].pairs(p);
 #pragma unroll
-          for (int i = 0; i < XParts<DT>::PARTS; ++i) {
-            const uint32_t* p = x.p[i];
-            if constexpr (GK == kGroup32) {
-              // the quad's first two lanes are in one group, its last two in the next
-              const bool one = tq < 2;
-              mma_w4<DT>(part[0][t], d0[0], d1[0], d0[1], d1[1], one ? p[0] : 0, one ? p[1] : 0);
-              mma_w4<DT>(part[0][t], d0[2], d1[2], d0[3], d1[3], one ? p[2] : 0, one ? p[3] : 0);
-              mma_w4<DT>(part[1][t], d0[0], d1[0], d0[1], d1[1], one ? 0 : p[0], one ? 0 : p[1]);
-              mma_w4<DT>(part[1][t], d0[2], d1[2], d0[3], d1[3], one ? 0 : p[2], one ? 0 : p[3]);
-            } else {
-              mma_w4<DT>(part[0][t], d0[0], d1[0], d0[1], d1[1], p[0], p[1]);
-              mma_w4<DT>(part[0][t], d0[2], d1[2], d0[3], d1[3], p[2], p[3]);
+          for (int y = 0; y < Activations<DT>::PARTS; ++y) {
+#pragma unroll
+            for (int set = 0; set < SETS; ++set) {
+              // groups of 32: the quad's first two lanes are in one group, its last two in the next
+              const bool in = SETS == 1 || (tq >> 1) == set;
+              const uint32_t b0 = in ? p[y][0] : 0, b1 = in ? p[y][1] : 0, b2 = in ? p[y][2] : 0, b3 = in ? p[y][3] : 0;
+              float(&sum)[4] = part[j % CHAINS][set][t];
+              if (first && j < CHAINS && y == 0)
+                mma_w4<DT, true>(sum, d0[0], d1[0], d0[1], d1[1], b0, b1);
+              else
+                mma_w4<DT, false>(sum, d0[0], d1[0], d0[1], d1[1], b0, b1);
+              mma_w4<DT, false>(sum, d0[2], d1[2], d0[3], d1[3], b2, b3);
             }
           }
         }
       }
-      if (GK == kGroup64) {
-        add(0, h);
-        clear();
-      } else if (GK == kGroup32) {
-        add(0, (2 * h) % GROUPS);
-        add(GK == kGroup32 ? 1 : 0, (2 * h + 1) % GROUPS);
-        clear();
-      }
+      if (GK == kGroup128 && first && (FULL || k + 64 < a.k)) continue;  // the next quarter has the same scale
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float s = col[e >> 1].x;
+          if (GK == kGroup32) {
+            const float o = other[e >> 1].x;
+            acc[t][e] = fmaf(tq < 2 ? s : o, part[0][0][t][e], acc[t][e]);
+            acc[t][e] = fmaf(tq < 2 ? o : s, part[0][SETS - 1][t][e], acc[t][e]);
+          } else {
+            acc[t][e] = fmaf(s, AHEAD ? part[0][0][t][e] + part[CHAINS - 1][0][t][e] : part[0][0][t][e], acc[t][e]);
+          }
+        }
     }
-    if (GK == kGroup128) add(0, 0);
   };
-
-  Chunk ring[DEPTH];
-#pragma unroll
-  for (int i = 0; i < DEPTH; ++i) fetch(warp + i * kWarps, ring[i]);
-  for (int c = warp; c < chunks; c += DEPTH * kWarps) {
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i) {
-      if (c + i * kWarps < chunks) {
-        compute(c + i * kWarps, ring[i]);
-        fetch(c + (i + DEPTH) * kWarps, ring[i]);
-      }
-    }
-  }
-
-  // the warps' sums
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) red[warp][t * 8 + tq * 2 + (e & 1)][gr + 8 * (e >> 1)] = acc[t][e];
-  __syncthreads();
-  for (int i = threadIdx.x; i < NT * 8 * kRows; i += kThreads) {
-    const int t = i / kRows, r = i % kRows, m = m0 + t, n = n0 + r;
-    if (m >= a.m || n >= a.n) continue;
-    float s = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) s += red[w][t][r];
+  auto write = [&](int m, int n, float s) {
+    if (m >= a.m || n >= a.n) return;
     if (a.bias) {
       float b;
       unpack_vec<DT, ES>(*reinterpret_cast<const RawVec<ES>*>(a.bias + static_cast<int64_t>(n) * ES), &b);
       s += b;
     }
-    *reinterpret_cast<RawVec<ES>*>(a.y + m * a.ys + static_cast<int64_t>(n) * ES) = pack_vec<DT, ES>(&s);
+    *reinterpret_cast<RawVec<ES>*>(a.y + static_cast<int64_t>(m) * a.ys + static_cast<int64_t>(n) * ES) = pack_vec<DT, ES>(&s);
+  };
+
+#pragma unroll 1
+  for (int i = 0; i < kStages - 1; ++i) push();
+  int stage = 0;
+  int tile = tile0 + u0 / chunks, c = u0 % chunks;
+  // (a partial last turn leaves x_ahead at the row's begin, where the next tile's first turn needs it)
+  if (AHEAD && a.k >= kChunk) load_ahead((c + 1) * kChunk <= a.k ? c * kChunk : 0);
+  for (int u = u0; u < u1;) {
+    const int turns = min(chunks - c, u1 - u);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+    for (int i = 0; i < turns; ++i) {
+      cp_async_wait<kStages - 2>();
+      __syncwarp();  // this turn's weights are there, and everybody is done with the turn before
+      push();
+      __syncwarp();
+      // where the activations of the next full turn begin: behind this one, or with the next tile at 0
+      const int now = (c + i) * kChunk, after = now + 2 * kChunk <= a.k ? now + kChunk : 0;
+      if (now + kChunk <= a.k)
+        compute(std::true_type{}, c + i, after, mine + stage * C::STAGE);
+      else
+        compute(std::false_type{}, c + i, 0, mine + stage * C::STAGE);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+    float* const part = red + (2 * warp + (tile == tile0 + u0 / chunks ? 0 : 1)) * C::RED;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int token = t * 8 + tq * 2 + (e & 1), r = gr + 8 * (e >> 1);
+        if (turns == chunks)
+          write(m0 + token, tile * kRows + r, acc[t][e]);
+        else
+          part[token * (kRows + 1) + r] = acc[t][e];
+      }
+    u += turns;
+    c = 0;
+    ++tile;
+  }
+  cp_async_wait<0>();
+
+  // the tiles that several warps have parts of
+  __syncthreads();
+  for (int i = threadIdx.x; i < (tile1 - tile0) * (NT * 8 * kRows); i += kThreads) {
+    const int r = i % kRows, token = i / kRows % (NT * 8), t = i / (kRows * NT * 8);
+    const int w0 = t * chunks / run, w1 = ((t + 1) * chunks - 1) / run;
+    if (w0 == w1) continue;
+    float s = 0.f;
+    for (int w = w0; w <= w1; ++w)
+      s += red[(2 * w + (t == w * run / chunks ? 0 : 1)) * C::RED + token * (kRows + 1) + r];
+    write(m0 + token, (tile0 + t) * kRows + r, s);
   }
 }
 
 GroupKind group_kind(int64_t group) { return group % 128 == 0 ? kGroup128 : group % 64 == 0 ? kGroup64 : kGroup32; }
 
-template <int DT, int NT>
-int launch(const W4Args& a, const LaunchCtx& ctx) {
-  const dim3 grid(static_cast<unsigned>((a.n + kRows - 1) / kRows), static_cast<unsigned>((a.m + 8 * NT - 1) / (8 * NT)));
-  switch (group_kind(a.group.d)) {
-    case kGroup128: linear_w4_kernel<DT, NT, kGroup128><<<grid, kThreads, 0, ctx.stream>>>(a); break;
-    case kGroup64: linear_w4_kernel<DT, NT, kGroup64><<<grid, kThreads, 0, ctx.stream>>>(a); break;
-    default: linear_w4_kernel<DT, NT, kGroup32><<<grid, kThreads, 0, ctx.stream>>>(a); break;
-  }
+template <int DT, int NT, int GK>
+int launch(W4Args& a, const LaunchCtx& ctx) {
+  using C = W4Cfg<NT, GK>;
+  auto kernel = linear_w4_kernel<DT, NT, GK>;
+  static std::once_flag once[64];
+  static cudaError_t attr_err[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::call_once(once[dev & 63], [&] {
+    attr_err[dev & 63] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  });
+  if (attr_err[dev & 63] != cudaSuccess) return CMPX_ERR_LAUNCH;
+  a.chunks = (a.k + kChunk - 1) / kChunk;
+  a.tiles = (a.n + kRows - 1) / kRows;
+  const dim3 grid(static_cast<unsigned>(std::min(a.tiles, ctx.num_sms)), static_cast<unsigned>((a.m + 8 * NT - 1) / (8 * NT)));
+  kernel<<<grid, kThreads, C::SMEM, ctx.stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
 }
 
+template <int DT, int NT>
+int launch_group(W4Args& a, const LaunchCtx& ctx) {
+  switch (group_kind(a.group.d)) {
+    case kGroup128: return launch<DT, NT, kGroup128>(a, ctx);
+    case kGroup64: return launch<DT, NT, kGroup64>(a, ctx);
+    default: return launch<DT, NT, kGroup32>(a, ctx);
+  }
+}
+
 template <int DT>
-int launch_dt(const W4Args& a, const LaunchCtx& ctx) {
-  return a.m <= 8 ? launch<DT, 1>(a, ctx) : launch<DT, 2>(a, ctx);
+int launch_dt(W4Args& a, const LaunchCtx& ctx) {
+  return a.m <= 8 ? launch_group<DT, 1>(a, ctx) : launch_group<DT, 2>(a, ctx);
 }
 
 }  // namespace
@@ -334,7 +471,7 @@ const char* linear_w4_plan(const cmpx_linear_w4_desc* d, int* status) {
   if (d->dtype != CMPX_F32 && d->dtype != CMPX_F16 && d->dtype != CMPX_BF16) return "none";
   const int64_t es = elt_size(d->dtype);
   *status = CMPX_ERR_UNSUPPORTED_SHAPE;
-  if (d->group % 32 != 0 || d->k > (1 << 24) || d->n > (1ll << 31) - 65536 || d->m > 65535ll * 8) return "none";
+  if (d->group % 32 != 0 || d->k > (1 << 24) || d->n > ((1ll << 38) / d->k) || d->n > (1ll << 31) - 65536 || d->m > 65535ll * 8) return "none";
   if (d->x_row_stride < 0 || d->w_row_stride < 0 || d->scales_row_stride < 0 || d->zeros_row_stride < 0 ||
       d->y_row_stride < d->n)
     return "none";
