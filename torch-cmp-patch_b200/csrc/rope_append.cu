@@ -7,10 +7,13 @@
 // through) of one token, computes the chunk's cos and sin once and walks over the heads: the query
 // heads, then (append) the key heads into the cache, then the value heads, copied.
 //
-// What bounds it: the bytes, each value read once and written once.  The trigonometry does not count
-// as long as a thread serves several heads: the angle is reduced to a quarter turn in fp64 (two
-// products and a rounding per pair; far positions need it: 1e6 radians in fp32 are off by 0.06) and
-// only the remainder, within an eighth of a turn, goes to fp32 sincospi.
+// What bounds it: the bytes, each value read once and written once, as long as a thread serves several
+// heads with its cos and sin.  Rotation alone streams best with the loads of two heads at a time and four blocks
+// per SM ([2, 32, 8192, 128] bf16, 268 MB: 46 us; 48 with four heads and two blocks); the append, whose
+// addresses take more registers, with four heads and two blocks (4 x 2048 tokens, 16 heads of 64, fp16, 71 MB:
+// 16.6 us; 18.9 with two and four).
+// The angle is reduced in fp64 (1e6 radians in fp32 are off by 0.06) to within an eighth of a turn, where
+// short Taylor sums of sine and cosine are exact to fp32.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -23,7 +26,9 @@ namespace cmpx {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kJobsAtOnce = 4;  // heads whose loads a thread issues together
+// Heads whose loads a thread issues together, and blocks per SM.
+constexpr int jobs_at_once(bool append) { return append ? 4 : 2; }
+constexpr int blocks_per_sm(bool append) { return append ? 2 : 4; }
 constexpr int kMaxHeadDim = 256;
 
 struct Rows {  // [batch, heads, len, head_dim] bytes
@@ -60,27 +65,29 @@ __device__ __forceinline__ double load_pos(const RopeArgs& a, int axis, int b, i
   return static_cast<double>(static_cast<const float*>(a.pos)[i]);
 }
 
-// cos and sin of pos * freq.  In quarter turns t = pos * freq * 2 / pi: the whole part picks the
-// quadrant, the rest r (|r| <= 1/2) is turned by sincospi(r / 2) with an error below 2^-25 of a
-// quarter turn.
-__device__ __forceinline__ void turn(double pos, float freq, float& c, float& s) {
-  const double t = pos * static_cast<double>(freq) * 0.63661977236758134308;
-  const double whole = rint(t);
-  const float r = static_cast<float>(t - whole);
-  // the quadrant: whole modulo 4, exact for any finite whole
-  const int quad = static_cast<int>(whole - 4.0 * floor(whole * 0.25));
-  float c0, s0;
-  sincospif(0.5f * r, &s0, &c0);
-  const bool swap = quad & 1;
-  const float cc = swap ? s0 : c0, ss = swap ? c0 : s0;
-  c = (quad == 1 || quad == 2) ? -cc : cc;
-  s = (quad & 2) ? -ss : ss;
+// cos and sin of pos * freq, given quarters = pos * 2 / pi.  quarters * freq is the angle in quarter turns: adding
+// 1.5 * 2^52 rounds it to a whole number, whose last two bits, now the sum's, are the quadrant; the
+// rest, at most half a quarter turn, goes to the Taylor sums up to x^9 / 9! and x^10 / 10! (the next
+// terms are below 2^-29 there).  Good for angles below 2^50.
+__device__ __forceinline__ void turn(double quarters, float freq, float& c, float& s) {
+  constexpr double kRound = 6755399441055744.0;
+  const double f = static_cast<double>(freq);
+  const double sum = fma(quarters, f, kRound);
+  const int quad = __double2loint(sum) & 3;
+  const float x = static_cast<float>(fma(quarters, f, -(sum - kRound)) * 1.57079632679489661923);
+  const float x2 = x * x;
+  const float sine = fmaf(x * x2, fmaf(x2, fmaf(x2, fmaf(x2, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f), x);
+  const float cosine =
+      fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, -1.f / 3628800.f, 1.f / 40320.f), -1.f / 720.f), 1.f / 24.f), -0.5f), 1.f);
+  const float cc = quad & 1 ? sine : cosine, ss = quad & 1 ? cosine : sine;
+  c = quad == 1 || quad == 2 ? -cc : cc;
+  s = quad & 2 ? -ss : ss;
 }
 
 template <int DT, int VB, bool APPEND>
-__global__ void __launch_bounds__(kThreads) rope_append_kernel(const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(APPEND)) rope_append_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int ES = elt_size(DT);
-  constexpr int VEC = VB / ES;
+  constexpr int VEC = VB / ES, kJobsAtOnce = jobs_at_once(APPEND);
   const int tokens_per_block = kThreads / a.chunks;
   const int tok = threadIdx.x / a.chunks;
   const int c = threadIdx.x - tok * a.chunks;
@@ -128,7 +135,7 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const __grid_cons
   if (turned && there) {
     double pos[CMPX_ROPE_MAX_AXES];
 #pragma unroll
-    for (int x = 0; x < CMPX_ROPE_MAX_AXES; ++x) pos[x] = x < a.axes ? load_pos(a, x, b, l, place) : 0.0;
+    for (int x = 0; x < CMPX_ROPE_MAX_AXES; ++x) pos[x] = x < a.axes ? load_pos(a, x, b, l, place) * 0.63661977236758134308 : 0.0;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const int j = c * VEC + i;
@@ -265,12 +272,13 @@ int launch(RopeArgs& a, int dt, int vec_bytes, const LaunchCtx& ctx) {
   const int tokens_per_block = kThreads / a.chunks;
   const int64_t gx = (static_cast<int64_t>(a.batch) * a.len + tokens_per_block - 1) / tokens_per_block;
   const int jobs = APPEND ? a.heads + 2 * a.heads_kv : a.heads;
-  // Heads per thread: as many as leave two full waves of blocks (8 of 256 threads per SM), so the
-  // trigonometry is shared where there is work enough, and one each where there is little.
-  const int64_t room = 2ll * 8 * ctx.num_sms;
-  int per = static_cast<int>(std::min<int64_t>(jobs, std::max<int64_t>(1, gx * jobs / room)));
-  per = std::max(per, (jobs + 65534) / 65535);
-  a.jobs_per_block = std::min(per, std::max(16, (jobs + 65534) / 65535));
+  // Heads per thread: as many as leave every SM its blocks once, so the trigonometry is shared where there is work
+  // enough, and one where there is little; whole sets of those that are loaded together.
+  const int64_t room = static_cast<int64_t>(blocks_per_sm(APPEND)) * ctx.num_sms, set = jobs_at_once(APPEND);
+  int64_t per = std::min<int64_t>(std::max<int64_t>(1, gx * jobs / room), 16);
+  if (per > 1) per = (per + set - 1) / set * set;
+  per = std::max<int64_t>(per, (jobs + 65534) / 65535);  // the grid's limit
+  a.jobs_per_block = static_cast<int>(std::min<int64_t>(per, jobs));
   const dim3 grid(static_cast<unsigned>(gx), static_cast<unsigned>((jobs + a.jobs_per_block - 1) / a.jobs_per_block));
 #define CMPX_ROPE(DT, VB) rope_append_kernel<DT, VB, APPEND><<<grid, kThreads, 0, ctx.stream>>>(a)
   if (dt == CMPX_F32) {
