@@ -104,6 +104,18 @@ def _keep(key, value) -> None:
     _SIGNATURES[key] = value
 
 
+# One value per device and type, expanded to the shapes of outputs and workspaces: torch.empty_like of such a
+# tensor costs half of what torch.empty with a type and a device does.  Never read.
+_ONES: dict = {}
+
+
+def _alike(shape, dtype, device) -> torch.Tensor:
+    one = _ONES.get((dtype, device))
+    if one is None:
+        one = _ONES[dtype, device] = torch.empty((), dtype=dtype, device=device)
+    return one.expand(shape)
+
+
 def _direct(fn, data: bytes, index: int) -> int:
     if index == torch._C._cuda_getDevice():
         return fn(data, torch._C._cuda_getCurrentRawStream(index))
@@ -166,6 +178,19 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _like(t: torch.Tensor) -> tuple[torch.Tensor, tuple]:
+    """An output laid out as t, contiguous along the last dimension, and its strides."""
+    out = torch.empty_like(t)
+    if out.stride(-1) != 1 and t.shape[-1] != 1:  # (rows of t overlap in some odd way)
+        out = torch.empty_like(t, memory_format=torch.contiguous_format)
+    return out, out.stride()
+
+
+def _is_like(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """True if torch.empty_like(t), which depends on t's shape and strides, is laid out as out."""
+    return out.stride() == torch.empty_like(t).stride()
+
+
 # ---------------------------------------------------------------------------------------------
 # rotary positions
 # ---------------------------------------------------------------------------------------------
@@ -225,13 +250,10 @@ def _rope_desc(x, positions, freqs, sections, interleaved, inverse):
     b, h, n, d = x.shape
     rot, keep = _rotation(positions, freqs, sections, interleaved, b, n, d, device)
     x = _unit(x)
-    y = torch.empty_like(x)
-    alike = y.stride(3) == 1 or d == 1
-    if not alike:
-        y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    desc = RopeDesc(x.data_ptr(), y.data_ptr(), rot, b, h, n, d, _I64x3(*x.stride()[:3]), _I64x3(*y.stride()[:3]),
+    y, ys = _like(x)
+    desc = RopeDesc(x.data_ptr(), y.data_ptr(), rot, b, h, n, d, _I64x3(*x.stride()[:3]), _I64x3(*ys[:3]),
                     _DTYPE[x.dtype], 1 if inverse else 0)
-    return desc, y, (x, keep, alike)
+    return desc, y, (x, keep)
 
 
 def _rope_call(x, positions, freqs, sections, interleaved, inverse):
@@ -251,7 +273,7 @@ def _rope_call(x, positions, freqs, sections, interleaved, inverse):
     desc, y, used = _rope_desc(x, positions, freqs, sections, interleaved, inverse)
     if y.numel():
         _run("rope", lib.cmpx_rope, desc, y.device)
-        if key is not None and used[0] is x and used[1][1] is freqs and used[2]:
+        if key is not None and used[0] is x and used[1][1] is freqs and _is_like(y, x):
             _keep(key, (bytes(desc)[32:], y.device.index))
     return y
 
@@ -356,9 +378,8 @@ def _append_desc(key, value, k_cache, v_cache, page_table, lengths, new_lengths,
         if query.shape[0] != b or query.shape[2] != n or query.shape[3] != d:
             raise RuntimeError(f"query {tuple(query.shape)} does not match key {tuple(key.shape)}")
         query = _unit(query)
-        # [batch, tokens, heads, head_dim] memory, as attention's output
-        out = torch.empty_strided((b, heads, n, d), (n * heads * d, d, heads * d, 1), dtype=key.dtype, device=device)
-        qp, qs, op, os_ = query.data_ptr(), query.stride()[:3], out.data_ptr(), out.stride()[:3]
+        out, os_ = _like(query)
+        qp, qs, op, os_ = query.data_ptr(), query.stride()[:3], out.data_ptr(), os_[:3]
     keep = ()
     if freqs is None:
         if positions is not None or sections is not None:
@@ -408,8 +429,8 @@ def kv_append(key, value, k_cache, v_cache, page_table, lengths, new_lengths=Non
     except (AttributeError, TypeError):
         sig = how = None
     if how is not None:
-        middle, tail, shape, stride, index = how
-        out = None if shape is None else torch.empty_strided(shape, stride, dtype=key.dtype, device=key.device)
+        middle, tail, index = how
+        out = None if query is None else torch.empty_like(query)
         data = b"".join((
             _pack9(key.data_ptr(), value.data_ptr(), 0 if out is None else query.data_ptr(),
                    0 if out is None else out.data_ptr(), 0 if new_lengths is None else new_lengths.data_ptr(),
@@ -426,16 +447,17 @@ def kv_append(key, value, k_cache, v_cache, page_table, lengths, new_lengths=Non
         _run("kv_append", lib.cmpx_kv_append, desc, key.device)
         _changed(k_cache, v_cache)
         if (sig is not None and used[0] is key and used[1] is value and used[2] is query
-                and (freqs is None or used[3][-1] is freqs)):
+                and (out is None or _is_like(out, query)) and (freqs is None or used[3][-1] is freqs)):
             data, at = bytes(desc), KvAppendDesc.rot.offset
-            _keep(sig, (data[72:at], data[at + 16:], None if out is None else tuple(out.shape),
-                        None if out is None else out.stride(), key.device.index))
+            _keep(sig, (data[72:at], data[at + 16:], key.device.index))
     return out
 
 
 def _changed(*caches) -> None:
     """Counts the caches as written in place, for autograd's check of saved tensors."""
-    torch.autograd.graph.increment_version([t for t in caches if not t.is_inference()])
+    for t in caches:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
 
 
 def kv_append_plan(key, value, k_cache, v_cache, page_table, lengths, new_lengths=None, query=None, positions=None,
@@ -464,9 +486,9 @@ def _paged_attn_desc(query, k_cache, v_cache, page_table, lengths, scale):
         if query.data_ptr() % 16:
             query = query.clone()
         st = query.stride()
-    out = torch.empty((b, heads, 1, d), dtype=query.dtype, device=device)
+    out, os_ = _like(query)  # whose rows are on 16-byte boundaries
     desc = PagedAttnDesc(query.data_ptr(), out.data_ptr(), None, cache, 0, b, heads, _I64x2(st[0], st[1]),
-                         _I64x2(heads * d, d), scale, _DTYPE[query.dtype], 0)
+                         _I64x2(os_[0], os_[1]), scale, _DTYPE[query.dtype], 0)
     return desc, out, query
 
 
@@ -492,9 +514,9 @@ def paged_attention(query, k_cache, v_cache, page_table, lengths, scale=None):
     except (AttributeError, TypeError):
         sig = how = None
     if how is not None:
-        tail, nbytes, index = how
-        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
+        tail, scratch, index = how
+        out = torch.empty_like(query)
+        ws = None if scratch is None else torch.empty_like(scratch)
         data = _pack7(query.data_ptr(), out.data_ptr(), 0 if ws is None else ws.data_ptr(), k_cache.data_ptr(),
                       v_cache.data_ptr(), page_table.data_ptr(), lengths.data_ptr()) + tail
         if _direct(_DIRECT["paged_attn"], data, index) == OK:
@@ -509,8 +531,8 @@ def paged_attention(query, k_cache, v_cache, page_table, lengths, scale=None):
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             desc.workspace, desc.workspace_bytes = ws.data_ptr(), nbytes
         _run("paged_attention", lib.cmpx_paged_attn, desc, dev)
-        if sig is not None and used is query:
-            _keep(sig, (bytes(desc)[56:], nbytes, dev.index))
+        if sig is not None and used is query and _is_like(out, query):
+            _keep(sig, (bytes(desc)[56:], _alike((nbytes,), torch.uint8, dev) if nbytes else None, dev.index))
     return out
 
 
@@ -589,8 +611,8 @@ def linear_w4(input, weight, scales, zeros=None, bias=None):
     except (AttributeError, TypeError):
         sig = how = None
     if how is not None:
-        tail, shape, index = how
-        y = torch.empty(shape, dtype=input.dtype, device=input.device)
+        tail, like, index = how
+        y = torch.empty_like(like)
         data = _pack6(input.data_ptr(), weight.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(),
                       0 if bias is None else bias.data_ptr(), y.data_ptr()) + tail
         if _direct(_DIRECT["linear_w4"], data, index) == OK:
@@ -602,7 +624,7 @@ def linear_w4(input, weight, scales, zeros=None, bias=None):
         _run("linear_w4", lib.cmpx_linear_w4, desc, y.device)
         if (sig is not None and used[0].data_ptr() == input.data_ptr()
                 and all(a is b for a, b in zip(used[1:], (weight, scales, zeros, bias)))):
-            _keep(sig, (bytes(desc)[48:], shape, y.device.index))
+            _keep(sig, (bytes(desc)[48:], _alike(shape, y.dtype, y.device), y.device.index))
     return y.view(shape)
 
 
