@@ -72,9 +72,23 @@ def test_every_short_length(cuda_device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
-@pytest.mark.parametrize("lengths", [[20000], [9000, 3, 0, 1200], [0, 0, 0], [1] * 700, [4096] * 3, [130, 129, 128] * 30])
-def test_shares_of_every_shape(cuda_device, dtype, lengths):
-    Case(dtype, 8, 2, 64, 16, lengths, seed=len(lengths)).check()
+@pytest.mark.parametrize("lengths,schedule", [
+    ([20000], "equal shares"), ([9000, 3, 0, 1200], "equal shares"), ([0, 0, 0, 9000], "equal shares"),
+    ([600] * 200, "equal shares"), ([1, 0, 1300, 17] * 40, "equal shares"),
+    ([0, 0, 0], "one CTA"), ([1] * 700, "one CTA"), ([130, 129, 128] * 30, "one CTA"), ([500] * 200, "one CTA"),
+    ([4096] * 3, "cluster"), ([513], "cluster"), ([8192], "cluster"), ([600, 0, 1, 599], "cluster"), ([2000, 15] * 4, "cluster")])
+def test_every_schedule(cuda_device, dtype, lengths, schedule):
+    c = Case(dtype, 8, 2, 64, 16, lengths, seed=len(lengths))
+    assert schedule in N.paged_attention_plan(*c.args)
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("H,Hkv,D", [(1, 1, 8), (8, 8, 40), (32, 8, 128), (5, 1, 96), (12, 2, 80), (16, 1, 160), (40, 2, 192),
+                                     (8, 2, 256), (33, 1, 128)])
+@pytest.mark.parametrize("lengths", [[3000, 1], [9500]])
+def test_head_layouts_of_long_caches(cuda_device, dtype, H, Hkv, D, lengths):
+    Case(dtype, H, Hkv, D, 16, lengths, seed=H + D + 1).check()
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)

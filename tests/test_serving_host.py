@@ -225,7 +225,9 @@ def _attn(dtype=2, H=8, B=3, scale=0.1, **cache):
 def test_paged_attention_plans_and_statuses():
     f = N.lib.cmpx_paged_attn_plan
     assert _status(f, _attn()) == (N.OK, "paged_attn<one CTA per item>")
+    assert _status(f, _attn(width=200)) == (N.OK, "paged_attn<cluster per item>")
     assert _status(f, _attn(width=1000)) == (N.OK, "paged_attn<equal shares, join>")
+    assert _status(f, _attn(width=200, B=300)) == (N.OK, "paged_attn<equal shares, join>")
     assert _status(f, _attn(dtype=3))[0] == N.ERR_UNSUPPORTED_DTYPE
     for bad in (dict(H=7), dict(scale=float("nan")), dict(page=0), dict(Hkv=0, H=0), dict(pages=-1), dict(ptr=None)):
         assert _status(f, _attn(**bad))[0] == N.ERR_INVALID_ARGUMENT, bad

@@ -57,14 +57,6 @@ struct W4Args {
 // Where groups may end: at multiples of 128 k, of 64 k, or of 32 k.
 enum GroupKind { kGroup128 = 0, kGroup64 = 1, kGroup32 = 2 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 // c = (FIRST ? 0 : c) + A B
 template <int DT, bool FIRST>
 __device__ __forceinline__ void mma_w4(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,

@@ -1,5 +1,5 @@
 // paged_attn.cu -- attention of one new token per sequence over a paged key-value cache, B200 sm_100a:
-// the choice of schedule, the fp32 kernel over the keys (fp16 / bf16: paged_attn_mma.cu) and the join.
+// the choice of schedule and the join (the kernels over the keys: paged_attn_mma.cu, paged_attn_f32.cu).
 //
 //   o[b, h] = sum_t p_t V[t] / sum_t p_t,   p_t = exp(q[b, h] . K[t] * scale - m),  t < lengths[b],
 // with the maximum m and both sums carried along (one pass over the keys).
@@ -18,221 +18,7 @@
 namespace cmpx {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kJoinThreads = 256;
-
-// Group of LPT lanes per key; a lane holds NV vectors of 4 values of the key's row.  Each lane group
-// runs its own online softmax over its keys; the groups are joined at the end of a stretch, and with
-// WHOLE (a CTA per item, its keys shared by the warps) the warps, too.
-template <int LPT, int HG>
-struct Ffma {
-  static constexpr int NV = 2;
-  static constexpr int KEYS = 32 / LPT;  // keys per warp and step
-  static constexpr int STEPS = 2;        // steps whose loads are issued together
-  static constexpr int VB = 16;
-};
-
-template <int LPT, int HG, bool WHOLE>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(const __grid_constant__ PagedArgs a) {
-  using C = Ffma<LPT, HG>;
-  constexpr int DT = CMPX_F32;
-  constexpr int NV = C::NV, KEYS = C::KEYS, STEPS = C::STEPS, VB = C::VB;
-  __shared__ int64_t scratch[33 + 2 * kWarps];
-  __shared__ float sm_ml[kWarps][HG][2];
-  extern __shared__ float sm_o[];  // [kWarps][HG][head_dim]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int sub = lane % LPT, slot = lane / LPT;
-  pdl_allow_dependents();
-
-  Share share{};
-  bool more = true;
-  Stretch st;
-  if (WHOLE) {
-    st = whole_item(a, blockIdx.x);
-  } else {
-    share = find_share<kWarps>(a, scratch);
-    more = next_stretch(a, share, st);
-  }
-  constexpr int kStep = (WHOLE ? kWarps : 1) * KEYS * STEPS;
-  int col[NV];
-  bool in[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    col[i] = 4 * (sub + LPT * i);
-    in[i] = col[i] < a.head_dim;
-  }
-  while (more) {
-    float q[HG][NV][4], o[HG][NV][4], m[HG], l[HG];
-#pragma unroll
-    for (int h = 0; h < HG; ++h) {
-      m[h] = -INFINITY;
-      l[h] = 0.f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) q[h][i][e] = o[h][i][e] = 0.f;
-        if (h < st.nh && in[i]) {
-          const uint8_t* p = a.q + st.b * a.q_sb + (st.h0 + h) * a.q_sh + col[i] * elt_size(DT);
-          unpack_vec<DT, VB>(*reinterpret_cast<const RawVec<VB>*>(p), q[h][i]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) q[h][i][e] *= a.scale_log2;
-        }
-      }
-    }
-    bool bad = st.bad;
-    const int32_t* table = a.table + st.b * a.table_stride;
-    const uint8_t* kb = a.kc + st.kvh * a.kc_sh;
-    const uint8_t* vb = a.vc + st.kvh * a.vc_sh;
-    for (int t0 = st.key0 + (WHOLE ? warp * KEYS * STEPS : 0); t0 < st.key1; t0 += kStep) {
-      RawVec<VB> kr[STEPS][NV], vr[STEPS][NV];
-      bool valid[STEPS];
-#pragma unroll
-      for (int u = 0; u < STEPS; ++u) {
-        const int t = t0 + u * KEYS + slot;
-        valid[u] = t < st.key1;
-        int id = 0, row = 0;
-        if (valid[u]) {
-          const uint32_t page = fast_div(t, a.page);
-          row = t - page * a.page.d;
-          id = __ldg(table + page);
-          if (id < 0 || id >= a.num_pages) {
-            bad = true;
-            valid[u] = false;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          kr[u][i] = RawVec<VB>{};
-          vr[u][i] = RawVec<VB>{};
-          if (valid[u] && in[i]) {
-            kr[u][i] = *reinterpret_cast<const RawVec<VB>*>(kb + id * a.kc_sp + row * a.kc_st + col[i] * elt_size(DT));
-            vr[u][i] = *reinterpret_cast<const RawVec<VB>*>(vb + id * a.vc_sp + row * a.vc_st + col[i] * elt_size(DT));
-          }
-        }
-      }
-      float s[STEPS][HG];
-#pragma unroll
-      for (int u = 0; u < STEPS; ++u) {
-        float k[NV][4];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) unpack_vec<DT, VB>(kr[u][i], k[i]);
-#pragma unroll
-        for (int h = 0; h < HG; ++h) {
-          float x = 0.f;
-#pragma unroll
-          for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x = fmaf(q[h][i][e], k[i][e], x);
-#pragma unroll
-          for (int off = LPT / 2; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
-          s[u][h] = valid[u] ? x : -INFINITY;
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < HG; ++h) {
-        float top = m[h];
-#pragma unroll
-        for (int u = 0; u < STEPS; ++u) top = fmaxf(top, s[u][h]);
-        const float base = top == -INFINITY ? 0.f : top;  // no key yet: exp2(-inf - 0) = 0
-        const float keep = ex2_approx(m[h] - base);
-        m[h] = top;
-        l[h] *= keep;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[h][i][e] *= keep;
-#pragma unroll
-        for (int u = 0; u < STEPS; ++u) {
-          s[u][h] = ex2_approx(s[u][h] - base);
-          l[h] += s[u][h];
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < STEPS; ++u) {
-        float v[NV][4];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) unpack_vec<DT, VB>(vr[u][i], v[i]);
-#pragma unroll
-        for (int h = 0; h < HG; ++h)
-#pragma unroll
-          for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[h][i][e] = fmaf(s[u][h], v[i][e], o[h][i][e]);
-      }
-    }
-#pragma unroll
-    for (int h = 0; h < HG; ++h) {
-#pragma unroll
-      for (int off = LPT; off < 32; off <<= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m[h], off);
-        const float top = fmaxf(m[h], m2), base = top == -INFINITY ? 0.f : top;
-        const float w1 = ex2_approx(m[h] - base), w2 = ex2_approx(m2 - base);
-        l[h] = l[h] * w1 + __shfl_xor_sync(0xffffffffu, l[h], off) * w2;
-        m[h] = top;
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            o[h][i][e] = o[h][i][e] * w1 + __shfl_xor_sync(0xffffffffu, o[h][i][e], off) * w2;
-      }
-    }
-    if constexpr (WHOLE) {
-      bad = __syncthreads_or(bad);
-      if (bad && threadIdx.x == 0) atomicOr(a.flags, CMPX_DEVFLAG_BAD_PAGE);
-#pragma unroll
-      for (int h = 0; h < HG; ++h) {
-        if (lane == 0) {
-          sm_ml[warp][h][0] = m[h];
-          sm_ml[warp][h][1] = l[h];
-        }
-        if (slot == 0)
-#pragma unroll
-          for (int i = 0; i < NV; ++i)
-            if (in[i])
-#pragma unroll
-              for (int e = 0; e < 4; ++e) sm_o[(warp * HG + h) * a.head_dim + col[i] + e] = o[h][i][e];
-      }
-      __syncthreads();
-      for (int x = threadIdx.x; x < st.nh * a.head_dim; x += kThreads) {
-        const int h = x / a.head_dim, d = x - h * a.head_dim;
-        float top = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_ml[w][h][0]);
-        const float base = top == -INFINITY ? 0.f : top;
-        float sum = 0.f, acc = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float weight = ex2_approx(sm_ml[w][h][0] - base);
-          sum = fmaf(weight, sm_ml[w][h][1], sum);
-          acc = fmaf(weight, sm_o[(w * HG + h) * a.head_dim + d], acc);
-        }
-        if (bad) sum = __int_as_float(0x7fffffff);
-        *reinterpret_cast<float*>(a.o + st.b * a.o_sb + (st.h0 + h) * a.o_sh + d * 4) = sum == 0.f ? 0.f : acc / sum;
-      }
-      break;
-    }
-    bad = __any_sync(0xffffffffu, bad);
-    if (bad && lane == 0) atomicOr(a.flags, CMPX_DEVFLAG_BAD_PAGE);
-#pragma unroll
-    for (int h = 0; h < HG; ++h) {
-      if (h >= st.nh || slot != 0) continue;
-      const float sum = bad ? __int_as_float(0x7fffffff) : l[h];
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      const int64_t row = st.slot * a.item_heads + h;
-      if (st.slot >= 0 && sub == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * row) = make_float2(m[h], sum);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (!in[i]) continue;
-        float* p = st.slot < 0 ? reinterpret_cast<float*>(a.o + st.b * a.o_sb + (st.h0 + h) * a.o_sh) + col[i]
-                               : a.part_o + row * a.head_dim + col[i];
-        const float f = st.slot < 0 ? inv : 1.f;
-        *reinterpret_cast<float4*>(p) = make_float4(o[h][i][0] * f, o[h][i][1] * f, o[h][i][2] * f, o[h][i][3] * f);
-      }
-    }
-    more = next_stretch(a, share, st);
-  }
-}
 
 // Loads of what the main kernel wrote: from L2, and, being volatile, never moved above pdl_wait().
 __device__ __forceinline__ float2 load_part2(const float* p) {
@@ -356,51 +142,43 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
 struct Schedule {
   int item_heads, items_per_head;
   int64_t items;
-  bool whole_items;  // a CTA per item, no join
+  int ranks;        // CTAs per whole item, 0: equal shares and a join
   int ctas;
-  int64_t workers;
+  int64_t workers;  // warps with shares
 };
 
-constexpr int kF32CtasPerSm = 2;
-constexpr int kWholeKeys = 256;  // longest table of which a CTA takes an item alone
+// Keys per CTA up to which whole items are taken whatever their number, and up to which they are where all
+// CTAs fit on the GPU at once.
+constexpr int kWholeKeys = 512;
+constexpr int kClusterKeys = 1024;
 
 Schedule schedule(const cmpx_paged_attn_desc* d, int num_sms) {
-  Schedule s;
+  Schedule s{};
   const bool f32 = d->dtype == CMPX_F32;
-  const int64_t group = d->heads / d->cache.heads_kv, most_heads = f32 ? 4 : 16;
+  const int64_t group = d->heads / d->cache.heads_kv, most_heads = f32 ? 8 : 16;
   // the fewest items of at most most_heads heads, and their heads shared out evenly
   s.items_per_head = static_cast<int>(std::max<int64_t>(1, (group + most_heads - 1) / most_heads));
   s.item_heads = static_cast<int>((group + s.items_per_head - 1) / s.items_per_head);
   s.items = d->batch * d->cache.heads_kv * s.items_per_head;
-  const int64_t keys = d->cache.table_width * d->cache.page_size;
-  s.whole_items = keys <= kWholeKeys;
-  const int64_t slots = static_cast<int64_t>(num_sms) * (f32 ? kF32CtasPerSm : paged_mma_ctas_per_sm(d->cache.head_dim));
+  const int64_t keys = d->cache.table_width * d->cache.page_size;  // of the longest sequence there can be
+  const int64_t slots = static_cast<int64_t>(num_sms) * (f32 ? paged_f32_ctas_per_sm() : paged_mma_ctas_per_sm(d->cache.head_dim));
+  // Whole items, by one CTA or a cluster of 2, 4 or 8 (256 keys each, as far as the CTAs fit on the GPU): one
+  // launch and no join.
+  int ranks = 1;
+  while (ranks < 8 && keys > 256 * ranks && s.items * ranks * 2 <= slots) ranks *= 2;
+  if (keys <= kWholeKeys || (keys <= kClusterKeys * ranks && s.items * ranks <= slots)) {
+    s.ranks = ranks;
+    s.ctas = static_cast<int>(s.items * ranks);
+    return s;
+  }
   const int64_t units = s.items * (std::max<int64_t>(1, (keys + kTile - 1) / kTile) + kItemCost);
-  s.ctas = static_cast<int>(s.whole_items ? s.items
-                                          : std::max<int64_t>(1, std::min(slots, (units + kShareMin - 1) / kShareMin)));
-  s.workers = static_cast<int64_t>(s.ctas) * (f32 ? kWarps : kPagedMmaWarps);
+  s.ctas = static_cast<int>(std::max<int64_t>(1, std::min(slots, (units + kShareMin - 1) / kShareMin)));
+  s.workers = static_cast<int64_t>(s.ctas) * kPagedWarps;
   return s;
 }
 
 size_t part_floats(const cmpx_paged_attn_desc* d, const Schedule& s) {
-  return s.whole_items ? 0 : 2ull * s.workers * s.item_heads * (d->cache.head_dim + 2);
-}
-
-template <int LPT, int HG>
-int launch_f32(const PagedArgs& a, int ctas, bool whole_items, const LaunchCtx& ctx) {
-  const int smem = kWarps * HG * a.head_dim * static_cast<int>(sizeof(float));
-  if (whole_items)
-    paged_attn_kernel<LPT, HG, true><<<ctas, kThreads, smem, ctx.stream>>>(a);
-  else
-    paged_attn_kernel<LPT, HG, false><<<ctas, kThreads, 0, ctx.stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
-}
-
-int launch_f32(const PagedArgs& a, int ctas, bool whole, const LaunchCtx& ctx) {
-#define CMPX_PAGED(LPT) \
-  (a.item_heads == 1 ? launch_f32<LPT, 1>(a, ctas, whole, ctx) : launch_f32<LPT, 4>(a, ctas, whole, ctx))
-  return a.head_dim <= 64 ? CMPX_PAGED(8) : a.head_dim <= 128 ? CMPX_PAGED(16) : CMPX_PAGED(32);
-#undef CMPX_PAGED
+  return s.ranks ? 0 : 2ull * s.workers * s.item_heads * (d->cache.head_dim + 2);
 }
 
 template <int DT>
@@ -437,7 +215,11 @@ const char* paged_attn_plan(const cmpx_paged_attn_desc* d, int* status) {
   *status = CMPX_ERR_UNSUPPORTED_SHAPE;
   if (d->heads > (1 << 20) || d->batch > (1 << 20) || d->batch * d->heads > (1ll << 31) - 65536) return "none";
   *status = CMPX_OK;
-  return schedule(d, 148).whole_items ? "paged_attn<one CTA per item>" : "paged_attn<equal shares, join>";
+  switch (schedule(d, current_num_sms()).ranks) {
+    case 0: return "paged_attn<equal shares, join>";
+    case 1: return "paged_attn<one CTA per item>";
+    default: return "paged_attn<cluster per item>";
+  }
 }
 
 size_t paged_attn_workspace_bytes(const cmpx_paged_attn_desc* d, int num_sms) {
@@ -490,9 +272,9 @@ int launch_paged_attn(const cmpx_paged_attn_desc* d, const LaunchCtx& ctx) {
     a.part_o = static_cast<float*>(d->workspace);
     a.part_ml = a.part_o + 2ull * s.workers * s.item_heads * c.head_dim;
   }
-  const int st = d->dtype == CMPX_F32 ? launch_f32(a, s.ctas, s.whole_items, ctx)
-                                        : launch_paged_mma(a, d->dtype, s.ctas, s.whole_items, ctx);
-  if (st != CMPX_OK || s.whole_items) return st;
+  const int st = d->dtype == CMPX_F32 ? launch_paged_f32(a, s.ctas, s.ranks, ctx)
+                                      : launch_paged_mma(a, d->dtype, s.ctas, s.ranks, ctx);
+  if (st != CMPX_OK || s.ranks) return st;
   if (d->dtype == CMPX_F32) return launch_join<CMPX_F32>(a, ctx);
   if (d->dtype == CMPX_F16) return launch_join<CMPX_F16>(a, ctx);
   return launch_join<CMPX_BF16>(a, ctx);

@@ -5,15 +5,14 @@
 // at a time, K and V fragments straight from shared memory (ldmatrix, transposed for V).  The
 // products are a few percent of what the tensor cores do even in this form; what bounds the kernel is the
 // one read of K and V, so it is built around loads in flight:
-//   * every warp runs its own pipeline of STAGES buffers of 16 keys, filled by 16-byte cp.async whose
-//     rows are found through the page table one by one (a page may end inside the 16 keys), and its own
+//   * every warp runs its own pipeline of STAGES buffers of 16 keys (KeyPipe, paged_schedule.cuh) and its own
 //     online softmax over its own share of the keys.  Nothing in a share waits for another warp, so one
 //     warp's first loads of an item hide behind the others' stream (with one share for a CTA's four
 //     warps, which met at the end of each item, [32, 32 heads, 8 key heads, 128] bf16 with 64 to 8192 keys took 81 us);
-//   * WHOLE (caches so short that a CTA takes an item): the CTA's warps share the item's keys and meet once;
+//   * WHOLE (short caches): a CTA, or a cluster of up to 8, takes an item; the warps share its keys, meet once
+//     and join their results through (distributed) shared memory, without a second kernel;
 //   * rows of a buffer are swizzled in 16-byte chunks (chunk ^ row % 8): ldmatrix reads without bank
-//     conflicts, and nothing is padded;
-//   * keys behind the stretch, pages that do not exist and columns behind head_dim are filled with zeros.
+//     conflicts, and nothing is padded.
 // P is used as the sum of two 16-bit parts (cut off, and the rounded rest), so the weights carry 16 bits
 // and more; a second product of P V costs nothing here, and one part alone would add as much error as the
 // output's rounding does.  The rest is kept above zero, so that an infinite value stays infinite (0 * inf is
@@ -30,18 +29,17 @@
 namespace cmpx {
 namespace {
 
-constexpr int kWarps = kPagedMmaWarps;
+constexpr int kWarps = kPagedWarps;
 constexpr int kThreads = kWarps * 32;
 constexpr int kKeys = 16;  // keys per buffer
 
 template <int DP>
 struct MmaCfg {
   static constexpr int ROW = DP * 2;                     // bytes of a row
-  static constexpr int CHUNKS = DP / 8;                  // 16-byte chunks of a row
-  static constexpr int STAGE = 2 * kKeys * ROW;          // K and V
   static constexpr int STAGES = DP == 64 ? 6 : DP == 192 ? 2 : 3;
   static constexpr int CTAS = DP == 256 ? 1 : 2;         // per SM: 96 KB of buffers each (192 KB at 256)
-  static constexpr int SMEM = kWarps * STAGES * STAGE;
+  using Pipe = KeyPipe<ROW, kKeys, STAGES, true>;
+  static constexpr int SMEM = kWarps * Pipe::BYTES;
   static_assert(SMEM >= kWarps * 16 * DP * 4, "the warps' outputs are joined in the buffers");
 };
 
@@ -73,15 +71,6 @@ __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
                  : "memory");
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return DT == CMPX_BF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
@@ -104,18 +93,19 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<DP>::CTAS) paged_attn_mma_ker
   constexpr float kBias = DT == CMPX_F16 ? 14.f : 0.f;
   constexpr float kLeast = DT == CMPX_F16 ? 0x1p-24f : 0x1p-126f;  // the types' smallest (normal) values
   __shared__ int64_t scratch[33 + 2 * kWarps];
-  __shared__ float sm_ml[kWarps][16][2];
+  __shared__ float2 sm_ml[kWarps][16];
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gr = lane >> 2, tq = lane & 3;  // fragment row and column pair
-  const uint32_t buf = smem_u32(smem) + warp * C::STAGES * C::STAGE;
+  typename C::Pipe pipe(a, smem_u32(smem) + warp * C::Pipe::BYTES, a.head_dim * 2);
   pdl_allow_dependents();
 
   Share share{};
   bool more = true;
   Stretch st;
   if (WHOLE) {
-    st = whole_item(a, blockIdx.x);
+    const int ranks = cluster_size();
+    st = whole_item(a, blockIdx.x / ranks, cluster_rank(), ranks);
   } else {
     share = find_share<kWarps>(a, scratch);
     more = next_stretch(a, share, st);
@@ -128,6 +118,9 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<DP>::CTAS) paged_attn_mma_ker
   const int v_row = (lane & 7) + (((lane >> 3) & 1) << 3), v_chunk = lane >> 4;
 
   while (more) {
+    const int subs = pipe.begin(st);
+#pragma unroll
+    for (int i = 0; i < C::STAGES - 1; ++i) pipe.issue(first + i * kStep, subs, i);
     uint32_t q[DP / 16][4];
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s)
@@ -144,49 +137,12 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<DP>::CTAS) paged_attn_mma_ker
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    bool bad = st.bad;
-    const int32_t* table = a.table + st.b * a.table_stride;
-    const uint8_t* kb = a.kc + st.kvh * a.kc_sh;
-    const uint8_t* vb = a.vc + st.kvh * a.vc_sh;
-
-    const int subs = (st.key1 - st.key0 + kKeys - 1) / kKeys;
-    // Starts the loads of the 16 keys of sub-tile i (nothing behind the last) and closes the group.
-    auto issue = [&](int i, int stage) {
-      if (i < subs) {
-        const int t = st.key0 + i * kKeys + (lane & 15);
-        int64_t ko = -1, vo = -1;
-        if (t < st.key1) {
-          const uint32_t page = fast_div(t, a.page);
-          const int row = t - page * a.page.d;
-          const int id = __ldg(table + page);
-          if (id >= 0 && id < a.num_pages) {
-            ko = id * a.kc_sp + row * a.kc_st;
-            vo = id * a.vc_sp + row * a.vc_st;
-          } else {
-            bad = true;
-          }
-        }
-        const uint32_t base = buf + stage * C::STAGE;
-#pragma unroll
-        for (int j = 0; j < kKeys * C::CHUNKS / 32; ++j) {
-          const int idx = j * 32 + lane, r = idx / C::CHUNKS, ch = idx % C::CHUNKS;
-          const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
-          const bool there = kr >= 0 && ch * 8 < a.head_dim;
-          const uint32_t dst = base + r * C::ROW + ((ch ^ (r & 7)) << 4);
-          cp_async16(dst, there ? kb + kr + ch * 16 : a.q, there ? 16 : 0);
-          cp_async16(dst + kKeys * C::ROW, there ? vb + vr + ch * 16 : a.q, there ? 16 : 0);
-        }
-      }
-      cp_async_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < C::STAGES - 1; ++i) issue(first + i * kStep, i);
     int stage = 0;
     for (int sub = first; sub < subs; sub += kStep) {
       cp_async_wait<C::STAGES - 2>();
       __syncwarp();  // this buffer is filled, and everybody is done with the one before it
-      issue(sub + (C::STAGES - 1) * kStep, stage == 0 ? C::STAGES - 1 : stage - 1);
-      const uint32_t kbuf = buf + stage * C::STAGE, vbuf = kbuf + kKeys * C::ROW;
+      pipe.issue(sub + (C::STAGES - 1) * kStep, subs, stage == 0 ? C::STAGES - 1 : stage - 1);
+      const uint32_t kbuf = pipe.buf + stage * C::Pipe::STAGE, vbuf = kbuf + kKeys * C::ROW;
       stage = stage + 1 == C::STAGES ? 0 : stage + 1;
 
       float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -256,45 +212,25 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<DP>::CTAS) paged_attn_mma_ker
     }
     if constexpr (WHOLE) {
       // the warps' results, through the buffers
-      bad = __syncthreads_or(bad);
+      const bool bad = __syncthreads_or(pipe.bad);
+      if (bad && threadIdx.x == 0) atomicOr(a.flags, CMPX_DEVFLAG_BAD_PAGE);
       float* sm_o = reinterpret_cast<float*>(smem);
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int h = gr + 8 * r;
         if (h >= st.nh) continue;
-        if (tq == 0) {
-          sm_ml[warp][h][0] = m[r];
-          sm_ml[warp][h][1] = l[r];
-        }
+        if (tq == 0) sm_ml[warp][h] = make_float2(m[r], bad ? __int_as_float(0x7fffffff) : l[r]);
 #pragma unroll
         for (int i = 0; i < DP / 8; ++i)
           *reinterpret_cast<float2*>(sm_o + (warp * 16 + h) * DP + i * 8 + tq * 2) =
               make_float2(o[i][2 * r], o[i][2 * r + 1]);
       }
-      __syncthreads();
-      for (int x = threadIdx.x; x < st.nh * (DP / 2); x += kThreads) {
-        const int h = x / (DP / 2), d = 2 * (x - h * (DP / 2));
-        if (d >= a.head_dim) continue;
-        float top = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm_ml[w][h][0]);
-        const float base = top == -INFINITY ? 0.f : top;
-        float sum = 0.f, x0 = 0.f, x1 = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float weight = ex2_approx(sm_ml[w][h][0] - base);
-          const float2 v = *reinterpret_cast<const float2*>(sm_o + (w * 16 + h) * DP + d);
-          sum = fmaf(weight, sm_ml[w][h][1], sum);
-          x0 = fmaf(weight, v.x, x0);
-          x1 = fmaf(weight, v.y, x1);
-        }
-        const float inv = bad ? __int_as_float(0x7fffffff) : sum == 0.f ? 0.f : 1.f / sum;
-        *reinterpret_cast<uint32_t*>(a.o + st.b * a.o_sb + (st.h0 + h) * a.o_sh + d * 2) = pack2<DT>(x0 * inv, x1 * inv);
-      }
-      if (bad && threadIdx.x == 0) atomicOr(a.flags, CMPX_DEVFLAG_BAD_PAGE);
+      join_cluster<kWarps, 16, DP>(st.nh, a.head_dim, smem_u32(sm_o), smem_u32(sm_ml), [&](int h, int d, float x, float y) {
+        *reinterpret_cast<uint32_t*>(a.o + st.b * a.o_sb + (st.h0 + h) * a.o_sh + d * 2) = pack2<DT>(x, y);
+      });
       break;
     }
-    bad = __any_sync(0xffffffffu, bad);
+    const bool bad = __any_sync(0xffffffffu, pipe.bad);
     if (bad && lane == 0) atomicOr(a.flags, CMPX_DEVFLAG_BAD_PAGE);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -322,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<DP>::CTAS) paged_attn_mma_ker
 }
 
 template <int DT, int DP, bool WHOLE>
-int launch(const PagedArgs& a, int ctas, const LaunchCtx& ctx) {
+int launch(const PagedArgs& a, int ctas, int ranks, const LaunchCtx& ctx) {
   auto kernel = paged_attn_mma_kernel<DT, DP, WHOLE>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
@@ -332,26 +268,27 @@ int launch(const PagedArgs& a, int ctas, const LaunchCtx& ctx) {
     attr_err[dev & 63] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MmaCfg<DP>::SMEM);
   });
   if (attr_err[dev & 63] != cudaSuccess) return CMPX_ERR_LAUNCH;
+  if (WHOLE) return launch_whole(kernel, a, ctas, ranks, kThreads, MmaCfg<DP>::SMEM, ctx.stream);
   kernel<<<ctas, kThreads, MmaCfg<DP>::SMEM, ctx.stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
 }
 
 template <int DT, bool WHOLE>
-int launch_dt(const PagedArgs& a, int ctas, const LaunchCtx& ctx) {
-  if (a.head_dim <= 64) return launch<DT, 64, WHOLE>(a, ctas, ctx);
-  if (a.head_dim <= 128) return launch<DT, 128, WHOLE>(a, ctas, ctx);
-  if (a.head_dim <= 192) return launch<DT, 192, WHOLE>(a, ctas, ctx);
-  return launch<DT, 256, WHOLE>(a, ctas, ctx);
+int launch_dt(const PagedArgs& a, int ctas, int ranks, const LaunchCtx& ctx) {
+  if (a.head_dim <= 64) return launch<DT, 64, WHOLE>(a, ctas, ranks, ctx);
+  if (a.head_dim <= 128) return launch<DT, 128, WHOLE>(a, ctas, ranks, ctx);
+  if (a.head_dim <= 192) return launch<DT, 192, WHOLE>(a, ctas, ranks, ctx);
+  return launch<DT, 256, WHOLE>(a, ctas, ranks, ctx);
 }
 
 }  // namespace
 
 int paged_mma_ctas_per_sm(int64_t head_dim) { return head_dim > 192 ? MmaCfg<256>::CTAS : MmaCfg<128>::CTAS; }
 
-int launch_paged_mma(const PagedArgs& a, int dtype, int ctas, bool whole_items, const LaunchCtx& ctx) {
+int launch_paged_mma(const PagedArgs& a, int dtype, int ctas, int ranks, const LaunchCtx& ctx) {
   if (dtype == CMPX_BF16)
-    return whole_items ? launch_dt<CMPX_BF16, true>(a, ctas, ctx) : launch_dt<CMPX_BF16, false>(a, ctas, ctx);
-  return whole_items ? launch_dt<CMPX_F16, true>(a, ctas, ctx) : launch_dt<CMPX_F16, false>(a, ctas, ctx);
+    return ranks ? launch_dt<CMPX_BF16, true>(a, ctas, ranks, ctx) : launch_dt<CMPX_BF16, false>(a, ctas, ranks, ctx);
+  return ranks ? launch_dt<CMPX_F16, true>(a, ctas, ranks, ctx) : launch_dt<CMPX_F16, false>(a, ctas, ranks, ctx);
 }
 
 }  // namespace cmpx

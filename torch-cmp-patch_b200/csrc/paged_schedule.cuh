@@ -175,22 +175,146 @@ __device__ __forceinline__ bool next_stretch(const PagedArgs& a, Share& s, Stret
   return false;
 }
 
-// An item as one stretch (a CTA for each, no join).
-__device__ __forceinline__ Stretch whole_item(const PagedArgs& a, int64_t index) {
+// Part `rank` of `ranks` of an item's keys as one stretch (a CTA or a cluster of CTAs per item, no join).
+__device__ __forceinline__ Stretch whole_item(const PagedArgs& a, int64_t index, int rank, int ranks) {
   const int items = a.heads_kv * a.items_per_head;
   Stretch st;
   st.b = static_cast<int>(index / items);
   stretch_heads(a, static_cast<int>(index - static_cast<int64_t>(st.b) * items), st);
-  st.key0 = 0;
-  st.key1 = seq_len(a, st.b, st.bad);
+  const int n = seq_len(a, st.b, st.bad);
+  const int64_t tiles = (n + kTile - 1) / kTile;
+  st.key0 = static_cast<int>(tiles * rank / ranks) * kTile;
+  st.key1 = min(n, static_cast<int>(tiles * (rank + 1) / ranks) * kTile);
   st.slot = -1;
   return st;
 }
 
-// The kernel over the keys for fp16 / bf16 (paged_attn_mma.cu): items of up to 16 heads.
-constexpr int kPagedMmaWarps = 4;
+// A warp's pipeline over the keys of a stretch: STAGES buffers of KEYS keys and values in shared memory,
+// ROW bytes each, filled by 16-byte cp.async.  The rows are found through the page table one by one (a page may
+// end inside a buffer).  With SWIZZLE the 16-byte chunks of row r lie at chunk ^ (r % 8).  Keys behind
+// the stretch, pages that do not exist and columns behind head_dim are filled with zeros.
+template <int ROW, int KEYS, int STAGES, bool SWIZZLE>
+struct KeyPipe {
+  static constexpr int CHUNKS = ROW / 16;
+  static constexpr int STAGE = 2 * KEYS * ROW;
+  static constexpr int BYTES = STAGES * STAGE;  // per warp
+
+  const PagedArgs& a;
+  const int32_t* table;
+  const uint8_t *kb, *vb;
+  int key0, key1, row_chunks;
+  uint32_t buf;
+  bool bad;
+
+  __device__ __forceinline__ KeyPipe(const PagedArgs& args, uint32_t buffers, int row_bytes)
+      : a(args), row_chunks(row_bytes / 16), buf(buffers) {}
+
+  __device__ __forceinline__ int begin(const Stretch& st) {  // the stretch's count of buffers
+    table = a.table + st.b * a.table_stride;
+    kb = a.kc + st.kvh * a.kc_sh;
+    vb = a.vc + st.kvh * a.vc_sh;
+    key0 = st.key0;
+    key1 = st.key1;
+    bad = st.bad;
+    return (key1 - key0 + KEYS - 1) / KEYS;
+  }
+  // Starts the loads of buffer i of `count` (nothing behind the last) and closes the group.
+  __device__ __forceinline__ void issue(int i, int count, int stage) {
+    const int lane = threadIdx.x & 31;
+    if (i < count) {
+      const int t = key0 + i * KEYS + lane % KEYS;
+      int64_t ko = -1, vo = -1;
+      if (t < key1) {
+        const uint32_t page = fast_div(t, a.page);
+        const int row = t - page * a.page.d;
+        const int id = __ldg(table + page);
+        if (id >= 0 && id < a.num_pages) {
+          ko = id * a.kc_sp + row * a.kc_st;
+          vo = id * a.vc_sp + row * a.vc_st;
+        } else {
+          bad = true;
+        }
+      }
+      const uint32_t base = buf + stage * STAGE;
+#pragma unroll
+      for (int j = 0; j < KEYS * CHUNKS / 32; ++j) {
+        const int idx = j * 32 + lane, r = idx / CHUNKS, ch = idx % CHUNKS;
+        const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+        const bool there = kr >= 0 && ch < row_chunks;
+        const uint32_t dst = base + r * ROW + ((SWIZZLE ? ch ^ (r & 7) : ch) << 4);
+        cp_async16(dst, there ? kb + kr + ch * 16 : a.q, there ? 16 : 0);
+        cp_async16(dst + KEYS * ROW, there ? vb + vr + ch * 16 : a.q, there ? 16 : 0);
+      }
+    }
+    cp_async_commit();
+  }
+};
+
+// Joins the results of the WARPS warps of each of a cluster's CTAs, which all have the same item: outputs
+// sm_o [warp][ROWS][DP], maxima and sums sm_ml [warp][ROWS].  Every CTA does its part of the outputs;
+// store(h, d, x, y) gets two neighbouring values of head h.
+template <int WARPS, int ROWS, int DP, typename Store>
+__device__ __forceinline__ void join_cluster(int nh, int head_dim, uint32_t sm_o, uint32_t sm_ml, Store store) {
+  const int ranks = cluster_size();
+  if (ranks > 1) cluster_sync();
+  else __syncthreads();
+  for (int x = cluster_rank() * blockDim.x + threadIdx.x; x < nh * (DP / 2); x += ranks * blockDim.x) {
+    const int h = x / (DP / 2), d = 2 * (x - h * (DP / 2));
+    if (d >= head_dim) continue;
+    float top = -INFINITY, sum = 0.f, x0 = 0.f, x1 = 0.f;
+    for (int r = 0; r < ranks; ++r) {
+      float2 ml[WARPS], v[WARPS];
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        ml[w] = cluster_load_f2(sm_ml + (w * ROWS + h) * 8, r);
+        v[w] = cluster_load_f2(sm_o + ((w * ROWS + h) * DP + d) * 4, r);
+      }
+      float now = top;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) now = fmaxf(now, ml[w].x);
+      const float base = now == -INFINITY ? 0.f : now, keep = ex2_approx(top - base);
+      top = now;
+      sum *= keep;
+      x0 *= keep;
+      x1 *= keep;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float weight = ex2_approx(ml[w].x - base);
+        sum = fmaf(weight, ml[w].y, sum);
+        x0 = fmaf(weight, v[w].x, x0);
+        x1 = fmaf(weight, v[w].y, x1);
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    store(h, d, x0 * inv, x1 * inv);
+  }
+  if (ranks > 1) cluster_sync();  // nobody leaves while its results are read
+}
+
+// Launches a kernel over whole items with `ranks` CTAs per item.
+template <typename Kernel>
+int launch_whole(Kernel kernel, const PagedArgs& a, int64_t ctas, int ranks, int threads, int smem, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ranks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = ranks > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, a) == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
+}
+
+// The kernels over the keys: fp16 / bf16 items of up to 16 heads (paged_attn_mma.cu), fp32 items of up to 8
+// (paged_attn_f32.cu).  ranks: CTAs per whole item, 0 for equal shares.
+constexpr int kPagedWarps = 4;
 int paged_mma_ctas_per_sm(int64_t head_dim);
-int launch_paged_mma(const PagedArgs& a, int dtype, int ctas, bool whole_items, const LaunchCtx& ctx);
+int paged_f32_ctas_per_sm();
+int launch_paged_mma(const PagedArgs& a, int dtype, int ctas, int ranks, const LaunchCtx& ctx);
+int launch_paged_f32(const PagedArgs& a, int ctas, int ranks, const LaunchCtx& ctx);
 
 // Programmatic dependent launch: the join kernel starts while the main kernel runs, reads the
 // lengths, and waits here for the main kernel's results.
