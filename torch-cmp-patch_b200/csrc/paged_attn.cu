@@ -18,8 +18,6 @@
 namespace cmpx {
 namespace {
 
-constexpr int kJoinThreads = 256;
-
 // Loads of what the main kernel wrote: from L2, and, being volatile, never moved above pdl_wait().
 __device__ __forceinline__ float2 load_part2(const float* p) {
   float2 v;
@@ -32,18 +30,21 @@ __device__ __forceinline__ float4 load_part4(const float* p) {
   return v;
 }
 
-// Joins the partial results of one (sequence, query head): a block per row.  A warp takes every
-// kJoinWarps'th partial result: up to 32 at a time, a lane each for the maxima and sums, all lanes along
-// the head for the outputs, whose loads do not wait for the weights.
-template <int DT, int V>  // V: float4 vectors per lane and row (head_dim <= 128 V)
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedArgs a) {
-  constexpr int W = kJoinThreads / 32;
+// Joins the partial results of each (sequence, query head) row: W warps of a block per row (WROW = W), or one warp
+// per row and W rows per block (WROW = 1).  A row's warps take every WROW'th partial result: up to 32 at a
+// time, a lane each for the maxima and sums, all lanes along the head for the outputs, whose loads do not
+// wait for the weights.
+template <int DT, int V, int W, int WROW>  // V: float4 vectors per lane and row (head_dim <= 128 V)
+__global__ void __launch_bounds__(32 * W) paged_join_kernel(const __grid_constant__ PagedArgs a) {
   constexpr int AHEAD = 8;
   constexpr int ES = elt_size(DT);
   __shared__ float sm_ml[W][2];
   __shared__ float4 sm_o[W][32 * V];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.x / a.heads, h = blockIdx.x - b * a.heads;
+  const int row_index = WROW == 1 ? static_cast<int>(blockIdx.x) * W + warp : static_cast<int>(blockIdx.x);
+  const int part_warp = WROW == 1 ? 0 : warp;  // this warp among its row's
+  const bool there = row_index < a.batch * a.heads;
+  const int b = there ? row_index / a.heads : 0, h = there ? row_index - b * a.heads : 0;
   int64_t first = 0, total = 0;  // units before sequence b, and in all
   for (int i = lane; i < a.batch; i += 32) {
     const int64_t n = seq_units(a, i);
@@ -61,16 +62,16 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   const int64_t begin = first + (static_cast<int64_t>(kvh) * a.items_per_head + part) * (tiles + kItemCost) + kItemCost;
   const int64_t c0 = begin / share, c1 = (begin + tiles - 1) / share;
   pdl_wait();  // every block: this kernel is not done before the main one is
-  if (c0 == c1) return;  // written by its warp
+  if (!there || c0 == c1) return;  // written by its warp
   const int hh = g - part * a.item_heads;
   float m = -INFINITY, l = 0.f;
   float4 o[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
   auto row_of = [&](int64_t c) { return (2 * c + (c == c0 ? 1 : 0)) * a.item_heads + hh; };
-  for (int64_t cb = c0 + warp; cb <= c1; cb += 32 * W) {
-    const int64_t mine = cb + static_cast<int64_t>(lane) * W;
-    const int count = static_cast<int>(min(static_cast<int64_t>(32), (c1 - cb) / W + 1));
+  for (int64_t cb = c0 + part_warp; cb <= c1; cb += 32 * WROW) {
+    const int64_t mine = cb + static_cast<int64_t>(lane) * WROW;
+    const int count = static_cast<int>(min(static_cast<int64_t>(32), (c1 - cb) / WROW + 1));
     float2 ml = make_float2(-INFINITY, 0.f);
     if (lane < count) ml = load_part2(a.part_ml + 2 * row_of(mine));
     float top = ml.x;
@@ -95,7 +96,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
           p[k][v] = make_float4(0.f, 0.f, 0.f, 0.f);
           const int d = 4 * (lane + 32 * v);
           if (k0 + k < count && d < a.head_dim)
-            p[k][v] = load_part4(a.part_o + row_of(cb + static_cast<int64_t>(k0 + k) * W) * a.head_dim + d);
+            p[k][v] = load_part4(a.part_o + row_of(cb + static_cast<int64_t>(k0 + k) * WROW) * a.head_dim + d);
         }
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
@@ -111,6 +112,17 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
       }
     }
   }
+  uint8_t* const out = a.o + b * a.o_sb + h * a.o_sh;
+  if (WROW == 1) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int d = 4 * (lane + 32 * v);
+      const float f[4] = {o[v].x * inv, o[v].y * inv, o[v].z * inv, o[v].w * inv};
+      if (d < a.head_dim) *reinterpret_cast<RawVec<4 * ES>*>(out + d * ES) = pack_vec<DT, 4 * ES>(f);
+    }
+    return;
+  }
   if (lane == 0) {
     sm_ml[warp][0] = m;
     sm_ml[warp][1] = l;
@@ -118,7 +130,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
 #pragma unroll
   for (int v = 0; v < V; ++v) sm_o[warp][lane + 32 * v] = o[v];
   __syncthreads();
-  for (int d = threadIdx.x; d < a.head_dim; d += kJoinThreads) {
+  for (int d = threadIdx.x; d < a.head_dim; d += 32 * W) {
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < W; ++w) top = fmaxf(top, sm_ml[w][0]);
@@ -131,7 +143,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
       acc = fmaf(weight, reinterpret_cast<const float*>(sm_o[w])[d], acc);
     }
     const float r = sum == 0.f ? 0.f : acc / sum;
-    *reinterpret_cast<RawVec<ES>*>(a.o + b * a.o_sb + h * a.o_sh + d * ES) = pack_vec<DT, ES>(&r);
+    *reinterpret_cast<RawVec<ES>*>(out + d * ES) = pack_vec<DT, ES>(&r);
   }
 }
 
@@ -181,20 +193,31 @@ size_t part_floats(const cmpx_paged_attn_desc* d, const Schedule& s) {
   return s.ranks ? 0 : 2ull * s.workers * s.item_heads * (d->cache.head_dim + 2);
 }
 
-template <int DT>
-int launch_join(const PagedArgs& a, const LaunchCtx& ctx) {
+template <int DT, int V, int W, int WROW>
+int launch_join_as(const PagedArgs& a, int64_t blocks, const LaunchCtx& ctx) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.heads));
-  cfg.blockDim = dim3(kJoinThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(32 * W);
   cfg.stream = ctx.stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t err = a.head_dim <= 128 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<DT, 1>, a)
-                                            : cudaLaunchKernelEx(&cfg, paged_join_kernel<DT, 2>, a);
-  return err == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<DT, V, W, WROW>, a) == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
+}
+
+template <int DT, int V>
+int launch_join(const PagedArgs& a, int64_t most_parts, const LaunchCtx& ctx) {
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.heads;
+  if (most_parts <= 32) return launch_join_as<DT, V, 4, 1>(a, (rows + 3) / 4, ctx);
+  if (rows <= ctx.num_sms) return launch_join_as<DT, V, 16, 16>(a, rows, ctx);
+  return launch_join_as<DT, V, 4, 4>(a, rows, ctx);
+}
+
+template <int DT>
+int launch_join_dim(const PagedArgs& a, int64_t most_parts, const LaunchCtx& ctx) {
+  return a.head_dim <= 128 ? launch_join<DT, 1>(a, most_parts, ctx) : launch_join<DT, 2>(a, most_parts, ctx);
 }
 
 }  // namespace
@@ -275,9 +298,13 @@ int launch_paged_attn(const cmpx_paged_attn_desc* d, const LaunchCtx& ctx) {
   const int st = d->dtype == CMPX_F32 ? launch_paged_f32(a, s.ctas, s.ranks, ctx)
                                       : launch_paged_mma(a, d->dtype, s.ctas, s.ranks, ctx);
   if (st != CMPX_OK || s.ranks) return st;
-  if (d->dtype == CMPX_F32) return launch_join<CMPX_F32>(a, ctx);
-  if (d->dtype == CMPX_F16) return launch_join<CMPX_F16>(a, ctx);
-  return launch_join<CMPX_BF16>(a, ctx);
+  // The most partial results that a row can have: the longest sequence beside empty ones.
+  const int64_t tiles = (static_cast<int64_t>(a.capacity) + kTile - 1) / kTile;
+  const int64_t units = (tiles + kItemCost + (d->batch - 1) * (1 + kItemCost)) * (s.items / d->batch);
+  const int64_t most = tiles / std::max<int64_t>(kShareMin, units / s.workers) + 2;
+  if (d->dtype == CMPX_F32) return launch_join_dim<CMPX_F32>(a, most, ctx);
+  if (d->dtype == CMPX_F16) return launch_join_dim<CMPX_F16>(a, most, ctx);
+  return launch_join_dim<CMPX_BF16>(a, most, ctx);
 }
 
 }  // namespace cmpx

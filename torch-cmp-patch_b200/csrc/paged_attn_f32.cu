@@ -62,9 +62,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attn_f32_kernel(co
   const int col[2] = {4 * sub, 4 * (sub + LPT)};
 
   while (more) {
-    const int count = pipe.begin(st);
+    const int count = pipe.begin(st, first);
 #pragma unroll
-    for (int i = 0; i < C::STAGES - 1; ++i) pipe.issue(first + i * kStep, count, i);
+    for (int i = 0; i < C::STAGES - 1; ++i) pipe.issue(first + i * kStep, kStep, count, i);
     float q[HG][8], o[HG][8], m[HG], l[HG];
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attn_f32_kernel(co
     for (int at = first; at < count; at += kStep) {
       cp_async_wait<C::STAGES - 2>();
       __syncwarp();  // this buffer is filled, and everybody is done with the one before it
-      pipe.issue(at + (C::STAGES - 1) * kStep, count, stage == 0 ? C::STAGES - 1 : stage - 1);
+      pipe.issue(at + (C::STAGES - 1) * kStep, kStep, count, stage == 0 ? C::STAGES - 1 : stage - 1);
       const uint8_t* const kbuf = buffers + stage * C::Pipe::STAGE;
       stage = stage + 1 == C::STAGES ? 0 : stage + 1;
       const int left = st.key1 - st.key0 - at * C::KEYS;  // keys of this buffer

@@ -118,9 +118,9 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<DP>::CTAS) paged_attn_mma_ker
   const int v_row = (lane & 7) + (((lane >> 3) & 1) << 3), v_chunk = lane >> 4;
 
   while (more) {
-    const int subs = pipe.begin(st);
+    const int subs = pipe.begin(st, first);
 #pragma unroll
-    for (int i = 0; i < C::STAGES - 1; ++i) pipe.issue(first + i * kStep, subs, i);
+    for (int i = 0; i < C::STAGES - 1; ++i) pipe.issue(first + i * kStep, kStep, subs, i);
     uint32_t q[DP / 16][4];
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s)
@@ -141,24 +141,29 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<DP>::CTAS) paged_attn_mma_ker
     for (int sub = first; sub < subs; sub += kStep) {
       cp_async_wait<C::STAGES - 2>();
       __syncwarp();  // this buffer is filled, and everybody is done with the one before it
-      pipe.issue(sub + (C::STAGES - 1) * kStep, subs, stage == 0 ? C::STAGES - 1 : stage - 1);
+      pipe.issue(sub + (C::STAGES - 1) * kStep, kStep, subs, stage == 0 ? C::STAGES - 1 : stage - 1);
       const uint32_t kbuf = pipe.buf + stage * C::Pipe::STAGE, vbuf = kbuf + kKeys * C::ROW;
       stage = stage + 1 == C::STAGES ? 0 : stage + 1;
 
-      float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      // two chains of products for each 8 keys
+      float s[2][4], s2[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
         uint32_t b[4];
         ldmatrix4<false>(kbuf + k_row * C::ROW + (((2 * ks + k_chunk) ^ (k_row & 7)) << 4), b);
-        mma16816<DT>(s[0], q[ks], b[0], b[1]);
-        mma16816<DT>(s[1], q[ks], b[2], b[3]);
+        mma16816<DT>(ks & 1 ? s2[0] : s[0], q[ks], b[0], b[1]);
+        mma16816<DT>(ks & 1 ? s2[1] : s[1], q[ks], b[2], b[3]);
       }
       const int left = st.key1 - st.key0 - sub * kKeys;  // keys of this buffer
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[n][e] *= a.scale_log2;
+          s[n][e] = (s[n][e] + s2[n][e]) * a.scale_log2;
           if (n * 8 + tq * 2 + (e & 1) >= left) s[n][e] = -INFINITY;
         }
       uint32_t hi[4], lo[4];

@@ -204,46 +204,69 @@ struct KeyPipe {
   const uint8_t *kb, *vb;
   int key0, key1, row_chunks;
   uint32_t buf;
+  int id_ahead, row_ahead;  // page and row of this lane's key of the next buffer
   bool bad;
 
   __device__ __forceinline__ KeyPipe(const PagedArgs& args, uint32_t buffers, int row_bytes)
       : a(args), row_chunks(row_bytes / 16), buf(buffers) {}
 
-  __device__ __forceinline__ int begin(const Stretch& st) {  // the stretch's count of buffers
+  __device__ __forceinline__ void look_up(int i) {
+    const int t = key0 + i * KEYS + (threadIdx.x & 31) % KEYS;
+    id_ahead = 0;
+    row_ahead = 0;
+    if (t < key1) {
+      const uint32_t page = fast_div(t, a.page);
+      row_ahead = t - page * a.page.d;
+      id_ahead = __ldg(table + page);
+    }
+  }
+  // Begins a stretch whose first buffer is `first`; the stretch's count of buffers.
+  __device__ __forceinline__ int begin(const Stretch& st, int first) {
     table = a.table + st.b * a.table_stride;
     kb = a.kc + st.kvh * a.kc_sh;
     vb = a.vc + st.kvh * a.vc_sh;
     key0 = st.key0;
     key1 = st.key1;
     bad = st.bad;
+    look_up(first);
     return (key1 - key0 + KEYS - 1) / KEYS;
   }
-  // Starts the loads of buffer i of `count` (nothing behind the last) and closes the group.
-  __device__ __forceinline__ void issue(int i, int count, int stage) {
+  // Starts the loads of buffer i of `count` (nothing behind the last), closes the group, and looks up the
+  // pages of buffer i + step, which is the next one.
+  __device__ __forceinline__ void issue(int i, int step, int count, int stage) {
     const int lane = threadIdx.x & 31;
     if (i < count) {
-      const int t = key0 + i * KEYS + lane % KEYS;
-      int64_t ko = -1, vo = -1;
-      if (t < key1) {
-        const uint32_t page = fast_div(t, a.page);
-        const int row = t - page * a.page.d;
-        const int id = __ldg(table + page);
-        if (id >= 0 && id < a.num_pages) {
-          ko = id * a.kc_sp + row * a.kc_st;
-          vo = id * a.vc_sp + row * a.vc_st;
-        } else {
-          bad = true;
-        }
-      }
+      const int t0 = key0 + i * KEYS, id = id_ahead, row = row_ahead;
+      look_up(i + step);
+      const bool ok = id >= 0 && id < a.num_pages;
+      if (!ok && t0 + lane % KEYS < key1) bad = true;
       const uint32_t base = buf + stage * STAGE;
+      const int row0 = __shfl_sync(0xffffffffu, row, 0);
+      if (t0 + KEYS <= key1 && row0 + KEYS <= static_cast<int>(a.page.d) && __shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) {
+        // all keys in one page
+        const int id0 = __shfl_sync(0xffffffffu, id, 0);
+        const uint8_t* const kp = kb + id0 * a.kc_sp + row0 * a.kc_st;
+        const uint8_t* const vp = vb + id0 * a.vc_sp + row0 * a.vc_st;
 #pragma unroll
-      for (int j = 0; j < KEYS * CHUNKS / 32; ++j) {
-        const int idx = j * 32 + lane, r = idx / CHUNKS, ch = idx % CHUNKS;
-        const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
-        const bool there = kr >= 0 && ch < row_chunks;
-        const uint32_t dst = base + r * ROW + ((SWIZZLE ? ch ^ (r & 7) : ch) << 4);
-        cp_async16(dst, there ? kb + kr + ch * 16 : a.q, there ? 16 : 0);
-        cp_async16(dst + KEYS * ROW, there ? vb + vr + ch * 16 : a.q, there ? 16 : 0);
+        for (int j = 0; j < KEYS * CHUNKS / 32; ++j) {
+          const int idx = j * 32 + lane, r = idx / CHUNKS, ch = idx % CHUNKS;
+          const int bytes = ch < row_chunks ? 16 : 0;
+          const uint32_t dst = base + r * ROW + ((SWIZZLE ? ch ^ (r & 7) : ch) << 4);
+          cp_async16(dst, kp + r * a.kc_st + (bytes ? ch * 16 : 0), bytes);
+          cp_async16(dst + KEYS * ROW, vp + r * a.vc_st + (bytes ? ch * 16 : 0), bytes);
+        }
+      } else {
+        const bool mine = ok && t0 + lane % KEYS < key1;
+        const int64_t ko = mine ? id * a.kc_sp + row * a.kc_st : -1, vo = mine ? id * a.vc_sp + row * a.vc_st : -1;
+#pragma unroll
+        for (int j = 0; j < KEYS * CHUNKS / 32; ++j) {
+          const int idx = j * 32 + lane, r = idx / CHUNKS, ch = idx % CHUNKS;
+          const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+          const bool there = kr >= 0 && ch < row_chunks;
+          const uint32_t dst = base + r * ROW + ((SWIZZLE ? ch ^ (r & 7) : ch) << 4);
+          cp_async16(dst, there ? kb + kr + ch * 16 : a.q, there ? 16 : 0);
+          cp_async16(dst + KEYS * ROW, there ? vb + vr + ch * 16 : a.q, there ? 16 : 0);
+        }
       }
     }
     cp_async_commit();
