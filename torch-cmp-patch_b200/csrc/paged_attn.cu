@@ -155,7 +155,7 @@ struct Schedule {
   int item_heads, items_per_head;
   int64_t items;
   int ranks;        // CTAs per whole item, 0: equal shares and a join
-  int ctas;
+  int ctas, warps;  // warps per CTA
   int64_t workers;  // warps with shares
 };
 
@@ -173,16 +173,22 @@ Schedule schedule(const cmpx_paged_attn_desc* d, int num_sms) {
   s.item_heads = static_cast<int>((group + s.items_per_head - 1) / s.items_per_head);
   s.items = d->batch * d->cache.heads_kv * s.items_per_head;
   const int64_t keys = d->cache.table_width * d->cache.page_size;  // of the longest sequence there can be
-  const int64_t slots = static_cast<int64_t>(num_sms) * (f32 ? paged_f32_ctas_per_sm() : paged_mma_ctas_per_sm(d->cache.head_dim));
-  // Whole items, by one CTA or a cluster of 2, 4 or 8 (256 keys each, as far as the CTAs fit on the GPU): one
-  // launch and no join.
+  const int per_sm = f32 ? paged_f32_ctas_per_sm() : paged_mma_ctas_per_sm(d->cache.head_dim);
+  const int64_t slots = static_cast<int64_t>(num_sms) * per_sm;
+  // Whole items, by one CTA or a cluster of 2, 4 or 8 (256 keys each): one launch and no join.  The CTAs have to
+  // fit on the GPU at once, and a cluster's into one GPC: 7/8 of the places can be counted on, 3/4 where a cluster
+  // takes 8 SMs.  Where they are few, each has an SM to itself and twice the warps, for the loads in
+  // flight ([1, 32/8, 128] bf16, 4096 keys: 10.5 us; equal shares and a join 13.5).
+  auto fits = [&](int ranks) { return s.items * ranks * 8 <= slots * (per_sm == 1 && ranks == 8 ? 6 : 7); };
   int ranks = 1;
-  while (ranks < 8 && keys > 256 * ranks && s.items * ranks * 2 <= slots) ranks *= 2;
-  if (keys <= kWholeKeys || (keys <= kClusterKeys * ranks && s.items * ranks <= slots)) {
+  while (ranks < 8 && keys > 256 * ranks && fits(2 * ranks)) ranks *= 2;
+  if (keys <= kWholeKeys || (keys <= kClusterKeys * ranks && fits(ranks))) {
     s.ranks = ranks;
     s.ctas = static_cast<int>(s.items * ranks);
+    s.warps = per_sm > 1 && s.ctas <= num_sms * 3 / 4 ? kPagedWideWarps : kPagedWarps;
     return s;
   }
+  s.warps = kPagedWarps;
   const int64_t units = s.items * (std::max<int64_t>(1, (keys + kTile - 1) / kTile) + kItemCost);
   s.ctas = static_cast<int>(std::max<int64_t>(1, std::min(slots, (units + kShareMin - 1) / kShareMin)));
   s.workers = static_cast<int64_t>(s.ctas) * kPagedWarps;
@@ -295,8 +301,8 @@ int launch_paged_attn(const cmpx_paged_attn_desc* d, const LaunchCtx& ctx) {
     a.part_o = static_cast<float*>(d->workspace);
     a.part_ml = a.part_o + 2ull * s.workers * s.item_heads * c.head_dim;
   }
-  const int st = d->dtype == CMPX_F32 ? launch_paged_f32(a, s.ctas, s.ranks, ctx)
-                                      : launch_paged_mma(a, d->dtype, s.ctas, s.ranks, ctx);
+  const int st = d->dtype == CMPX_F32 ? launch_paged_f32(a, s.ctas, s.ranks, s.warps, ctx)
+                                      : launch_paged_mma(a, d->dtype, s.ctas, s.ranks, s.warps, ctx);
   if (st != CMPX_OK || s.ranks) return st;
   // The most partial results that a row can have: the longest sequence beside empty ones.
   const int64_t tiles = (static_cast<int64_t>(a.capacity) + kTile - 1) / kTile;

@@ -17,8 +17,6 @@
 namespace cmpx {
 namespace {
 
-constexpr int kWarps = kPagedWarps;
-constexpr int kThreads = kWarps * 32;
 constexpr int kCtasPerSm = 2;
 
 template <int DP>
@@ -30,16 +28,15 @@ struct F32Cfg {
   static constexpr int ROW = DP * 4;
   static constexpr int STAGES = 3;
   using Pipe = KeyPipe<ROW, KEYS, STAGES, false>;
-  static constexpr int SMEM = kWarps * Pipe::BYTES;
 };
 
-template <int DP, int HG, bool WHOLE>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attn_f32_kernel(const __grid_constant__ PagedArgs a) {
+template <int DP, int HG, bool WHOLE, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, kWarps == kPagedWarps ? kCtasPerSm : 1) paged_attn_f32_kernel(const __grid_constant__ PagedArgs a) {
   using C = F32Cfg<DP>;
   constexpr int LPT = C::LPT, STEPS = C::STEPS;
-  static_assert(C::SMEM >= kWarps * HG * DP * 4, "the warps' outputs are joined in the buffers");
+  static_assert(C::Pipe::BYTES >= HG * DP * 4, "the warps' outputs are joined in the buffers");
   __shared__ int64_t scratch[33 + 2 * kWarps];
-  __shared__ float2 sm_ml[kWarps][HG];
+  __shared__ float2 sm_ml[kWarps][HG], cta_ml[HG];
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane % LPT, group = lane / LPT;
@@ -170,7 +167,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attn_f32_kernel(co
           *reinterpret_cast<float4*>(sm_o + (warp * HG + h) * DP + col[i]) =
               make_float4(o[h][4 * i], o[h][4 * i + 1], o[h][4 * i + 2], o[h][4 * i + 3]);
       }
-      join_cluster<kWarps, HG, DP>(st.nh, a.head_dim, smem_u32(sm_o), smem_u32(sm_ml), [&](int h, int d, float x, float y) {
+      join_cluster<kWarps, HG, DP>(st.nh, a.head_dim, sm_o, &sm_ml[0][0], cta_ml, [&](int h, int d, float x, float y) {
         *reinterpret_cast<float2*>(a.o + st.b * a.o_sb + (st.h0 + h) * a.o_sh + d * 4) = make_float2(x, y);
       });
       break;
@@ -197,42 +194,45 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attn_f32_kernel(co
   }
 }
 
-template <int DP, int HG, bool WHOLE>
+template <int DP, int HG, bool WHOLE, int W>
 int launch(const PagedArgs& a, int ctas, int ranks, const LaunchCtx& ctx) {
-  auto kernel = paged_attn_f32_kernel<DP, HG, WHOLE>;
+  auto kernel = paged_attn_f32_kernel<DP, HG, WHOLE, W>;
+  constexpr int kSmem = W * F32Cfg<DP>::Pipe::BYTES;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
   int dev = 0;
   cudaGetDevice(&dev);
   std::call_once(once[dev & 63], [&] {
-    attr_err[dev & 63] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, F32Cfg<DP>::SMEM);
+    attr_err[dev & 63] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   });
   if (attr_err[dev & 63] != cudaSuccess) return CMPX_ERR_LAUNCH;
-  if (WHOLE) return launch_whole(kernel, a, ctas, ranks, kThreads, F32Cfg<DP>::SMEM, ctx.stream);
-  kernel<<<ctas, kThreads, F32Cfg<DP>::SMEM, ctx.stream>>>(a);
+  if (WHOLE) return launch_whole(kernel, a, ctas, ranks, 32 * W, kSmem, ctx.stream);
+  kernel<<<ctas, 32 * W, kSmem, ctx.stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
 }
 
-template <int DP, bool WHOLE>
-int launch_heads(const PagedArgs& a, int ctas, int ranks, const LaunchCtx& ctx) {
-  if (a.item_heads == 1) return launch<DP, 1, WHOLE>(a, ctas, ranks, ctx);
-  if (a.item_heads <= 4) return launch<DP, 4, WHOLE>(a, ctas, ranks, ctx);
-  return launch<DP, 8, WHOLE>(a, ctas, ranks, ctx);
+template <int DP, int HG>
+int launch_as(const PagedArgs& a, int ctas, int ranks, int warps, const LaunchCtx& ctx) {
+  if (ranks == 0) return launch<DP, HG, false, kPagedWarps>(a, ctas, ranks, ctx);
+  return warps == kPagedWideWarps ? launch<DP, HG, true, kPagedWideWarps>(a, ctas, ranks, ctx)
+                                  : launch<DP, HG, true, kPagedWarps>(a, ctas, ranks, ctx);
 }
 
-template <bool WHOLE>
-int launch_dim(const PagedArgs& a, int ctas, int ranks, const LaunchCtx& ctx) {
-  if (a.head_dim <= 64) return launch_heads<64, WHOLE>(a, ctas, ranks, ctx);
-  if (a.head_dim <= 128) return launch_heads<128, WHOLE>(a, ctas, ranks, ctx);
-  return launch_heads<256, WHOLE>(a, ctas, ranks, ctx);
+template <int DP>
+int launch_heads(const PagedArgs& a, int ctas, int ranks, int warps, const LaunchCtx& ctx) {
+  if (a.item_heads == 1) return launch_as<DP, 1>(a, ctas, ranks, warps, ctx);
+  if (a.item_heads <= 4) return launch_as<DP, 4>(a, ctas, ranks, warps, ctx);
+  return launch_as<DP, 8>(a, ctas, ranks, warps, ctx);
 }
 
 }  // namespace
 
 int paged_f32_ctas_per_sm() { return kCtasPerSm; }
 
-int launch_paged_f32(const PagedArgs& a, int ctas, int ranks, const LaunchCtx& ctx) {
-  return ranks ? launch_dim<true>(a, ctas, ranks, ctx) : launch_dim<false>(a, ctas, ranks, ctx);
+int launch_paged_f32(const PagedArgs& a, int ctas, int ranks, int warps, const LaunchCtx& ctx) {
+  if (a.head_dim <= 64) return launch_heads<64>(a, ctas, ranks, warps, ctx);
+  if (a.head_dim <= 128) return launch_heads<128>(a, ctas, ranks, warps, ctx);
+  return launch_heads<256>(a, ctas, ranks, warps, ctx);
 }
 
 }  // namespace cmpx

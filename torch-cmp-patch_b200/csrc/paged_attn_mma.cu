@@ -29,8 +29,6 @@
 namespace cmpx {
 namespace {
 
-constexpr int kWarps = kPagedWarps;
-constexpr int kThreads = kWarps * 32;
 constexpr int kKeys = 16;  // keys per buffer
 
 template <int DP>
@@ -39,8 +37,7 @@ struct MmaCfg {
   static constexpr int STAGES = DP == 64 ? 6 : DP == 192 ? 2 : 3;
   static constexpr int CTAS = DP == 256 ? 1 : 2;         // per SM: 96 KB of buffers each (192 KB at 256)
   using Pipe = KeyPipe<ROW, kKeys, STAGES, true>;
-  static constexpr int SMEM = kWarps * Pipe::BYTES;
-  static_assert(SMEM >= kWarps * 16 * DP * 4, "the warps' outputs are joined in the buffers");
+  static_assert(Pipe::BYTES >= 16 * DP * 4, "the warps' outputs are joined in the buffers");
 };
 
 template <int DT>
@@ -87,13 +84,13 @@ __device__ __forceinline__ uint32_t cut2(float lo, float hi) {
   return r;
 }
 
-template <int DT, int DP, bool WHOLE>
-__global__ void __launch_bounds__(kThreads, MmaCfg<DP>::CTAS) paged_attn_mma_kernel(const __grid_constant__ PagedArgs a) {
+template <int DT, int DP, bool WHOLE, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, kWarps == kPagedWarps ? MmaCfg<DP>::CTAS : 1) paged_attn_mma_kernel(const __grid_constant__ PagedArgs a) {
   using C = MmaCfg<DP>;
   constexpr float kBias = DT == CMPX_F16 ? 14.f : 0.f;
   constexpr float kLeast = DT == CMPX_F16 ? 0x1p-24f : 0x1p-126f;  // the types' smallest (normal) values
   __shared__ int64_t scratch[33 + 2 * kWarps];
-  __shared__ float2 sm_ml[kWarps][16];
+  __shared__ float2 sm_ml[kWarps][16], cta_ml[16];
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gr = lane >> 2, tq = lane & 3;  // fragment row and column pair
@@ -230,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<DP>::CTAS) paged_attn_mma_ker
           *reinterpret_cast<float2*>(sm_o + (warp * 16 + h) * DP + i * 8 + tq * 2) =
               make_float2(o[i][2 * r], o[i][2 * r + 1]);
       }
-      join_cluster<kWarps, 16, DP>(st.nh, a.head_dim, smem_u32(sm_o), smem_u32(sm_ml), [&](int h, int d, float x, float y) {
+      join_cluster<kWarps, 16, DP>(st.nh, a.head_dim, sm_o, &sm_ml[0][0], cta_ml, [&](int h, int d, float x, float y) {
         *reinterpret_cast<uint32_t*>(a.o + st.b * a.o_sb + (st.h0 + h) * a.o_sh + d * 2) = pack2<DT>(x, y);
       });
       break;
@@ -262,38 +259,45 @@ __global__ void __launch_bounds__(kThreads, MmaCfg<DP>::CTAS) paged_attn_mma_ker
   }
 }
 
-template <int DT, int DP, bool WHOLE>
+template <int DT, int DP, bool WHOLE, int W>
 int launch(const PagedArgs& a, int ctas, int ranks, const LaunchCtx& ctx) {
-  auto kernel = paged_attn_mma_kernel<DT, DP, WHOLE>;
+  auto kernel = paged_attn_mma_kernel<DT, DP, WHOLE, W>;
+  constexpr int kSmem = W * MmaCfg<DP>::Pipe::BYTES;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
   int dev = 0;
   cudaGetDevice(&dev);
   std::call_once(once[dev & 63], [&] {
-    attr_err[dev & 63] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MmaCfg<DP>::SMEM);
+    attr_err[dev & 63] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   });
   if (attr_err[dev & 63] != cudaSuccess) return CMPX_ERR_LAUNCH;
-  if (WHOLE) return launch_whole(kernel, a, ctas, ranks, kThreads, MmaCfg<DP>::SMEM, ctx.stream);
-  kernel<<<ctas, kThreads, MmaCfg<DP>::SMEM, ctx.stream>>>(a);
+  if (WHOLE) return launch_whole(kernel, a, ctas, ranks, 32 * W, kSmem, ctx.stream);
+  kernel<<<ctas, 32 * W, kSmem, ctx.stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
 }
 
-template <int DT, bool WHOLE>
-int launch_dt(const PagedArgs& a, int ctas, int ranks, const LaunchCtx& ctx) {
-  if (a.head_dim <= 64) return launch<DT, 64, WHOLE>(a, ctas, ranks, ctx);
-  if (a.head_dim <= 128) return launch<DT, 128, WHOLE>(a, ctas, ranks, ctx);
-  if (a.head_dim <= 192) return launch<DT, 192, WHOLE>(a, ctas, ranks, ctx);
-  return launch<DT, 256, WHOLE>(a, ctas, ranks, ctx);
+template <int DT, int DP>
+int launch_as(const PagedArgs& a, int ctas, int ranks, int warps, const LaunchCtx& ctx) {
+  if (ranks == 0) return launch<DT, DP, false, kPagedWarps>(a, ctas, ranks, ctx);
+  if constexpr (MmaCfg<DP>::CTAS > 1)
+    if (warps == kPagedWideWarps) return launch<DT, DP, true, kPagedWideWarps>(a, ctas, ranks, ctx);
+  return launch<DT, DP, true, kPagedWarps>(a, ctas, ranks, ctx);
+}
+
+template <int DT>
+int launch_dt(const PagedArgs& a, int ctas, int ranks, int warps, const LaunchCtx& ctx) {
+  if (a.head_dim <= 64) return launch_as<DT, 64>(a, ctas, ranks, warps, ctx);
+  if (a.head_dim <= 128) return launch_as<DT, 128>(a, ctas, ranks, warps, ctx);
+  if (a.head_dim <= 192) return launch_as<DT, 192>(a, ctas, ranks, warps, ctx);
+  return launch_as<DT, 256>(a, ctas, ranks, warps, ctx);
 }
 
 }  // namespace
 
 int paged_mma_ctas_per_sm(int64_t head_dim) { return head_dim > 192 ? MmaCfg<256>::CTAS : MmaCfg<128>::CTAS; }
 
-int launch_paged_mma(const PagedArgs& a, int dtype, int ctas, int ranks, const LaunchCtx& ctx) {
-  if (dtype == CMPX_BF16)
-    return ranks ? launch_dt<CMPX_BF16, true>(a, ctas, ranks, ctx) : launch_dt<CMPX_BF16, false>(a, ctas, ranks, ctx);
-  return ranks ? launch_dt<CMPX_F16, true>(a, ctas, ranks, ctx) : launch_dt<CMPX_F16, false>(a, ctas, ranks, ctx);
+int launch_paged_mma(const PagedArgs& a, int dtype, int ctas, int ranks, int warps, const LaunchCtx& ctx) {
+  return dtype == CMPX_BF16 ? launch_dt<CMPX_BF16>(a, ctas, ranks, warps, ctx) : launch_dt<CMPX_F16>(a, ctas, ranks, warps, ctx);
 }
 
 }  // namespace cmpx

@@ -274,44 +274,70 @@ struct KeyPipe {
 };
 
 // Joins the results of the WARPS warps of each of a cluster's CTAs, which all have the same item: outputs
-// sm_o [warp][ROWS][DP], maxima and sums sm_ml [warp][ROWS].  Every CTA does its part of the outputs;
-// store(h, d, x, y) gets two neighbouring values of head h.
+// sm_o [warp][ROWS][DP], maxima and sums sm_ml [warp][ROWS].  First each CTA its warps', in the place of the first
+// warp's (cta_ml [ROWS]: maxima and sums), then every CTA its part of the cluster's.  store(h, d, x, y) gets two
+// neighbouring values of head h.
 template <int WARPS, int ROWS, int DP, typename Store>
-__device__ __forceinline__ void join_cluster(int nh, int head_dim, uint32_t sm_o, uint32_t sm_ml, Store store) {
+__device__ __forceinline__ void join_cluster(int nh, int head_dim, float* sm_o, const float2* sm_ml, float2* cta_ml,
+                                             Store store) {
   const int ranks = cluster_size();
-  if (ranks > 1) cluster_sync();
-  else __syncthreads();
+  __syncthreads();
+  for (int x = threadIdx.x; x < nh * (DP / 2); x += blockDim.x) {
+    const int h = x / (DP / 2), d = 2 * (x - h * (DP / 2));
+    if (d >= head_dim) continue;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sm_ml[w * ROWS + h].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, x0 = 0.f, x1 = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float2 ml = sm_ml[w * ROWS + h], v = *reinterpret_cast<const float2*>(sm_o + (w * ROWS + h) * DP + d);
+      const float weight = ex2_approx(ml.x - base);
+      sum = fmaf(weight, ml.y, sum);
+      x0 = fmaf(weight, v.x, x0);
+      x1 = fmaf(weight, v.y, x1);
+    }
+    if (ranks == 1) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      store(h, d, x0 * inv, x1 * inv);
+    } else {
+      *reinterpret_cast<float2*>(sm_o + h * DP + d) = make_float2(x0, x1);  // read by this thread alone so far
+      if (d == 0) cta_ml[h] = make_float2(top, sum);
+    }
+  }
+  if (ranks == 1) return;
+  cluster_sync();
   for (int x = cluster_rank() * blockDim.x + threadIdx.x; x < nh * (DP / 2); x += ranks * blockDim.x) {
     const int h = x / (DP / 2), d = 2 * (x - h * (DP / 2));
     if (d >= head_dim) continue;
-    float top = -INFINITY, sum = 0.f, x0 = 0.f, x1 = 0.f;
-    for (int r = 0; r < ranks; ++r) {
-      float2 ml[WARPS], v[WARPS];
+    constexpr int MOST = 8;
+    float2 ml[MOST], v[MOST];
+    float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        ml[w] = cluster_load_f2(sm_ml + (w * ROWS + h) * 8, r);
-        v[w] = cluster_load_f2(sm_o + ((w * ROWS + h) * DP + d) * 4, r);
+    for (int r = 0; r < MOST; ++r) {
+      ml[r] = make_float2(-INFINITY, 0.f);
+      v[r] = make_float2(0.f, 0.f);
+      if (r < ranks) {
+        ml[r] = cluster_load_f2(smem_u32(cta_ml + h), r);
+        v[r] = cluster_load_f2(smem_u32(sm_o + h * DP + d), r);
       }
-      float now = top;
+    }
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) now = fmaxf(now, ml[w].x);
-      const float base = now == -INFINITY ? 0.f : now, keep = ex2_approx(top - base);
-      top = now;
-      sum *= keep;
-      x0 *= keep;
-      x1 *= keep;
+    for (int r = 0; r < MOST; ++r) top = fmaxf(top, ml[r].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, x0 = 0.f, x1 = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float weight = ex2_approx(ml[w].x - base);
-        sum = fmaf(weight, ml[w].y, sum);
-        x0 = fmaf(weight, v[w].x, x0);
-        x1 = fmaf(weight, v[w].y, x1);
-      }
+    for (int r = 0; r < MOST; ++r) {
+      const float weight = ex2_approx(ml[r].x - base);
+      sum = fmaf(weight, ml[r].y, sum);
+      x0 = fmaf(weight, v[r].x, x0);
+      x1 = fmaf(weight, v[r].y, x1);
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     store(h, d, x0 * inv, x1 * inv);
   }
-  if (ranks > 1) cluster_sync();  // nobody leaves while its results are read
+  cluster_sync();  // nobody leaves while its results are read
 }
 
 // Launches a kernel over whole items with `ranks` CTAs per item.
@@ -332,12 +358,13 @@ int launch_whole(Kernel kernel, const PagedArgs& a, int64_t ctas, int ranks, int
 }
 
 // The kernels over the keys: fp16 / bf16 items of up to 16 heads (paged_attn_mma.cu), fp32 items of up to 8
-// (paged_attn_f32.cu).  ranks: CTAs per whole item, 0 for equal shares.
-constexpr int kPagedWarps = 4;
+// (paged_attn_f32.cu).  ranks: CTAs per whole item, 0 for equal shares; warps: 4 per CTA, or 8 (whole items, one
+// CTA per SM; not for 16-bit heads above 192, whose buffers take the SM with 4).
+constexpr int kPagedWarps = 4, kPagedWideWarps = 8;
 int paged_mma_ctas_per_sm(int64_t head_dim);
 int paged_f32_ctas_per_sm();
-int launch_paged_mma(const PagedArgs& a, int dtype, int ctas, int ranks, const LaunchCtx& ctx);
-int launch_paged_f32(const PagedArgs& a, int ctas, int ranks, const LaunchCtx& ctx);
+int launch_paged_mma(const PagedArgs& a, int dtype, int ctas, int ranks, int warps, const LaunchCtx& ctx);
+int launch_paged_f32(const PagedArgs& a, int ctas, int ranks, int warps, const LaunchCtx& ctx);
 
 // Programmatic dependent launch: the join kernel starts while the main kernel runs, reads the
 // lengths, and waits here for the main kernel's results.
