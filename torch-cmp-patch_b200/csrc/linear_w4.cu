@@ -37,9 +37,7 @@ constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;    // rows of W per tile
 constexpr int kChunk = 256;  // k per turn
-constexpr int kStages = 4;   // turns in a warp's pipeline
-constexpr int kHeld = kStages - 1;  // turns between the load of a scale and its entry in the table: turn u's
-                                    // scales are entered by the push that comes before its products
+constexpr int kStages = 3;   // turns in a warp's pipeline
 
 struct W4Args {
   const uint8_t* x;
@@ -155,31 +153,42 @@ struct Activations {
   }
 };
 
-template <int NT, int GK>
+// XS: all activations in shared memory.
+template <int DT, int NT, int GK, bool XS>
 struct W4Cfg {
+  static constexpr int SUPER = GK == kGroup32 ? 2 : 4;                         // turns per table
   static constexpr int GROUPS = GK == kGroup128 ? 2 : GK == kGroup64 ? 4 : 8;  // columns of the table per turn
-  static constexpr int ENTRIES = GROUPS * kRows / 32;                          // per lane
+  static constexpr int COLS = SUPER * GROUPS;
+  static constexpr int ENTRIES = COLS * kRows / 32;                            // per lane
   static constexpr int STAGE = kRows * kChunk / 2;
-  static constexpr int TABLE = GROUPS * (kRows + 1) * 8;                       // bytes
-  static constexpr int WARP = kStages * STAGE + TABLE;
+  static constexpr int TABLE = COLS * (kRows + 1) * 8;                         // bytes
   static constexpr int RED = NT * 8 * (kRows + 1);                             // floats of a part
-  static constexpr int SMEM = kWarps * (WARP + 2 * RED * 4);
+  static constexpr int WARP = kStages * STAGE + TABLE + RED * 4;
+  static constexpr int SMEM = kWarps * WARP;                                   // without the activations
+  static constexpr int X_MOST = 65536;                                         // bytes of activations
+  static_assert(SMEM + (XS ? X_MOST : 0) <= 227 * 1024 && RED * 4 <= STAGE, "shared memory; a part takes a buffer's place");
 };
 
-template <int DT, int NT, int GK>
+template <int DT, int NT, int GK, bool XS>
 __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_constant__ W4Args a) {
-  using C = W4Cfg<NT, GK>;
-  constexpr int ES = elt_size(DT), GROUPS = C::GROUPS;
-  // Where registers allow it, the next quarter turn's activations are loaded before this one's products, and
-  // the two words of a quarter have sums of their own (8 x 131072 x 4096 fp16: 113 us without, 98 with).
-  constexpr bool AHEAD = DT != CMPX_F32 && NT == 1 && GK != kGroup32;
+  using C = W4Cfg<DT, NT, GK, XS>;
+  constexpr int ES = elt_size(DT), GROUPS = C::GROUPS, COLS = C::COLS;
+  // Where registers allow it, the two words of a quarter turn have sums of their own, and activations that are
+  // not in shared memory are loaded a quarter turn ahead.
+  constexpr bool TWO = DT != CMPX_F32 && NT == 1 && GK != kGroup32;
+  constexpr bool AHEAD = TWO && !XS;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, tq = lane & 3;
   const int m0 = blockIdx.y * (8 * NT);
   uint8_t* const mine = smem + warp * C::WARP;
   const uint32_t buf = smem_u32(mine);
   float2* const table = reinterpret_cast<float2*>(mine + kStages * C::STAGE);
-  float* const red = reinterpret_cast<float*>(smem + kWarps * C::WARP);  // [warp][first or later tile][token][kRows + 1]
+  uint4* const x_all = reinterpret_cast<uint4*>(smem + C::SMEM);  // [quarter][word][NT][lane]
+  // A warp's parts of tiles that it shares, [token][kRows + 1]: of its run's first tile in a place of its own,
+  // of a later one, which is its last, where its first buffer was.
+  auto part_of = [&](int w, bool later) {
+    return reinterpret_cast<float*>(smem + w * C::WARP + (later ? 0 : kStages * C::STAGE + C::TABLE));
+  };
 
   const int chunks = a.chunks;
   const int tile0 = static_cast<int>(static_cast<int64_t>(a.tiles) * blockIdx.x / gridDim.x);
@@ -192,64 +201,27 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
   for (int t = 0; t < NT; ++t)
     xp[t] = a.x + static_cast<int64_t>(min(m0 + t * 8 + gr, a.m - 1)) * a.xs + tq * 16 * ES;
 
-  // ---- loads: a cursor over this warp's turns, kStages - 1 ahead of the products
+  // ---- weights: a cursor over this warp's turns, kStages - 1 ahead of the products
   int f_left = u1 - u0, f_tile = tile0 + u0 / chunks, f_chunk = u0 % chunks, f_stage = 0;
-  const uint8_t *f_w[2], *f_s[C::ENTRIES], *f_z[C::ENTRIES];
+  const uint8_t* f_w;  // this lane's 16 bytes (lane % 8) of row lane / 8; rows 4 j further are f_off[j] behind it
+  int f_off[4];
   auto f_rows = [&] {  // rows behind the last read the last one; their results are not written
-    const int n0 = f_tile * kRows;
+    const int n = min(f_tile * kRows + (lane >> 3), a.n - 1);
+    f_w = a.w + static_cast<int64_t>(n) * a.ws + (lane & 7) * 16;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) f_w[i] = a.w + static_cast<int64_t>(min(n0 + 8 * i + gr, a.n - 1)) * a.ws + tq * 16;
-#pragma unroll
-    for (int i = 0; i < C::ENTRIES; ++i) {
-      const int64_t r = min(n0 + (lane + 32 * i) / GROUPS, a.n - 1);
-      f_s[i] = a.scales + r * a.ss;
-      f_z[i] = a.zeros + r * a.zs;
-    }
+    for (int j = 0; j < 4; ++j) f_off[j] = min(4 * j, a.n - 1 - n) * static_cast<int>(a.ws);
   };
   f_rows();
-  RawVec<ES> s_raw[kHeld][C::ENTRIES];
-  uint32_t z_raw[kHeld][C::ENTRIES];
-#pragma unroll
-  for (int q = 0; q < kHeld; ++q)
-#pragma unroll
-    for (int i = 0; i < C::ENTRIES; ++i) {
-      s_raw[q][i] = RawVec<ES>{};
-      z_raw[q][i] = 0;
-    }
-  // where this lane's 16 bytes of a row go: halves of 64 k of odd row pairs change places, so that a
-  // quad's 32 bytes of 4 rows fill the banks once
-  const uint32_t put = buf + gr * (kChunk / 2) + ((tq * 16) ^ (((gr >> 1) & 1) << 5));
-  // Starts the loads of the cursor's turn and enters the scales of the turn kHeld before it in the table.
-  auto push = [&] {
-#pragma unroll
-    for (int i = 0; i < C::ENTRIES; ++i) {
-      const int e = lane + 32 * i, g = e % GROUPS, r = e / GROUPS;
-      float s;
-      unpack_vec<DT, ES>(s_raw[kHeld - 1][i], &s);
-      table[g * (kRows + 1) + r] = make_float2(s, __uint_as_float(zero_pair<DT>(z_raw[kHeld - 1][i])));
-#pragma unroll
-      for (int q = kHeld - 1; q > 0; --q) {
-        s_raw[q][i] = s_raw[q - 1][i];
-        z_raw[q][i] = z_raw[q - 1][i];
-      }
-    }
+  // Chunk c of row r lies at chunk c ^ (r % 4) * 2: a quad's 32 bytes of 4 rows fill the banks once.
+  const uint32_t put = buf + (lane >> 3) * (kChunk / 2) + (((lane & 7) ^ ((lane >> 3) << 1)) << 4);
+  auto push = [&] {  // starts the loads of the cursor's turn
     if (f_left > 0) {
       --f_left;
-      const int k0 = f_chunk * kChunk;
+      const int there = f_chunk * kChunk + (lane & 7) * 32 < a.k ? 16 : 0;
+      const uint8_t* const from = f_w + f_chunk * (kChunk / 2);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int there = k0 + h * 128 + tq * 32 < a.k ? 16 : 0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          cp_async16(put + f_stage * C::STAGE + i * 8 * (kChunk / 2) + h * 64, there ? f_w[i] + (k0 >> 1) + h * 64 : a.w, there);
-      }
-#pragma unroll
-      for (int i = 0; i < C::ENTRIES; ++i) {
-        const int g = (lane + 32 * i) % GROUPS;
-        const int at = fast_div(min(k0 + g * (kChunk / GROUPS), a.k - 1), a.group);
-        s_raw[0][i] = *reinterpret_cast<const RawVec<ES>*>(f_s[i] + at * ES);
-        z_raw[0][i] = a.zeros ? __ldg(f_z[i] + at) : 8u;
-      }
+      for (int j = 0; j < 4; ++j)
+        cp_async16(put + f_stage * C::STAGE + j * 4 * (kChunk / 2), there ? from + f_off[j] : a.w, there);
       if (++f_chunk == chunks) {
         f_chunk = 0;
         ++f_tile;
@@ -258,6 +230,29 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
     }
     cp_async_commit();
     f_stage = f_stage + 1 == kStages ? 0 : f_stage + 1;
+  };
+
+  // ---- scales and zero points: SUPER turns of a tile at a time, loaded one set ahead (whole stretches of rows:
+  // a load instruction touches few lines) and entered in the table when their turns begin
+  RawVec<ES> s_raw[C::ENTRIES];
+  uint32_t z_raw[C::ENTRIES];
+  const int g_col = lane % COLS, g_row = lane / COLS;
+  auto load_groups = [&](int tile, int set) {
+    const int at = fast_div(min((set * COLS + g_col) * (kChunk / GROUPS), a.k - 1), a.group);
+#pragma unroll
+    for (int i = 0; i < C::ENTRIES; ++i) {
+      const int64_t r = min(tile * kRows + i * (32 / COLS) + g_row, a.n - 1);
+      s_raw[i] = *reinterpret_cast<const RawVec<ES>*>(a.scales + r * a.ss + at * ES);
+      z_raw[i] = a.zeros ? __ldg(a.zeros + r * a.zs + at) : 8u;
+    }
+  };
+  auto enter_groups = [&] {
+#pragma unroll
+    for (int i = 0; i < C::ENTRIES; ++i) {
+      float s;
+      unpack_vec<DT, ES>(s_raw[i], &s);
+      table[g_col * (kRows + 1) + i * (32 / COLS) + g_row] = make_float2(s, __uint_as_float(zero_pair<DT>(z_raw[i])));
+    }
   };
 
   // ---- products
@@ -272,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
   auto compute = [&](auto full, int c, int next, const uint8_t* stage) {  // full: the turn has all its 256 k
     constexpr bool FULL = decltype(full)::value;
     constexpr int SETS = GK == kGroup32 ? 2 : 1;  // sums of a quarter that have scales of their own
-    constexpr int CHAINS = AHEAD ? 2 : 1;
+    constexpr int CHAINS = TWO ? 2 : 1;
     float part[CHAINS][SETS][NT][4];
     float2 col[2], other[2];  // this lane's k's column, and (groups of 32) the quad's other one
 #pragma unroll
@@ -280,7 +275,12 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
       const int k = c * kChunk + h * 64;
       if (!FULL && k >= a.k) break;
       Activations<DT> x[2][NT];
-      if (AHEAD && FULL) {
+      if (XS) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) x[j][t].v[0] = x_all[((k / 64 * 2 + j) * NT + t) * 32 + lane];
+      } else if (AHEAD && FULL) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -300,13 +300,12 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
       uint2 w[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r)
-        w[r] = *reinterpret_cast<const uint2*>(stage + (8 * r + gr) * (kChunk / 2) + (((h & 1) ^ ((gr >> 1) & 1)) << 5) +
-                                               (h >> 1) * 64 + tq * 8);
+        w[r] = *reinterpret_cast<const uint2*>(stage + (8 * r + gr) * (kChunk / 2) + ((h ^ (gr & 3)) << 5) + tq * 8);
       const bool first = GK != kGroup128 || (h & 1) == 0;  // of the products that share a scale
       if (first) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int g = GK == kGroup128 ? h >> 1 : GK == kGroup64 ? h : 2 * h + (tq >> 1);
+          const int g = c % C::SUPER * GROUPS + (GK == kGroup128 ? h >> 1 : GK == kGroup64 ? h : 2 * h + (tq >> 1));
           col[r] = table[g * (kRows + 1) + 8 * r + gr];
           if (GK == kGroup32) other[r] = table[(g ^ 1) * (kRows + 1) + 8 * r + gr];
         }
@@ -319,7 +318,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           uint32_t p[Activations<DT>::PARTS][4];
-          x[j][t].pairs(p);
+          if (XS) {
+            p[0][0] = x[j][t].v[0].x;
+            p[0][1] = x[j][t].v[0].y;
+            p[0][2] = x[j][t].v[0].z;
+            p[0][3] = x[j][t].v[0].w;
+          } else {
+            x[j][t].pairs(p);
+          }
 #pragma unroll
           for (int y = 0; y < Activations<DT>::PARTS; ++y) {
 #pragma unroll
@@ -348,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
             acc[t][e] = fmaf(tq < 2 ? s : o, part[0][0][t][e], acc[t][e]);
             acc[t][e] = fmaf(tq < 2 ? o : s, part[0][SETS - 1][t][e], acc[t][e]);
           } else {
-            acc[t][e] = fmaf(s, AHEAD ? part[0][0][t][e] + part[CHAINS - 1][0][t][e] : part[0][0][t][e], acc[t][e]);
+            acc[t][e] = fmaf(s, TWO ? part[0][0][t][e] + part[CHAINS - 1][0][t][e] : part[0][0][t][e], acc[t][e]);
           }
         }
     }
@@ -367,6 +373,21 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
   for (int i = 0; i < kStages - 1; ++i) push();
   int stage = 0;
   int tile = tile0 + u0 / chunks, c = u0 % chunks;
+  load_groups(tile, c / C::SUPER);
+  if constexpr (XS) {
+    for (int i = threadIdx.x; i < (a.k + 63) / 64 * (2 * NT * 32); i += kThreads) {
+      const int l = i % 32, t = i / 32 % NT, j = i / (32 * NT) % 2, k = i / (64 * NT) * 64 + (l & 3) * 16 + j * 8;
+      Activations<DT> v;
+      if (k < a.k)
+        v.load(a.x + static_cast<int64_t>(min(m0 + t * 8 + (l >> 2), a.m - 1)) * a.xs + k * ES);
+      else
+        v.zero();
+      uint32_t p[Activations<DT>::PARTS][4];
+      v.pairs(p);
+      x_all[i] = make_uint4(p[0][0], p[0][1], p[0][2], p[0][3]);
+    }
+    __syncthreads();
+  }
   // (a partial last turn leaves x_ahead at the row's begin, where the next tile's first turn needs it)
   if (AHEAD && a.k >= kChunk) load_ahead((c + 1) * kChunk <= a.k ? c * kChunk : 0);
   for (int u = u0; u < u1;) {
@@ -379,7 +400,13 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
       cp_async_wait<kStages - 2>();
       __syncwarp();  // this turn's weights are there, and everybody is done with the turn before
       push();
-      __syncwarp();
+      if (u + i == u0 || (c + i) % C::SUPER == 0) {
+        enter_groups();
+        __syncwarp();
+        const int set = (c + i) / C::SUPER + 1;
+        const bool on = set * C::SUPER < chunks;
+        if (on || tile + 1 < tile1) load_groups(on ? tile : tile + 1, on ? set : 0);
+      }
       // where the activations of the next full turn begin: behind this one, or with the next tile at 0
       const int now = (c + i) * kChunk, after = now + 2 * kChunk <= a.k ? now + kChunk : 0;
       if (now + kChunk <= a.k)
@@ -388,7 +415,12 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
         compute(std::false_type{}, c + i, 0, mine + stage * C::STAGE);
       stage = stage + 1 == kStages ? 0 : stage + 1;
     }
-    float* const part = red + (2 * warp + (tile == tile0 + u0 / chunks ? 0 : 1)) * C::RED;
+    const bool later = tile != tile0 + u0 / chunks;
+    if (turns != chunks && later) {
+      cp_async_wait<0>();
+      __syncwarp();
+    }
+    float* const part = part_of(warp, later);
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -413,30 +445,39 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
     if (w0 == w1) continue;
     float s = 0.f;
     for (int w = w0; w <= w1; ++w)
-      s += red[(2 * w + (t == w * run / chunks ? 0 : 1)) * C::RED + token * (kRows + 1) + r];
+      s += part_of(w, t != w * run / chunks)[token * (kRows + 1) + r];
     write(m0 + token, (tile0 + t) * kRows + r, s);
   }
 }
 
 GroupKind group_kind(int64_t group) { return group % 128 == 0 ? kGroup128 : group % 64 == 0 ? kGroup64 : kGroup32; }
 
-template <int DT, int NT, int GK>
-int launch(W4Args& a, const LaunchCtx& ctx) {
-  using C = W4Cfg<NT, GK>;
-  auto kernel = linear_w4_kernel<DT, NT, GK>;
+template <int DT, int NT, int GK, bool XS>
+int launch_as(W4Args& a, const LaunchCtx& ctx) {
+  using C = W4Cfg<DT, NT, GK, XS>;
+  auto kernel = linear_w4_kernel<DT, NT, GK, XS>;
   static std::once_flag once[64];
   static cudaError_t attr_err[64];
   int dev = 0;
   cudaGetDevice(&dev);
   std::call_once(once[dev & 63], [&] {
-    attr_err[dev & 63] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    attr_err[dev & 63] =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM + (XS ? C::X_MOST : 0));
   });
   if (attr_err[dev & 63] != cudaSuccess) return CMPX_ERR_LAUNCH;
   a.chunks = (a.k + kChunk - 1) / kChunk;
   a.tiles = (a.n + kRows - 1) / kRows;
   const dim3 grid(static_cast<unsigned>(std::min(a.tiles, ctx.num_sms)), static_cast<unsigned>((a.m + 8 * NT - 1) / (8 * NT)));
-  kernel<<<grid, kThreads, C::SMEM, ctx.stream>>>(a);
+  kernel<<<grid, kThreads, C::SMEM + (XS ? (a.k + 63) / 64 * (2 * NT * 512) : 0), ctx.stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
+}
+
+template <int DT, int NT, int GK>
+int launch(W4Args& a, const LaunchCtx& ctx) {
+  // Activations of up to 64 KB (8 tokens: 4096 k) are laid out for the products once per CTA.
+  if constexpr (DT != CMPX_F32)
+    if ((a.k + 63) / 64 * (2 * NT * 512) <= W4Cfg<DT, NT, GK, true>::X_MOST) return launch_as<DT, NT, GK, true>(a, ctx);
+  return launch_as<DT, NT, GK, false>(a, ctx);
 }
 
 template <int DT, int NT>
