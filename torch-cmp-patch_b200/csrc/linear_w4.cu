@@ -11,15 +11,17 @@
 // has a run of tiles of 16 rows of W, and its warps have equal runs of the tiles' turns of 256 k laid
 // end to end; mma.m16n8k16 multiplies the 16 rows with 8 NT tokens.  Every warp has its own pipeline
 // of turns (2 KB each, cp.async) that runs on across tiles.  A tile that one warp has to itself is written from
-// its registers; the others' parts are summed once, at the CTA's end, in a fixed order.  (A tile
-// shared by all warps and summed before the next one took twice the instructions and 22 us for 8 x 16384 x 4096
-// in fp16, whose bytes take 5.7.)
-// A lane takes 16 k of a row that lie side by side, and the products run over k in the order that falls out
+// its registers; the others' parts are summed once, at the CTA's end, in a fixed order.
+// A lane multiplies 16 k of a row that lie side by side, and the products run over k in the order that falls out
 // of it: word j of the lanes tq = 0..3 holds k = 16 tq + 8 j .. + 7, and nibbles e and e + 4 of a word, which
-// one mask isolates as the halves of a register, are a pair.  x follows that order with one byte
-// permutation a register.  Scales and zero points pass through a table in shared memory that holds them
-// as the products take them.  Instructions come next to the bytes: for eight weights 3 shifts, 4
-// masks and 4 subtractions (fp16: 1, 4, 4), and as many again for the rest.
+// one mask isolates as the halves of a register, are a pair.  16-bit activations of up to 64 KB are laid out
+// in that order in shared memory once per CTA; others follow it with one byte permutation a register.
+// What bounds it beside the bytes: first the lines that its loads touch (one a cycle), which is why eight lanes load
+// 128 bytes of a row together and scales and zero points come for sets of turns, through a table in shared
+// memory; then the half-rate units: for eight weights 3 shifts and 4 masks beside 4 subtractions (fp16: 1,
+// 4, 4).  Measured from a graph: 8 x 16384 x 4096 fp16, groups of 64: 14.7 us for 37 MB (5.7 at the
+// copy rate; 8 x 131072 x 4096: 70 us, 4.3 TB/s); 1 x 4096 x 4096 bf16: 5.9 us, most of it the launch and one pass
+// through the pipeline.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -49,7 +51,8 @@ struct W4Args {
   int64_t xs, ws, ss, zs, ys;  // row strides in bytes
   int m, n, k;
   FastDiv group;
-  int tiles, chunks;  // row tiles, turns per tile
+  int chunks;                     // turns per tile
+  int tiles_per_cta, tiles_rest;  // row tiles of a CTA; the first tiles_rest have one more
 };
 
 // Where groups may end: at multiples of 128 k, of 64 k, or of 32 k.
@@ -156,7 +159,7 @@ struct Activations {
 // XS: all activations in shared memory.
 template <int DT, int NT, int GK, bool XS>
 struct W4Cfg {
-  static constexpr int SUPER = GK == kGroup32 ? 2 : 4;                         // turns per table
+  static constexpr int SUPER = GK == kGroup128 ? 4 : 2;                        // turns per table
   static constexpr int GROUPS = GK == kGroup128 ? 2 : GK == kGroup64 ? 4 : 8;  // columns of the table per turn
   static constexpr int COLS = SUPER * GROUPS;
   static constexpr int ENTRIES = COLS * kRows / 32;                            // per lane
@@ -173,9 +176,10 @@ template <int DT, int NT, int GK, bool XS>
 __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_constant__ W4Args a) {
   using C = W4Cfg<DT, NT, GK, XS>;
   constexpr int ES = elt_size(DT), GROUPS = C::GROUPS, COLS = C::COLS;
-  // Where registers allow it, the two words of a quarter turn have sums of their own, and activations that are
-  // not in shared memory are loaded a quarter turn ahead.
-  constexpr bool TWO = DT != CMPX_F32 && NT == 1 && GK != kGroup32;
+  // Where registers allow it (a spill costs more than either gives: 8 x 16384 x 4096 with groups of 64 takes 16.4
+  // us with 20 bytes of them, 14.7 with none), the two words of a quarter turn have sums of their own, and
+  // activations that are not in shared memory are loaded a quarter turn ahead.
+  constexpr bool TWO = DT != CMPX_F32 && NT == 1 && GK == kGroup128;
   constexpr bool AHEAD = TWO && !XS;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, tq = lane & 3;
@@ -191,8 +195,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
   };
 
   const int chunks = a.chunks;
-  const int tile0 = static_cast<int>(static_cast<int64_t>(a.tiles) * blockIdx.x / gridDim.x);
-  const int tile1 = static_cast<int>(static_cast<int64_t>(a.tiles) * (blockIdx.x + 1) / gridDim.x);
+  const int b = blockIdx.x;
+  const int tile0 = b * a.tiles_per_cta + min(b, a.tiles_rest), tile1 = tile0 + a.tiles_per_cta + (b < a.tiles_rest ? 1 : 0);
   const int run = ((tile1 - tile0) * chunks + kWarps - 1) / kWarps;  // turns per warp
   const int u0 = min(warp * run, (tile1 - tile0) * chunks), u1 = min(u0 + run, (tile1 - tile0) * chunks);
 
@@ -375,17 +379,35 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
   int tile = tile0 + u0 / chunks, c = u0 % chunks;
   load_groups(tile, c / C::SUPER);
   if constexpr (XS) {
-    for (int i = threadIdx.x; i < (a.k + 63) / 64 * (2 * NT * 32); i += kThreads) {
-      const int l = i % 32, t = i / 32 % NT, j = i / (32 * NT) % 2, k = i / (64 * NT) * 64 + (l & 3) * 16 + j * 8;
-      Activations<DT> v;
-      if (k < a.k)
-        v.load(a.x + static_cast<int64_t>(min(m0 + t * 8 + (l >> 2), a.m - 1)) * a.xs + k * ES);
-      else
-        v.zero();
-      uint32_t p[Activations<DT>::PARTS][4];
-      v.pairs(p);
-      x_all[i] = make_uint4(p[0][0], p[0][1], p[0][2], p[0][3]);
-    }
+    // (what the lanes of tokens that are not there find makes columns that are not written)
+    const int lanes = 4 * min(8 * NT, a.m - m0), count = (a.k + 63) / 64 * 2 * lanes;
+    auto fill = [&](auto full, auto at_once) {  // full: all 8 NT tokens are there; at_once: loads in flight per thread
+      constexpr int AT_ONCE = decltype(at_once)::value;
+      for (int i0 = threadIdx.x; i0 < count; i0 += AT_ONCE * kThreads) {
+        Activations<DT> x[AT_ONCE];
+        int to[AT_ONCE];
+#pragma unroll
+        for (int e = 0; e < AT_ONCE; ++e) {
+          const int i = i0 + e * kThreads;
+          const int set = decltype(full)::value ? i / (32 * NT) : i / lanes, l = i - set * lanes;  // set: quarter and word
+          const int k = set / 2 * 64 + (l & 3) * 16 + set % 2 * 8;
+          to[e] = i < count ? (set * NT + l / 32) * 32 + l % 32 : -1;
+          if (i < count && k < a.k)
+            x[e].load(a.x + static_cast<int64_t>(m0 + (l >> 2)) * a.xs + k * ES);
+          else
+            x[e].zero();
+        }
+#pragma unroll
+        for (int e = 0; e < AT_ONCE; ++e) {
+          uint32_t p[Activations<DT>::PARTS][4];
+          x[e].pairs(p);
+          if (to[e] >= 0) x_all[to[e]] = make_uint4(p[0][0], p[0][1], p[0][2], p[0][3]);
+        }
+      }
+    };
+    if (count <= kThreads) fill(std::false_type{}, std::integral_constant<int, 1>{});
+    else if (lanes < 32 * NT) fill(std::false_type{}, std::integral_constant<int, 4>{});
+    else fill(std::true_type{}, std::integral_constant<int, 8>{});
     __syncthreads();
   }
   // (a partial last turn leaves x_ahead at the row's begin, where the next tile's first turn needs it)
@@ -439,13 +461,24 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
 
   // the tiles that several warps have parts of
   __syncthreads();
+  if (tile1 - tile0 == 1) {  // one tile, a part from every warp: four lanes an output
+    for (int i = threadIdx.x; i < NT * 8 * kRows * 4; i += kThreads) {
+      const int r = i / 4 % kRows, token = i / (4 * kRows), warps = (chunks + run - 1) / run;
+      if (warps == 1) break;
+      float s = 0.f;
+      for (int w = i % 4; w < warps; w += 4) s += part_of(w, false)[token * (kRows + 1) + r];
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      if (i % 4 == 0) write(m0 + token, tile0 * kRows + r, s);
+    }
+    return;
+  }
   for (int i = threadIdx.x; i < (tile1 - tile0) * (NT * 8 * kRows); i += kThreads) {
     const int r = i % kRows, token = i / kRows % (NT * 8), t = i / (kRows * NT * 8);
     const int w0 = t * chunks / run, w1 = ((t + 1) * chunks - 1) / run;
     if (w0 == w1) continue;
     float s = 0.f;
-    for (int w = w0; w <= w1; ++w)
-      s += part_of(w, t != w * run / chunks)[token * (kRows + 1) + r];
+    for (int w = w0; w <= w1; ++w) s += part_of(w, t != w * run / chunks)[token * (kRows + 1) + r];
     write(m0 + token, (tile0 + t) * kRows + r, s);
   }
 }
@@ -466,8 +499,10 @@ int launch_as(W4Args& a, const LaunchCtx& ctx) {
   });
   if (attr_err[dev & 63] != cudaSuccess) return CMPX_ERR_LAUNCH;
   a.chunks = (a.k + kChunk - 1) / kChunk;
-  a.tiles = (a.n + kRows - 1) / kRows;
-  const dim3 grid(static_cast<unsigned>(std::min(a.tiles, ctx.num_sms)), static_cast<unsigned>((a.m + 8 * NT - 1) / (8 * NT)));
+  const int tiles = (a.n + kRows - 1) / kRows, ctas = std::min(tiles, ctx.num_sms);
+  a.tiles_per_cta = tiles / ctas;
+  a.tiles_rest = tiles % ctas;
+  const dim3 grid(static_cast<unsigned>(ctas), static_cast<unsigned>((a.m + 8 * NT - 1) / (8 * NT)));
   kernel<<<grid, kThreads, C::SMEM + (XS ? (a.k + 63) / 64 * (2 * NT * 512) : 0), ctx.stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
 }
