@@ -358,7 +358,7 @@ typedef struct cmpx_paged_cache {
  * [batch, heads, len, head_dim] or NULL with heads = 0.  Sequence b has new_lengths[b] new tokens (all
  * len when NULL; values outside 0..len are clipped to it): its token i, i < new_lengths[b], goes to
  * place lengths[b] - new_lengths[b] + i.  Rows i >= new_lengths[b] are padding: nothing is stored for
- * them and q_out gets q as it is.  A token whose place is negative, behind the table, or in a page
+ * them and q_out gets q as it is (a batch row that is padding altogether has new_lengths 0).  A token whose place is negative, behind the table, or in a page
  * outside 0..num_pages-1 is not stored and raises CMPX_DEVFLAG_BAD_PAGE.  Two tokens of one call
  * that share a slot (a page that two sequences both append to) leave either's values there. */
 typedef struct cmpx_kv_append_desc {
@@ -415,7 +415,7 @@ CMPX_API int cmpx_paged_attn_plan(const cmpx_paged_attn_desc* desc, char* buf, s
  * x's type; zeros [n, k / group] bytes (0..15) or NULL (8).  group is a multiple of 32 and
  * divides k.  The differences code - zero are exact in every type, their products with x are summed
  * in fp32 and multiplied by the fp32 value of the scale group by group; the bias is added before the
- * one rounding.  Rows of x and w start on 16-byte boundaries. */
+ * one rounding.  Rows of x and w start on 16-byte boundaries; w's row stride is at most 2^27 bytes. */
 typedef struct cmpx_linear_w4_desc {
   const void* x;
   const uint8_t* w;

@@ -135,6 +135,26 @@ def test_sharp_scores(cuda_device, dtype):
     Case(dtype, 8, 2, 64, 16, [1, 50, 700, 3000], seed=7, sharp=30.0).check()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("n", [40, 3000, 9000])
+def test_infinite_values_and_scores(cuda_device, dtype, n):
+    c = Case(dtype, 4, 2, 64, 16, [n], seed=16)
+    page, row = int(c.table[0, (n - 1) // 16]), (n - 1) % 16
+    c.args[2][page, 0, row, 5] = float("inf")             # a value: its column is infinite, the others stay
+    out = cmpext3.ops.paged_attention(*c.args)[0, :, 0]
+    assert (out[:2, 5] == float("inf")).all()
+    rest = torch.cat((out[:2, :5], out[:2, 6:]), 1)
+    assert torch.isfinite(rest).all() and torch.isfinite(out[2:]).all()
+    c.args[2][page, 0, row, 5] = 0.0
+    c.args[0][0, :, 0, 3] = 2.0
+    c.args[1][page, 1, row, 3] = -float("inf")            # a score of -inf: the key does not count
+    c.q[0, :, 0, 3] = 2.0
+    out = cmpext3.ops.paged_attention(*c.args)[0, 2:, 0]
+    torch.cuda.synchronize()
+    want, bound = O.attention(c.q[0, 2:, 0], c.k[0][1:, :n - 1], c.v[0][1:, :n - 1], 1 / 8)
+    O.assert_within(out, want, bound, "a key with a score of -inf")
+
+
 def test_nan_and_infinite_keys_spread_to_their_sequence_alone(cuda_device):
     c = Case(torch.bfloat16, 4, 2, 64, 16, [40, 700, 30], seed=8)
     c.args[1][int(c.table[1, 20]), 0, 3] = float("nan")
@@ -177,9 +197,10 @@ def test_the_same_call_gives_the_same_bits(cuda_device, dtype):
         assert torch.equal(cmpext3.ops.paged_attention(*c.args), first)
 
 
-def test_two_graphs_at_once_and_other_lengths(cuda_device):
-    c = Case(torch.bfloat16, 8, 2, 128, 16, [3000, 200, 1], seed=11)
-    d = Case(torch.bfloat16, 8, 2, 128, 16, [2500, 2600], seed=12)
+@pytest.mark.parametrize("longest", [100, 3000, 12000])   # a CTA, a cluster, shares and a join
+def test_two_graphs_at_once_and_other_lengths(cuda_device, longest):
+    c = Case(torch.bfloat16, 8, 2, 128, 16, [longest, 50, 1], seed=11)
+    d = Case(torch.bfloat16, 8, 2, 128, 16, [longest - 7, longest // 2], seed=12)
     graphs = []
     for case in (c, d):
         side = torch.cuda.Stream()
@@ -192,7 +213,7 @@ def test_two_graphs_at_once_and_other_lengths(cuda_device):
             out = cmpext3.ops.paged_attention(*case.args)
         graphs.append((graph, out, case))
     streams = [torch.cuda.Stream() for _ in graphs]
-    for lengths in ([3000, 200, 1], [17, 0, 1], [2999, 100, 0]):
+    for lengths in ([longest, 50, 1], [17, 0, 1], [longest - 1, 20, 0]):
         c.args[4].copy_(torch.tensor(lengths, dtype=torch.int32))
         torch.cuda.synchronize()
         for (graph, _, _), s in zip(graphs, streams):
@@ -204,8 +225,9 @@ def test_two_graphs_at_once_and_other_lengths(cuda_device):
             assert torch.equal(out, cmpext3.ops.paged_attention(*case.args))
 
 
-def test_two_streams_at_once(cuda_device):
-    cases = [Case(torch.float16, 8, 2, 64, 16, [6000, 30], seed=s) for s in (13, 14)]
+@pytest.mark.parametrize("longest", [6000, 15000])
+def test_two_streams_at_once(cuda_device, longest):
+    cases = [Case(torch.float16, 8, 2, 64, 16, [longest, 30], seed=s) for s in (13, 14)]
     want = [cmpext3.ops.paged_attention(*c.args) for c in cases]
     torch.cuda.synchronize()
     streams, got = [torch.cuda.Stream() for _ in cases], [[], []]

@@ -183,3 +183,21 @@ def test_on_another_stream(cuda_device):
         y = cmpext3.ops.rope(xd, pd, fd)
     s.synchronize()
     O.assert_within(y, *O.rope(x, positions, freqs), "side stream")
+
+
+def test_a_capture_of_a_leaf_with_an_eager_graph_is_refused(cuda_device):
+    x = torch.randn(1, 1, 8, 16, device=cuda_device, requires_grad=True)
+    positions, freqs = torch.arange(8, device=cuda_device), _freqs(8).to(cuda_device)
+    eager = cmpext3.ops.rope(x, positions, freqs)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph of this leaf"):
+        with torch.cuda.graph(graph):
+            cmpext3.ops.rope(x, positions, freqs)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = cmpext3.ops.rope(x, positions, freqs)
+        (grad,) = torch.autograd.grad(y.sum(), x)
+    graph.replay()
+    torch.cuda.synchronize()
+    O.assert_within(grad, *O.rope(torch.ones(1, 1, 8, 16), positions.cpu(), freqs.cpu(), sign=-1.0), "captured gradient")

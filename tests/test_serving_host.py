@@ -118,6 +118,24 @@ def _cache_refusals(call):
     refused("lengths must be a Tensor", call, kc, vc, table, [1, 1], error=TypeError)
 
 
+def test_a_leaf_with_an_eager_graph_is_refused_in_a_capture(monkeypatch):
+    # the note on the leaf's autograd node, with the streams and the capture played on the CPU
+    stream, capturing = [1], [False]
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: stream[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    x = torch.randn(3, requires_grad=True)
+    edge = S._note_leaf(x)
+    eager = x * 2                      # (recorded while the edge is held, as rope does)
+    del edge
+    stream[0] = 2
+    S._note_leaf(x)                    # another stream, no capture: torch's own business
+    capturing[0] = True
+    with pytest.raises(RuntimeError, match="eager graph of this leaf"):
+        S._note_leaf(x)
+    del eager                          # the node goes with the last graph that uses it
+    S._note_leaf(x)
+
+
 def test_kv_append_refusals(cpu):
     ops = cmpext3.ops
     k, q, f = torch.randn(2, 2, 3, 16), torch.randn(2, 4, 3, 16), torch.ones(8)
@@ -278,6 +296,8 @@ def test_linear_w4_plans_and_statuses():
         assert _status(f, _linear(**bad) if bad != dict(group=0) else S.LinearW4Desc(
             PTR, PTR, PTR, None, None, PTR, 2, 10, 256, 0, 256, 10, 128, 4, 0, 2, 0))[0] == N.ERR_INVALID_ARGUMENT, bad
     assert _status(f, _linear(group=16))[0] == N.ERR_UNSUPPORTED_SHAPE
+    assert _status(f, _linear(ws=(1 << 27) + 16))[0] == N.ERR_UNSUPPORTED_SHAPE
+    assert _status(f, _linear(n=1 << 30, k=1 << 20))[0] == N.ERR_UNSUPPORTED_SHAPE
     assert _status(f, _linear(dtype=4))[0] == N.ERR_UNSUPPORTED_DTYPE
     assert _status(f, _linear(xs=257))[0] == N.ERR_MISALIGNED
     assert _status(f, _linear(ws=130))[0] == N.ERR_MISALIGNED

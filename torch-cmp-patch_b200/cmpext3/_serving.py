@@ -278,6 +278,20 @@ def _rope_call(x, positions, freqs, sections, interleaved, inverse):
     return y
 
 
+def _note_leaf(x: torch.Tensor):
+    """The leaf's gradient edge, to be held until rope has recorded x (the leaf's node lives as long as somebody holds
+    it).  Refuses to record a leaf inside a graph capture while an eager graph that rope recorded of it on another stream
+    is alive: the captured backward pass would make that stream, which the leaf's node belongs to, wait for the
+    capturing one, an error in autograd's thread that ends the process.  The note lives as long as the node, that
+    is, as the graphs that use it."""
+    edge = torch.autograd.graph.get_gradient_edge(x)
+    notes = edge.node.metadata
+    stream = torch._C._cuda_getCurrentRawStream(x.device.index)
+    if notes.setdefault("cmpext3.rope stream", stream) != stream and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("rope: an eager graph of this leaf is alive; drop its outputs before the capture")
+    return edge
+
+
 class _Rope(torch.autograd.Function):
     """The rotation's gradient is the rotation by the negative angles (which has one, too)."""
 
@@ -308,12 +322,14 @@ def rope(input, positions, freqs, sections=None, interleaved=False):
     ``positions`` (int32, int64 or float32) is [tokens] or [batch, tokens].  With ``sections``, up to
     four counts that add up to pairs, positions has a leading axis of that many (time, height, width,
     ...): the first sections[0] pairs turn by positions[0], the next by positions[1], and so on.
-    Angles are computed in 64 bits; the result, a new tensor, is rounded once.  Differentiable in
-    ``input``; positions and freqs have no gradient.  head_dim <= 256."""
+    Angles are computed in 64 bits (good below 2^50 radians); the result, a new tensor, is rounded once.
+    Differentiable in ``input``; positions and freqs have no gradient.  A capture of forward and backward pass
+    into a CUDA graph needs its leaves free of eager graphs (RuntimeError).  head_dim <= 256."""
     sections, interleaved = None if sections is None else tuple(sections), bool(interleaved)
     if torch.is_grad_enabled():
         _no_grad_only("rope in positions and freqs", positions, freqs)
         if isinstance(input, torch.Tensor) and input.requires_grad:
+            _edge = _note_leaf(input) if input.is_leaf and input.is_cuda else None
             return _Rope.apply(input, positions, freqs, sections, interleaved, False)
     return _rope_call(input, positions, freqs, sections, interleaved, False)
 
@@ -548,7 +564,8 @@ def paged_attention_plan(query, k_cache, v_cache, page_table, lengths, scale=Non
 
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     """A 2-D operand with contiguous rows on 16-byte boundaries (a copy where it has none)."""
-    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] == 1 or t.stride(0) * t.element_size() % 16 == 0):
+    row = t.stride(0) * t.element_size()
+    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] == 1 or row % 16 == 0 and row <= 1 << 27):
         return t
     t = t.contiguous()
     return t.clone() if t.data_ptr() % 16 else t
@@ -598,7 +615,7 @@ def linear_w4(input, weight, scales, zeros=None, bias=None):
     scales [N, K // group] in input's dtype; zeros [N, K // group] uint8 (0..15), 8 everywhere when
     None; bias [N] in input's dtype.  group, a multiple of 32 that divides K, follows from scales.  The
     weights are not rounded (whole-number differences, fp32 sums, one product with the scale a group)
-    and the result is rounded once.  The weights are read once per 8 tokens: with many tokens a
+    and the result is rounded once.  The weights are read once per 16 tokens: with many tokens a
     dequantised weight and ``linear`` are the faster way."""
     if torch.is_grad_enabled():
         _no_grad_only("linear_w4", input, scales, bias)
