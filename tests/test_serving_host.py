@@ -119,21 +119,19 @@ def _cache_refusals(call):
 
 
 def test_a_leaf_with_an_eager_graph_is_refused_in_a_capture(monkeypatch):
-    # the note on the leaf's autograd node, with the streams and the capture played on the CPU
-    stream, capturing = [1], [False]
+    # the note on the leaf's autograd node, with the streams played on the CPU
+    stream = [1]
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: stream[0], raising=False)
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
     x = torch.randn(3, requires_grad=True)
-    edge = S._note_leaf(x)
-    eager = x * 2                      # (recorded while the edge is held, as rope does)
-    del edge
+    S._check_leaf(x)
+    eager = x * 2
+    S._note_leaf(eager, x.device)
+    S._check_leaf(x)                   # the same stream
     stream[0] = 2
-    S._note_leaf(x)                    # another stream, no capture: torch's own business
-    capturing[0] = True
     with pytest.raises(RuntimeError, match="eager graph of this leaf"):
-        S._note_leaf(x)
+        S._check_leaf(x)
     del eager                          # the node goes with the last graph that uses it
-    S._note_leaf(x)
+    S._check_leaf(x)
 
 
 def test_kv_append_refusals(cpu):

@@ -278,18 +278,23 @@ def _rope_call(x, positions, freqs, sections, interleaved, inverse):
     return y
 
 
-def _note_leaf(x: torch.Tensor):
-    """The leaf's gradient edge, to be held until rope has recorded x (the leaf's node lives as long as somebody holds
-    it).  Refuses to record a leaf inside a graph capture while an eager graph that rope recorded of it on another stream
-    is alive: the captured backward pass would make that stream, which the leaf's node belongs to, wait for the
-    capturing one, an error in autograd's thread that ends the process.  The note lives as long as the node, that
-    is, as the graphs that use it."""
-    edge = torch.autograd.graph.get_gradient_edge(x)
-    notes = edge.node.metadata
+_STREAM_NOTE = "cmpext3.rope stream"
+
+
+def _check_leaf(x: torch.Tensor) -> None:
+    """In a graph capture: refuses a leaf of which rope has recorded an eager graph on another stream that is alive.
+    The captured backward pass would make that stream, which the leaf's autograd node belongs to, wait for
+    the capturing one, an error in autograd's thread that ends the process.  The note is on the node, which lives
+    as long as the graphs that use it."""
     stream = torch._C._cuda_getCurrentRawStream(x.device.index)
-    if notes.setdefault("cmpext3.rope stream", stream) != stream and torch.cuda.is_current_stream_capturing():
+    if torch.autograd.graph.get_gradient_edge(x).node.metadata.get(_STREAM_NOTE, stream) != stream:
         raise RuntimeError("rope: an eager graph of this leaf is alive; drop its outputs before the capture")
-    return edge
+
+
+def _note_leaf(y: torch.Tensor, device: torch.device) -> None:
+    """Notes on the node of the leaf that y was computed from the stream on which that was recorded."""
+    notes = y.grad_fn.next_functions[0][0].metadata
+    notes.setdefault(_STREAM_NOTE, torch._C._cuda_getCurrentRawStream(device.index))
 
 
 class _Rope(torch.autograd.Function):
@@ -329,8 +334,13 @@ def rope(input, positions, freqs, sections=None, interleaved=False):
     if torch.is_grad_enabled():
         _no_grad_only("rope in positions and freqs", positions, freqs)
         if isinstance(input, torch.Tensor) and input.requires_grad:
-            _edge = _note_leaf(input) if input.is_leaf and input.is_cuda else None
-            return _Rope.apply(input, positions, freqs, sections, interleaved, False)
+            leaf = input.is_leaf and input.is_cuda
+            if leaf and torch.cuda.is_current_stream_capturing():
+                _check_leaf(input)
+            y = _Rope.apply(input, positions, freqs, sections, interleaved, False)
+            if leaf:
+                _note_leaf(y, input.device)
+            return y
     return _rope_call(input, positions, freqs, sections, interleaved, False)
 
 
