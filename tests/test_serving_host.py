@@ -310,7 +310,7 @@ def test_the_new_device_flag_is_the_header_s():
 
 # ---- the schedule of the paged attention ------------------------------------------------------
 
-TILE, COST, LEAST = 16, 2, 6
+TILE, COST, LEAST = 16, 3, 6
 
 
 def _stretches(lengths, items, workers):

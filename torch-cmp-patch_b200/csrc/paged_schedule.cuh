@@ -21,7 +21,7 @@
 namespace cmpx {
 
 constexpr int kTile = 16;      // keys per tile
-constexpr int kItemCost = 2;   // an item's fixed cost, in tiles
+constexpr int kItemCost = 3;   // an item's fixed cost, in tiles
 constexpr int kShareMin = 6;   // units per warp at least, where there are more warps than work
 
 struct PagedArgs {
