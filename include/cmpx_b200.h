@@ -360,7 +360,8 @@ typedef struct cmpx_paged_cache {
  * place lengths[b] - new_lengths[b] + i.  Rows i >= new_lengths[b] are padding: nothing is stored for
  * them and q_out gets q as it is (a batch row that is padding altogether has new_lengths 0).  A token whose place is negative, behind the table, or in a page
  * outside 0..num_pages-1 is not stored and raises CMPX_DEVFLAG_BAD_PAGE.  Two tokens of one call
- * that share a slot (a page that two sequences both append to) leave either's values there. */
+ * that share a slot (a page that two sequences both append to) leave either's values there; k and v must
+ * not overlap the cache. */
 typedef struct cmpx_kv_append_desc {
   const void* k;
   const void* v;

@@ -194,6 +194,12 @@ def test_a_capture_of_a_leaf_with_an_eager_graph_is_refused(cuda_device):
         with torch.cuda.graph(graph):
             cmpext3.ops.rope(x, positions, freqs)
     del eager
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):      # a warm-up, whose graph stays alive
+        warm = cmpext3.ops.rope(x, positions, freqs)
+        torch.autograd.grad(warm.sum(), x)
+    torch.cuda.current_stream().wait_stream(side)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         y = cmpext3.ops.rope(x, positions, freqs)

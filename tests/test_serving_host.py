@@ -120,17 +120,19 @@ def _cache_refusals(call):
 
 def test_a_leaf_with_an_eager_graph_is_refused_in_a_capture(monkeypatch):
     # the note on the leaf's autograd node, with the streams played on the CPU
-    stream = [1]
+    stream = [0]
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: stream[0], raising=False)
     x = torch.randn(3, requires_grad=True)
     S._check_leaf(x)
     eager = x * 2
     S._note_leaf(eager, x.device)
-    S._check_leaf(x)                   # the same stream
-    stream[0] = 2
     with pytest.raises(RuntimeError, match="eager graph of this leaf"):
         S._check_leaf(x)
     del eager                          # the node goes with the last graph that uses it
+    S._check_leaf(x)
+    stream[0] = 5                      # a warm-up on a side stream may stay alive
+    eager = x * 2
+    S._note_leaf(eager, x.device)
     S._check_leaf(x)
 
 

@@ -282,13 +282,14 @@ _STREAM_NOTE = "cmpext3.rope stream"
 
 
 def _check_leaf(x: torch.Tensor) -> None:
-    """In a graph capture: refuses a leaf of which rope has recorded an eager graph on another stream that is alive.
-    The captured backward pass would make that stream, which the leaf's autograd node belongs to, wait for
-    the capturing one, an error in autograd's thread that ends the process.  The note is on the node, which lives
-    as long as the graphs that use it."""
-    stream = torch._C._cuda_getCurrentRawStream(x.device.index)
-    if torch.autograd.graph.get_gradient_edge(x).node.metadata.get(_STREAM_NOTE, stream) != stream:
-        raise RuntimeError("rope: an eager graph of this leaf is alive; drop its outputs before the capture")
+    """In a graph capture: refuses a leaf of which rope has recorded an eager graph on the default stream that is
+    alive.  The captured backward pass would make that stream, which the leaf's autograd node belongs to and
+    which cannot be captured, wait for the capturing one, an error in autograd's thread that ends the process (a
+    graph recorded on a side stream, as in a warm-up, does no harm).  The note is on the node, which lives as long
+    as the graphs that use it."""
+    if torch.autograd.graph.get_gradient_edge(x).node.metadata.get(_STREAM_NOTE) == 0:
+        raise RuntimeError("rope: an eager graph of this leaf from the default stream is alive; drop its outputs "
+                           "before the capture")
 
 
 def _note_leaf(y: torch.Tensor, device: torch.device) -> None:
@@ -327,9 +328,11 @@ def rope(input, positions, freqs, sections=None, interleaved=False):
     ``positions`` (int32, int64 or float32) is [tokens] or [batch, tokens].  With ``sections``, up to
     four counts that add up to pairs, positions has a leading axis of that many (time, height, width,
     ...): the first sections[0] pairs turn by positions[0], the next by positions[1], and so on.
-    Angles are computed in 64 bits (good below 2^50 radians); the result, a new tensor, is rounded once.
+    Angles are computed in 64 bits (good below 2^50 radians); the result, a new tensor laid out as
+    input, is rounded once.
     Differentiable in ``input``; positions and freqs have no gradient.  A capture of forward and backward pass
-    into a CUDA graph needs its leaves free of eager graphs (RuntimeError).  head_dim <= 256."""
+    into a CUDA graph needs its leaves free of eager graphs from the default stream (RuntimeError).
+    head_dim <= 256."""
     sections, interleaved = None if sections is None else tuple(sections), bool(interleaved)
     if torch.is_grad_enabled():
         _no_grad_only("rope in positions and freqs", positions, freqs)
@@ -440,7 +443,8 @@ def kv_append(key, value, k_cache, v_cache, page_table, lengths, new_lengths=Non
     was.  A token's position is its place in its sequence unless ``positions`` says otherwise.
 
     A token whose place is negative, behind the table or in a page that does not exist is not stored and
-    sets a bit of ``device_status()``.  Which of two tokens that share a slot stays is not defined."""
+    sets a bit of ``device_status()``.  Which of two tokens that share a slot stays is not defined; key and
+    value must not lie in the caches' memory."""
     sections, interleaved = None if sections is None else tuple(sections), bool(interleaved)
     if torch.is_grad_enabled():
         _no_grad_only("kv_append", key, value, k_cache, v_cache, query, positions, freqs)
@@ -527,7 +531,8 @@ def paged_attention(query, k_cache, v_cache, page_table, lengths, scale=None):
 
     A sequence of length 0 gets zeros.  A length beyond the table, or a page that does not exist among a
     sequence's pages, makes that sequence's rows NaN and sets a bit of ``device_status()``.  The lengths
-    are read on the device: a captured call can be replayed with other ones."""
+    are read on the device: a captured call can be replayed with other ones.  The schedule goes by the
+    table's width: a table much wider than the sequences are long costs a few microseconds."""
     scale = None if scale is None else float(scale)
     if torch.is_grad_enabled():
         _no_grad_only("paged_attention", query, k_cache, v_cache)

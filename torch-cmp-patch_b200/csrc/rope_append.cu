@@ -91,9 +91,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(APPEND)) rope_append_k
   const int tokens_per_block = kThreads / a.chunks;
   const int tok = threadIdx.x / a.chunks;
   const int c = threadIdx.x - tok * a.chunks;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * tokens_per_block + tok;
-  if (tok >= tokens_per_block || t >= static_cast<int64_t>(a.batch) * a.len) return;
-  const int b = static_cast<int>(t / a.len), l = static_cast<int>(t - static_cast<int64_t>(b) * a.len);
+  const uint32_t t = blockIdx.x * tokens_per_block + tok;  // batch * len is below 2^31 - 65536
+  if (tok >= tokens_per_block || t >= static_cast<uint32_t>(a.batch) * static_cast<uint32_t>(a.len)) return;
+  const int b = static_cast<int>(t / static_cast<uint32_t>(a.len)), l = static_cast<int>(t - static_cast<uint32_t>(b) * a.len);
 
   const int rot_chunks = a.pairs / VEC;
   const bool turned = c < rot_chunks;
