@@ -14,13 +14,15 @@
 // its registers; the others' parts are summed once, at the CTA's end, in a fixed order.
 // A lane multiplies 16 k of a row that lie side by side, and the products run over k in the order that falls out
 // of it: word j of the lanes tq = 0..3 holds k = 16 tq + 8 j .. + 7, and nibbles e and e + 4 of a word, which
-// one mask isolates as the halves of a register, are a pair.  16-bit activations of up to 64 KB are laid out
-// in that order in shared memory once per CTA; others follow it with one byte permutation a register.
+// one mask isolates as the halves of a register, are a pair.  Activations of up to 64 KB (2 bytes a value, fp32's
+// parts 6) are laid out in that order in shared memory once per CTA; others follow it with one byte
+// permutation a register, and fp32's are cut again for every tile (1 x 16384 x 4096 fp32: 18 us from
+// shared memory, 26 without).
 // What bounds it beside the bytes: first the lines that its loads touch (one a cycle), which is why eight lanes load
 // 128 bytes of a row together and scales and zero points come for sets of turns, through a table in shared
 // memory; then the half-rate units: for eight weights 3 shifts and 4 masks beside 4 subtractions (fp16: 1,
-// 4, 4).  Measured from a graph: 8 x 16384 x 4096 fp16, groups of 64: 14.7 us for 37 MB (5.7 at the
-// copy rate; 8 x 131072 x 4096: 70 us, 4.3 TB/s); 1 x 4096 x 4096 bf16: 5.9 us, most of it the launch and one pass
+// 4, 4).  Measured from a graph: 8 x 16384 x 4096 fp16, groups of 64: 15 us for 37 MB (5.7 at the
+// copy rate; 8 x 131072 x 4096: 72 us, 4.1 TB/s); 1 x 4096 x 4096 bf16: 5.9 us, most of it the launch and one pass
 // through the pipeline.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -187,7 +189,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
   uint8_t* const mine = smem + warp * C::WARP;
   const uint32_t buf = smem_u32(mine);
   float2* const table = reinterpret_cast<float2*>(mine + kStages * C::STAGE);
-  uint4* const x_all = reinterpret_cast<uint4*>(smem + C::SMEM);  // [quarter][word][NT][lane]
+  constexpr int PARTS = Activations<DT>::PARTS;
+  uint4* const x_all = reinterpret_cast<uint4*>(smem + C::SMEM);  // [quarter][word][part][token][tq]
+  const int x_lanes = 4 * min(8 * NT, a.m - m0);
   // A warp's parts of tiles that it shares, [token][kRows + 1]: of its run's first tile in a place of its own,
   // of a later one, which is its last, where its first buffer was.
   auto part_of = [&](int w, bool later) {
@@ -280,10 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
       if (!FULL && k >= a.k) break;
       Activations<DT> x[2][NT];
       if (XS) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int t = 0; t < NT; ++t) x[j][t].v[0] = x_all[((k / 64 * 2 + j) * NT + t) * 32 + lane];
+        // (read below)
       } else if (AHEAD && FULL) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -321,17 +322,22 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
         codes_minus_zero<DT>(j ? w[1].y : w[1].x, __float_as_uint(col[1].y), d1);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          uint32_t p[Activations<DT>::PARTS][4];
+          uint32_t p[PARTS][4];
           if (XS) {
-            p[0][0] = x[j][t].v[0].x;
-            p[0][1] = x[j][t].v[0].y;
-            p[0][2] = x[j][t].v[0].z;
-            p[0][3] = x[j][t].v[0].w;
+            // lanes of tokens that are not there read the last one's: columns that are not written
+#pragma unroll
+            for (int y = 0; y < PARTS; ++y) {
+              const uint4 v = x_all[((k / 64 * 2 + j) * PARTS + y) * x_lanes + min(t * 32 + lane, x_lanes - 1)];
+              p[y][0] = v.x;
+              p[y][1] = v.y;
+              p[y][2] = v.z;
+              p[y][3] = v.w;
+            }
           } else {
             x[j][t].pairs(p);
           }
 #pragma unroll
-          for (int y = 0; y < Activations<DT>::PARTS; ++y) {
+          for (int y = 0; y < PARTS; ++y) {
 #pragma unroll
             for (int set = 0; set < SETS; ++set) {
               // groups of 32: the quad's first two lanes are in one group, its last two in the next
@@ -379,35 +385,37 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
   int tile = tile0 + u0 / chunks, c = u0 % chunks;
   load_groups(tile, c / C::SUPER);
   if constexpr (XS) {
-    // (what the lanes of tokens that are not there find makes columns that are not written)
-    const int lanes = 4 * min(8 * NT, a.m - m0), count = (a.k + 63) / 64 * 2 * lanes;
+    const int count = (a.k + 63) / 64 * 2 * x_lanes;
     auto fill = [&](auto full, auto at_once) {  // full: all 8 NT tokens are there; at_once: loads in flight per thread
       constexpr int AT_ONCE = decltype(at_once)::value;
       for (int i0 = threadIdx.x; i0 < count; i0 += AT_ONCE * kThreads) {
         Activations<DT> x[AT_ONCE];
-        int to[AT_ONCE];
+        int set[AT_ONCE], l[AT_ONCE];  // set: quarter and word
 #pragma unroll
         for (int e = 0; e < AT_ONCE; ++e) {
           const int i = i0 + e * kThreads;
-          const int set = decltype(full)::value ? i / (32 * NT) : i / lanes, l = i - set * lanes;  // set: quarter and word
-          const int k = set / 2 * 64 + (l & 3) * 16 + set % 2 * 8;
-          to[e] = i < count ? (set * NT + l / 32) * 32 + l % 32 : -1;
+          set[e] = decltype(full)::value ? i / (32 * NT) : i / x_lanes;
+          l[e] = i - set[e] * x_lanes;
+          const int k = set[e] / 2 * 64 + (l[e] & 3) * 16 + set[e] % 2 * 8;
           if (i < count && k < a.k)
-            x[e].load(a.x + static_cast<int64_t>(m0 + (l >> 2)) * a.xs + k * ES);
+            x[e].load(a.x + static_cast<int64_t>(m0 + (l[e] >> 2)) * a.xs + k * ES);
           else
             x[e].zero();
         }
 #pragma unroll
         for (int e = 0; e < AT_ONCE; ++e) {
-          uint32_t p[Activations<DT>::PARTS][4];
+          uint32_t p[PARTS][4];
           x[e].pairs(p);
-          if (to[e] >= 0) x_all[to[e]] = make_uint4(p[0][0], p[0][1], p[0][2], p[0][3]);
+#pragma unroll
+          for (int y = 0; y < PARTS; ++y)
+            if (i0 + e * kThreads < count)
+              x_all[(set[e] * PARTS + y) * x_lanes + l[e]] = make_uint4(p[y][0], p[y][1], p[y][2], p[y][3]);
         }
       }
     };
     if (count <= kThreads) fill(std::false_type{}, std::integral_constant<int, 1>{});
-    else if (lanes < 32 * NT) fill(std::false_type{}, std::integral_constant<int, 4>{});
-    else fill(std::true_type{}, std::integral_constant<int, 8>{});
+    else if (x_lanes < 32 * NT) fill(std::false_type{}, std::integral_constant<int, 4>{});
+    else fill(std::true_type{}, std::integral_constant<int, DT == CMPX_F32 ? 4 : 8>{});
     __syncthreads();
   }
   // (a partial last turn leaves x_ahead at the row's begin, where the next tile's first turn needs it)
@@ -485,6 +493,12 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
 
 GroupKind group_kind(int64_t group) { return group % 128 == 0 ? kGroup128 : group % 64 == 0 ? kGroup64 : kGroup32; }
 
+// Bytes of a CTA's activations as the products take them.
+template <int DT, int NT>
+int64_t x_bytes(const W4Args& a) {
+  return static_cast<int64_t>(a.k + 63) / 64 * 64 * 2 * Activations<DT>::PARTS * std::min(8 * NT, a.m);
+}
+
 template <int DT, int NT, int GK, bool XS>
 int launch_as(W4Args& a, const LaunchCtx& ctx) {
   using C = W4Cfg<DT, NT, GK, XS>;
@@ -503,15 +517,15 @@ int launch_as(W4Args& a, const LaunchCtx& ctx) {
   a.tiles_per_cta = tiles / ctas;
   a.tiles_rest = tiles % ctas;
   const dim3 grid(static_cast<unsigned>(ctas), static_cast<unsigned>((a.m + 8 * NT - 1) / (8 * NT)));
-  kernel<<<grid, kThreads, C::SMEM + (XS ? (a.k + 63) / 64 * (2 * NT * 512) : 0), ctx.stream>>>(a);
+  kernel<<<grid, kThreads, C::SMEM + (XS ? static_cast<int>(x_bytes<DT, NT>(a)) : 0), ctx.stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? CMPX_OK : CMPX_ERR_LAUNCH;
 }
 
 template <int DT, int NT, int GK>
 int launch(W4Args& a, const LaunchCtx& ctx) {
-  // Activations of up to 64 KB (8 tokens: 4096 k) are laid out for the products once per CTA.
-  if constexpr (DT != CMPX_F32)
-    if ((a.k + 63) / 64 * (2 * NT * 512) <= W4Cfg<DT, NT, GK, true>::X_MOST) return launch_as<DT, NT, GK, true>(a, ctx);
+  // Activations of up to 64 KB (16-bit: 8 tokens of 4096 k; fp32 takes 6 bytes a value) are laid out for the products
+  // once per CTA.
+  if (x_bytes<DT, NT>(a) <= W4Cfg<DT, NT, GK, true>::X_MOST) return launch_as<DT, NT, GK, true>(a, ctx);
   return launch_as<DT, NT, GK, false>(a, ctx);
 }
 
