@@ -92,6 +92,14 @@ def test_head_layouts_of_long_caches(cuda_device, dtype, H, Hkv, D, lengths):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("D", [64, 256])
+def test_many_rows_beside_a_long_one(cuda_device, dtype, D):
+    # more rows than SMs, one of them in many parts; then more sequences than a block has threads
+    Case(dtype, 8, 2, D, 16, [9000] + [20] * 30, seed=17).check()
+    Case(dtype, 2, 2, D, 16, [1500] + [7, 0, 300] * 60, seed=18).check()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_one_head_over_a_long_context(cuda_device, dtype):
     Case(dtype, 1, 1, 128, 64, [70001], seed=3).check()
 

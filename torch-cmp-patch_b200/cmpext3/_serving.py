@@ -22,7 +22,7 @@ import struct
 
 import torch
 
-from ._native import OK, CmpxError, _DTYPE, _post_check, _stream_handle, _traced, lib
+from ._native import _CHECK, _DTYPE, OK, CmpxError, _post_check, _stream_handle, _traced, lib
 
 _MAX_AXES = 4
 _POS_KIND = {torch.int32: 1, torch.int64: 2, torch.float32: 3}
@@ -90,11 +90,17 @@ lib.cmpx_paged_attn_workspace_size.restype = ctypes.c_size_t
 # of the checks.  A call whose pointers the kernel declines (misaligned ones) goes the long way again.
 _SIGNATURES: dict = {}
 _SIGNATURES_MOST = 4096
-_DIRECT = {}
-for _name in ("rope", "kv_append", "paged_attn", "linear_w4"):
-    _fn = lib[f"cmpx_{_name}"]  # the same entry point, taking the descriptor as bytes
-    _fn.argtypes, _fn.restype = [ctypes.c_char_p, ctypes.c_void_p], ctypes.c_int
-    _DIRECT[_name] = _fn
+
+
+def _from_bytes(name: str):
+    """The entry point, taking its descriptor as bytes."""
+    fn = lib[name]
+    fn.argtypes, fn.restype = [ctypes.c_char_p, ctypes.c_void_p], ctypes.c_int
+    return fn
+
+
+_ROPE, _KV_APPEND, _PAGED_ATTN, _LINEAR_W4 = map(_from_bytes, ("cmpx_rope", "cmpx_kv_append", "cmpx_paged_attn",
+                                                              "cmpx_linear_w4"))
 _pack2, _pack4, _pack6, _pack7, _pack9 = (struct.Struct(f"={n}Q").pack for n in (2, 4, 6, 7, 9))
 
 
@@ -116,11 +122,19 @@ def _alike(shape, dtype, device) -> torch.Tensor:
     return one.expand(shape)
 
 
+_grad_on, _like_of = torch.is_grad_enabled, torch.empty_like
+_device_now, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _direct(fn, data: bytes, index: int) -> int:
-    if index == torch._C._cuda_getDevice():
-        return fn(data, torch._C._cuda_getCurrentRawStream(index))
-    with torch.cuda.device(index):
-        return fn(data, torch._C._cuda_getCurrentRawStream(index))
+    if index == _device_now():
+        st = fn(data, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            st = fn(data, _raw_stream(index))
+    if st == OK and _CHECK:
+        _post_check()
+    return st
 
 
 def _run(what: str, fn, desc, device: torch.device) -> None:
@@ -265,10 +279,8 @@ def _rope_call(x, positions, freqs, sections, interleaved, inverse):
         key = how = None
     if how is not None:
         tail, index = how
-        y = torch.empty_like(x)
-        if _direct(_DIRECT["rope"], _pack4(x.data_ptr(), y.data_ptr(), positions.data_ptr(), freqs.data_ptr()) + tail,
-                   index) == OK:
-            _post_check()
+        y = _like_of(x)
+        if _direct(_ROPE, _pack4(x.data_ptr(), y.data_ptr(), positions.data_ptr(), freqs.data_ptr()) + tail, index) == OK:
             return y
     desc, y, used = _rope_desc(x, positions, freqs, sections, interleaved, inverse)
     if y.numel():
@@ -460,15 +472,14 @@ def kv_append(key, value, k_cache, v_cache, page_table, lengths, new_lengths=Non
         sig = how = None
     if how is not None:
         middle, tail, index = how
-        out = None if query is None else torch.empty_like(query)
+        out = None if query is None else _like_of(query)
         data = b"".join((
             _pack9(key.data_ptr(), value.data_ptr(), 0 if out is None else query.data_ptr(),
                    0 if out is None else out.data_ptr(), 0 if new_lengths is None else new_lengths.data_ptr(),
                    k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), lengths.data_ptr()),
             middle, _pack2(0 if positions is None else positions.data_ptr(), 0 if freqs is None else freqs.data_ptr()),
             tail))
-        if _direct(_DIRECT["kv_append"], data, index) == OK:
-            _post_check()
+        if _direct(_KV_APPEND, data, index) == OK:
             _changed(k_cache, v_cache)
             return out
     desc, out, used = _append_desc(key, value, k_cache, v_cache, page_table, lengths, new_lengths, query, positions,
@@ -546,12 +557,11 @@ def paged_attention(query, k_cache, v_cache, page_table, lengths, scale=None):
         sig = how = None
     if how is not None:
         tail, scratch, index = how
-        out = torch.empty_like(query)
-        ws = None if scratch is None else torch.empty_like(scratch)
+        out = _like_of(query)
+        ws = None if scratch is None else _like_of(scratch)
         data = _pack7(query.data_ptr(), out.data_ptr(), 0 if ws is None else ws.data_ptr(), k_cache.data_ptr(),
                       v_cache.data_ptr(), page_table.data_ptr(), lengths.data_ptr()) + tail
-        if _direct(_DIRECT["paged_attn"], data, index) == OK:
-            _post_check()
+        if _direct(_PAGED_ATTN, data, index) == OK:
             return out
     desc, out, used = _paged_attn_desc(query, k_cache, v_cache, page_table, lengths, scale)
     if out.numel():
@@ -644,11 +654,10 @@ def linear_w4(input, weight, scales, zeros=None, bias=None):
         sig = how = None
     if how is not None:
         tail, like, index = how
-        y = torch.empty_like(like)
+        y = _like_of(like)
         data = _pack6(input.data_ptr(), weight.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(),
                       0 if bias is None else bias.data_ptr(), y.data_ptr()) + tail
-        if _direct(_DIRECT["linear_w4"], data, index) == OK:
-            _post_check()
+        if _direct(_LINEAR_W4, data, index) == OK:
             return y
     desc, y, used = _linear_w4_desc(input, weight, scales, zeros, bias)
     shape = tuple(input.shape[:-1]) + (y.shape[1],)
