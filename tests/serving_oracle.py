@@ -46,8 +46,8 @@ def rope(x, positions, freqs, sections=None, interleaved=False, sign=1.0):
     out[..., re], out[..., im] = u * cos - w * sin, u * sin + w * cos
     size[..., re] = size[..., im] = u.abs() + w.abs()
     far[..., re] = far[..., im] = angle.abs()[:, None].expand_as(u)
-    # cos and sin are off by at most 2^-23 (half a step of the fp32 remainder times pi / 2, and
-    # sincospi's own), the two products and the sum by 2^-24 each of at most |u| + |w|; an angle of a
+    # cos and sin are off by at most 2^-23 (half a step of the fp32 remainder, and their
+    # polynomials' own), the two products and the sum by 2^-24 each of at most |u| + |w|; an angle of a
     # radians carries four roundings of 2^-53 a between the kernel and this definition
     return out, rounding(out, x.dtype) + size * (2.0 ** -21 + far * 2.0 ** -51)
 

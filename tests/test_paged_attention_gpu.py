@@ -163,6 +163,17 @@ def test_infinite_values_and_scores(cuda_device, dtype, n):
     O.assert_within(out, want, bound, "a key with a score of -inf")
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("lengths", [[40, 0], [3000, 0], [9000, 0], [9000, 0] + [20] * 300])
+def test_scores_that_are_all_minus_infinity_have_no_softmax(cuda_device, dtype, lengths):
+    c = Case(dtype, 4, 2, 64, 16, lengths, seed=19)
+    c.args[0][..., 3] = 2.0
+    c.args[1][:, 1, :, 3] = -float("inf")
+    out = cmpext3.ops.paged_attention(*c.args)
+    some = [b for b, n in enumerate(lengths) if n]
+    assert torch.isnan(out[some][:, 2:]).all() and torch.isfinite(out[some][:, :2]).all() and (out[1] == 0).all()
+
+
 def test_nan_and_infinite_keys_spread_to_their_sequence_alone(cuda_device):
     c = Case(torch.bfloat16, 4, 2, 64, 16, [40, 700, 30], seed=8)
     c.args[1][int(c.table[1, 20]), 0, 3] = float("nan")

@@ -60,9 +60,9 @@ __global__ void __launch_bounds__(32 * W) paged_join_kernel(const __grid_constan
   const int tiles = seq_tiles(a, b);
   const int kvh = h / a.group, g = h - kvh * a.group, part = g / a.item_heads;
   const int64_t begin = first + (static_cast<int64_t>(kvh) * a.items_per_head + part) * (tiles + kItemCost) + kItemCost;
-  const int64_t c0 = begin / share, c1 = (begin + tiles - 1) / share;
+  const int64_t c0 = begin / share, c1 = min((begin + tiles - 1) / share, a.workers - 1);
   pdl_wait();  // every block: this kernel is not done before the main one is
-  if (!there || c0 == c1) return;  // written by its warp
+  if (!there || c0 >= c1) return;  // written by its warp
   const int hh = g - part * a.item_heads;
   float m = -INFINITY, l = 0.f;
   float4 o[V];
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(32 * W) paged_join_kernel(const __grid_constan
   }
   uint8_t* const out = a.o + b * a.o_sb + h * a.o_sh;
   if (WROW == 1) {
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = inverse_sum(l, false);  // (a row in several parts has keys)
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int d = 4 * (lane + 32 * v);
@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(32 * W) paged_join_kernel(const __grid_constan
       sum = fmaf(weight, sm_ml[w][1], sum);
       acc = fmaf(weight, reinterpret_cast<const float*>(sm_o[w])[d], acc);
     }
-    const float r = sum == 0.f ? 0.f : acc / sum;
+    const float r = acc * inverse_sum(sum, false);
     *reinterpret_cast<RawVec<ES>*>(out + d * ES) = pack_vec<DT, ES>(&r);
   }
 }

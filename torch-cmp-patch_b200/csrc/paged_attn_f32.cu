@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == kPagedWarps ? kCtasPerS
           *reinterpret_cast<float4*>(sm_o + (warp * HG + h) * DP + col[i]) =
               make_float4(o[h][4 * i], o[h][4 * i + 1], o[h][4 * i + 2], o[h][4 * i + 3]);
       }
-      join_cluster<kWarps, HG, DP>(st.nh, a.head_dim, sm_o, &sm_ml[0][0], cta_ml, [&](int h, int d, float x, float y) {
+      join_cluster<kWarps, HG, DP>(st.nh, a.head_dim, st.empty, sm_o, &sm_ml[0][0], cta_ml, [&](int h, int d, float x, float y) {
         *reinterpret_cast<float2*>(a.o + st.b * a.o_sb + (st.h0 + h) * a.o_sh + d * 4) = make_float2(x, y);
       });
       break;
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == kPagedWarps ? kCtasPerS
     for (int h = 0; h < HG; ++h) {
       if (h >= st.nh || group != 0) continue;
       const float sum = bad ? __int_as_float(0x7fffffff) : l[h];
-      const float f = st.slot >= 0 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+      const float f = st.slot >= 0 ? 1.f : inverse_sum(sum, st.empty);
       const int64_t row = st.slot * a.item_heads + h;
       float* const p = st.slot < 0 ? reinterpret_cast<float*>(a.o + st.b * a.o_sb + (st.h0 + h) * a.o_sh)
                                    : a.part_o + row * a.head_dim;

@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == kPagedWarps ? MmaCfg<DP
           *reinterpret_cast<float2*>(sm_o + (warp * 16 + h) * DP + i * 8 + tq * 2) =
               make_float2(o[i][2 * r], o[i][2 * r + 1]);
       }
-      join_cluster<kWarps, 16, DP>(st.nh, a.head_dim, sm_o, &sm_ml[0][0], cta_ml, [&](int h, int d, float x, float y) {
+      join_cluster<kWarps, 16, DP>(st.nh, a.head_dim, st.empty, sm_o, &sm_ml[0][0], cta_ml, [&](int h, int d, float x, float y) {
         *reinterpret_cast<uint32_t*>(a.o + st.b * a.o_sb + (st.h0 + h) * a.o_sh + d * 2) = pack2<DT>(x, y);
       });
       break;
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == kPagedWarps ? MmaCfg<DP
       if (h >= st.nh) continue;
       const float sum = bad ? __int_as_float(0x7fffffff) : l[r];
       if (st.slot < 0) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const float inv = inverse_sum(sum, st.empty);
         uint8_t* p = a.o + st.b * a.o_sb + (st.h0 + h) * a.o_sh + tq * 4;
 #pragma unroll
         for (int i = 0; i < DP / 8; ++i)

@@ -137,8 +137,15 @@ __device__ __forceinline__ Share find_share(const PagedArgs& a, int64_t* scratch
 struct Stretch {
   int b, kvh, h0, nh, key0, key1;
   int64_t slot;
-  bool bad;  // the sequence's length is beyond the table
+  bool bad;    // the sequence's length is beyond the table
+  bool empty;  // it has no keys
 };
+
+// One over a row's sum of weights: 0 of a sequence without keys.  Keys whose scores are all -inf (the only other
+// way to no weight: the largest is 1) have no softmax: NaN.
+__device__ __forceinline__ float inverse_sum(float sum, bool empty) {
+  return sum != 0.f ? 1.f / sum : empty ? 0.f : __int_as_float(0x7fffffff);
+}
 
 __device__ __forceinline__ void stretch_heads(const PagedArgs& a, int item, Stretch& st) {
   st.kvh = item / a.items_per_head;
@@ -154,7 +161,8 @@ __device__ __forceinline__ bool next_stretch(const PagedArgs& a, Share& s, Stret
     int units = seq_tiles(a, s.b) + kItemCost;
     while (s.cur >= s.before + static_cast<int64_t>(units) * items) {
       s.before += static_cast<int64_t>(units) * items;
-      units = seq_tiles(a, ++s.b) + kItemCost;
+      if (++s.b >= a.batch) return false;  // (lengths that were written meanwhile)
+      units = seq_tiles(a, s.b) + kItemCost;
     }
     const int64_t off = s.cur - s.before;
     const int item = static_cast<int>(off / units);
@@ -167,6 +175,7 @@ __device__ __forceinline__ bool next_stretch(const PagedArgs& a, Share& s, Stret
     st.b = s.b;
     stretch_heads(a, item, st);
     const int n = seq_len(a, st.b, st.bad);
+    st.empty = n == 0;
     st.key0 = min(n, tile0 * kTile);
     st.key1 = tile1 == tiles ? n : tile1 * kTile;
     st.slot = tile0 == 0 && tile1 == tiles ? -1 : s.slot + (tile0 == 0 ? 1 : 0);
@@ -183,6 +192,7 @@ __device__ __forceinline__ Stretch whole_item(const PagedArgs& a, int64_t index,
   stretch_heads(a, static_cast<int>(index - static_cast<int64_t>(st.b) * items), st);
   const int n = seq_len(a, st.b, st.bad);
   const int64_t tiles = (n + kTile - 1) / kTile;
+  st.empty = n == 0;
   st.key0 = static_cast<int>(tiles * rank / ranks) * kTile;
   st.key1 = min(n, static_cast<int>(tiles * (rank + 1) / ranks) * kTile);
   st.slot = -1;
@@ -278,7 +288,7 @@ struct KeyPipe {
 // warp's (cta_ml [ROWS]: maxima and sums), then every CTA its part of the cluster's.  store(h, d, x, y) gets two
 // neighbouring values of head h.
 template <int WARPS, int ROWS, int DP, typename Store>
-__device__ __forceinline__ void join_cluster(int nh, int head_dim, float* sm_o, const float2* sm_ml, float2* cta_ml,
+__device__ __forceinline__ void join_cluster(int nh, int head_dim, bool empty, float* sm_o, const float2* sm_ml, float2* cta_ml,
                                              Store store) {
   const int ranks = cluster_size();
   __syncthreads();
@@ -299,7 +309,7 @@ __device__ __forceinline__ void join_cluster(int nh, int head_dim, float* sm_o, 
       x1 = fmaf(weight, v.y, x1);
     }
     if (ranks == 1) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const float inv = inverse_sum(sum, empty);
       store(h, d, x0 * inv, x1 * inv);
     } else {
       *reinterpret_cast<float2*>(sm_o + h * DP + d) = make_float2(x0, x1);  // read by this thread alone so far
@@ -334,7 +344,7 @@ __device__ __forceinline__ void join_cluster(int nh, int head_dim, float* sm_o, 
       x0 = fmaf(weight, v[r].x, x0);
       x1 = fmaf(weight, v[r].y, x1);
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float inv = inverse_sum(sum, empty);
     store(h, d, x0 * inv, x1 * inv);
   }
   cluster_sync();  // nobody leaves while its results are read
