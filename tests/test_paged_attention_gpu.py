@@ -74,7 +74,7 @@ def test_every_short_length(cuda_device, dtype):
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("lengths,schedule", [
     ([20000], "equal shares"), ([9000, 3, 0, 1200], "equal shares"), ([0, 0, 0, 9000], "equal shares"),
-    ([600] * 200, "equal shares"), ([1, 0, 1300, 17] * 40, "equal shares"),
+    ([600] * 300, "equal shares"), ([1, 0, 1300, 17] * 40, "equal shares"),
     ([0, 0, 0], "one CTA"), ([1] * 700, "one CTA"), ([130, 129, 128] * 30, "one CTA"), ([500] * 200, "one CTA"),
     ([4096] * 3, "cluster"), ([513], "cluster"), ([8192], "cluster"), ([600, 0, 1, 599], "cluster"), ([2000, 15] * 4, "cluster")])
 def test_every_schedule(cuda_device, dtype, lengths, schedule):

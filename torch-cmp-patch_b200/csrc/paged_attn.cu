@@ -178,7 +178,9 @@ Schedule schedule(const cmpx_paged_attn_desc* d, int num_sms) {
   // Whole items, by one CTA or a cluster of 2, 4 or 8 (256 keys each): one launch and no join.  The CTAs have to
   // fit on the GPU at once, and a cluster's into one GPC: 7/8 of the places can be counted on, 3/4 where a cluster
   // takes 8 SMs.  Where they are few, each has an SM to itself and twice the warps, for the loads in
-  // flight ([1, 32/8, 128] bf16, 4096 keys: 10.5 us; equal shares and a join 13.5).
+  // flight ([1, 32/8, 128] bf16, 4096 keys: 10.5 us; equal shares and a join 13.5).  Of many, that lengths differ
+  // costs less than the join does ([100, 16/4, 64] fp16, 900 keys: 19.4 us; equal shares 23.4; [64, 32/8, 64], 10 to
+  // 1000 keys: 15.4 and 14.3).
   auto fits = [&](int ranks) { return s.items * ranks * 8 <= slots * (per_sm == 1 && ranks == 8 ? 6 : 7); };
   int ranks = 1;
   while (ranks < 8 && keys > 256 * ranks && fits(2 * ranks)) ranks *= 2;

@@ -34,8 +34,11 @@ constexpr int kKeys = 16;  // keys per buffer
 template <int DP>
 struct MmaCfg {
   static constexpr int ROW = DP * 2;                     // bytes of a row
-  static constexpr int STAGES = DP == 64 ? 6 : DP == 192 ? 2 : 3;
-  static constexpr int CTAS = DP == 256 ? 1 : 2;         // per SM: 96 KB of buffers each (192 KB at 256)
+  static constexpr int STAGES = DP == 192 ? 2 : 3;
+  // Per SM: 192 KB of buffers in all.  At 64, where a tile is 4 KB and its products' latency counts, more warps with
+  // fewer buffers each serve better ([8, 16 heads, 4 key heads, 40] fp16 with 39062 keys: 51 us, 59 with two CTAs
+  // and six stages); at 128 they do not (3 CTAs and two stages: 39.7 us for 12207 keys, 38.8 so).
+  static constexpr int CTAS = DP == 64 ? 4 : DP == 256 ? 1 : 2;
   using Pipe = KeyPipe<ROW, kKeys, STAGES, true>;
   static_assert(Pipe::BYTES >= 16 * DP * 4, "the warps' outputs are joined in the buffers");
 };
@@ -294,7 +297,9 @@ int launch_dt(const PagedArgs& a, int ctas, int ranks, int warps, const LaunchCt
 
 }  // namespace
 
-int paged_mma_ctas_per_sm(int64_t head_dim) { return head_dim > 192 ? MmaCfg<256>::CTAS : MmaCfg<128>::CTAS; }
+int paged_mma_ctas_per_sm(int64_t head_dim) {
+  return head_dim <= 64 ? MmaCfg<64>::CTAS : head_dim <= 192 ? MmaCfg<128>::CTAS : MmaCfg<256>::CTAS;
+}
 
 int launch_paged_mma(const PagedArgs& a, int dtype, int ctas, int ranks, int warps, const LaunchCtx& ctx) {
   return dtype == CMPX_BF16 ? launch_dt<CMPX_BF16>(a, ctas, ranks, warps, ctx) : launch_dt<CMPX_F16>(a, ctas, ranks, warps, ctx);
