@@ -174,6 +174,37 @@ def test_scores_that_are_all_minus_infinity_have_no_softmax(cuda_device, dtype, 
     assert torch.isnan(out[some][:, 2:]).all() and torch.isfinite(out[some][:, :2]).all() and (out[1] == 0).all()
 
 
+@pytest.mark.parametrize("D", [40, 64, 96, 128, 160, 192, 256])
+@pytest.mark.parametrize("n", [40, 3000, 9000])
+def test_infinite_values_and_scores_with_many_heads_in_full_precision(cuda_device, D, n):
+    c = Case(torch.float32, 16, 2, D, 16, [n, 30], seed=20)
+    page, row = int(c.table[0, (n - 1) // 16]), (n - 1) % 16
+    c.args[2][page, 0, row, 5] = -float("inf")
+    c.args[0][0, :, 0, 3] = 2.0
+    c.args[1][page, 1, row, 3] = -float("inf")
+    c.q[0, :, 0, 3] = 2.0
+    out = cmpext3.ops.paged_attention(*c.args)[:, :, 0]
+    torch.cuda.synchronize()
+    assert (out[0, :8, 5] == -float("inf")).all()
+    want, bound = O.attention(c.q[0, :8, 0], c.k[0][:1], c.v[0][:1], D ** -0.5)
+    want[:, 5], bound[:, 5] = 0, 1                                            # (seen above)
+    out[0, :8, 5] = 0
+    O.assert_within(out[0, :8], want, bound, "the other columns")
+    want, bound = O.attention(c.q[0, 8:, 0], c.k[0][1:, :n - 1], c.v[0][1:, :n - 1], D ** -0.5)
+    O.assert_within(out[0, 8:], want, bound, "a key with a score of -inf")
+    want, bound = O.attention(c.q[1, :, 0], c.k[1], c.v[1], D ** -0.5)
+    O.assert_within(out[1], want, bound, "the other sequence")
+    c.args[1][page, 0, row, 0] = float("nan")
+    out = cmpext3.ops.paged_attention(*c.args)[:, :, 0]
+    assert torch.isnan(out[0, :8]).all() and torch.isfinite(out[0, 8:]).all() and torch.isfinite(out[1]).all()
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(8, 1, 40), (5, 1, 64), (16, 2, 64), (12, 2, 96), (24, 3, 128), (6, 1, 160), (14, 2, 192)])
+@pytest.mark.parametrize("lengths", [list(range(0, 70)), [600] * 300, [9500, 3, 0], [4096] * 3])
+def test_many_heads_in_full_precision(cuda_device, H, Hkv, D, lengths):
+    Case(torch.float32, H, Hkv, D, 24, lengths, seed=H + D, fill=float("nan")).check()
+
+
 def test_nan_and_infinite_keys_spread_to_their_sequence_alone(cuda_device):
     c = Case(torch.bfloat16, 4, 2, 64, 16, [40, 700, 30], seed=8)
     c.args[1][int(c.table[1, 20]), 0, 3] = float("nan")

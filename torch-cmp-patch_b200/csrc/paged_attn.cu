@@ -1,5 +1,5 @@
 // paged_attn.cu -- attention of one new token per sequence over a paged key-value cache, B200 sm_100a:
-// the choice of schedule and the join (the kernels over the keys: paged_attn_mma.cu, paged_attn_f32.cu).
+// the choice of schedule and the join (the kernels over the keys: paged_attn_mma.cu, paged_attn_f32.cu, paged_attn_f32_mma.cu).
 //
 //   o[b, h] = sum_t p_t V[t] / sum_t p_t,   p_t = exp(q[b, h] . K[t] * scale - m),  t < lengths[b],
 // with the maximum m and both sums carried along (one pass over the keys).
@@ -151,11 +151,19 @@ __global__ void __launch_bounds__(32 * W) paged_join_kernel(const __grid_constan
 // host
 // ---------------------------------------------------------------------------------------------
 
+// fp32 on the tensor cores: from five heads per item on, where the FMA units bound the other kernel ([8, 32/4, 128],
+// 6103 keys: 42 us, 53 there; four heads: 42 and 35), and from two where that kernel pads the heads to 128 and this
+// one to 96 ([8, 16/4, 80], 9765 keys: 42 and 48).  Above 192 the queries do not fit its registers.
+bool f32_mma(int item_heads, int64_t head_dim) {
+  return item_heads > 4 ? head_dim <= 192 : item_heads > 1 && head_dim > 64 && head_dim <= 96;
+}
+
 struct Schedule {
   int item_heads, items_per_head;
   int64_t items;
   int ranks;        // CTAs per whole item, 0: equal shares and a join
-  int ctas, warps;  // warps per CTA
+  int ctas;
+  bool wide;        // a CTA of a whole item has an SM to itself
   int64_t workers;  // warps with shares
 };
 
@@ -173,11 +181,14 @@ Schedule schedule(const cmpx_paged_attn_desc* d, int num_sms) {
   s.item_heads = static_cast<int>((group + s.items_per_head - 1) / s.items_per_head);
   s.items = d->batch * d->cache.heads_kv * s.items_per_head;
   const int64_t keys = d->cache.table_width * d->cache.page_size;  // of the longest sequence there can be
-  const int per_sm = f32 ? paged_f32_ctas_per_sm() : paged_mma_ctas_per_sm(d->cache.head_dim);
+  const PagedShape shape = !f32                                         ? paged_mma_shape(d->cache.head_dim)
+                           : f32_mma(s.item_heads, d->cache.head_dim) ? paged_f32_mma_shape(d->cache.head_dim)
+                                                                      : paged_f32_shape();
+  const int per_sm = shape.ctas;
   const int64_t slots = static_cast<int64_t>(num_sms) * per_sm;
   // Whole items, by one CTA or a cluster of 2, 4 or 8 (256 keys each): one launch and no join.  The CTAs have to
   // fit on the GPU at once, and a cluster's into one GPC: 7/8 of the places can be counted on, 3/4 where a cluster
-  // takes 8 SMs.  Where they are few, each has an SM to itself and twice the warps, for the loads in
+  // takes 8 SMs.  Where they are few, each has an SM to itself and all its warps, for the loads in
   // flight ([1, 32/8, 128] bf16, 4096 keys: 10.5 us; equal shares and a join 13.5).  Of many, that lengths differ
   // costs less than the join does ([100, 16/4, 64] fp16, 900 keys: 19.4 us; equal shares 23.4; [64, 32/8, 64], 10 to
   // 1000 keys: 15.4 and 14.3).
@@ -187,13 +198,12 @@ Schedule schedule(const cmpx_paged_attn_desc* d, int num_sms) {
   if (keys <= kWholeKeys || (keys <= kClusterKeys * ranks && fits(ranks))) {
     s.ranks = ranks;
     s.ctas = static_cast<int>(s.items * ranks);
-    s.warps = per_sm > 1 && s.ctas <= num_sms * 3 / 4 ? kPagedWideWarps : kPagedWarps;
+    s.wide = per_sm > 1 && s.ctas <= num_sms * 3 / 4;
     return s;
   }
-  s.warps = kPagedWarps;
   const int64_t units = s.items * (std::max<int64_t>(1, (keys + kTile - 1) / kTile) + kItemCost);
   s.ctas = static_cast<int>(std::max<int64_t>(1, std::min(slots, (units + kShareMin - 1) / kShareMin)));
-  s.workers = static_cast<int64_t>(s.ctas) * kPagedWarps;
+  s.workers = static_cast<int64_t>(s.ctas) * shape.warps;
   return s;
 }
 
@@ -303,8 +313,9 @@ int launch_paged_attn(const cmpx_paged_attn_desc* d, const LaunchCtx& ctx) {
     a.part_o = static_cast<float*>(d->workspace);
     a.part_ml = a.part_o + 2ull * s.workers * s.item_heads * c.head_dim;
   }
-  const int st = d->dtype == CMPX_F32 ? launch_paged_f32(a, s.ctas, s.ranks, s.warps, ctx)
-                                      : launch_paged_mma(a, d->dtype, s.ctas, s.ranks, s.warps, ctx);
+  const int st = d->dtype != CMPX_F32                    ? launch_paged_mma(a, d->dtype, s.ctas, s.ranks, s.wide, ctx)
+                 : f32_mma(s.item_heads, c.head_dim) ? launch_paged_f32_mma(a, s.ctas, s.ranks, s.wide, ctx)
+                                                     : launch_paged_f32(a, s.ctas, s.ranks, s.wide, ctx);
   if (st != CMPX_OK || s.ranks) return st;
   // The most partial results that a row can have: the longest sequence beside empty ones.
   const int64_t tiles = (static_cast<int64_t>(a.capacity) + kTile - 1) / kTile;

@@ -5,7 +5,7 @@
 // lanes share a key, each with two vectors of 4 values of its row; a lane group runs its own online
 // softmax over its keys for up to HG heads, so a key and a value are read from memory once for 8 heads and
 // from shared memory once for all of them.  At one head per key head the stream bounds it, at eight the
-// FMA units (about 40 instructions per key, head and lane group).
+// FMA units (about 40 instructions per key, head and lane group), where paged_attn_f32_mma.cu takes over.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -17,7 +17,7 @@
 namespace cmpx {
 namespace {
 
-constexpr int kCtasPerSm = 2;
+constexpr int kCtasPerSm = 2, kCtaWarps = 4;
 
 template <int DP>
 struct F32Cfg {
@@ -27,11 +27,11 @@ struct F32Cfg {
   static constexpr int KEYS = GROUPS * STEPS;  // per buffer: 8 KB of keys and values
   static constexpr int ROW = DP * 4;
   static constexpr int STAGES = 3;
-  using Pipe = KeyPipe<ROW, KEYS, STAGES, false>;
+  using Pipe = KeyPipe<ROW, KEYS, STAGES, 0>;
 };
 
 template <int DP, int HG, bool WHOLE, int kWarps>
-__global__ void __launch_bounds__(32 * kWarps, kWarps == kPagedWarps ? kCtasPerSm : 1) paged_attn_f32_kernel(const __grid_constant__ PagedArgs a) {
+__global__ void __launch_bounds__(32 * kWarps, kWarps == kCtaWarps ? kCtasPerSm : 1) paged_attn_f32_kernel(const __grid_constant__ PagedArgs a) {
   using C = F32Cfg<DP>;
   constexpr int LPT = C::LPT, STEPS = C::STEPS;
   static_assert(C::Pipe::BYTES >= HG * DP * 4, "the warps' outputs are joined in the buffers");
@@ -212,27 +212,27 @@ int launch(const PagedArgs& a, int ctas, int ranks, const LaunchCtx& ctx) {
 }
 
 template <int DP, int HG>
-int launch_as(const PagedArgs& a, int ctas, int ranks, int warps, const LaunchCtx& ctx) {
-  if (ranks == 0) return launch<DP, HG, false, kPagedWarps>(a, ctas, ranks, ctx);
-  return warps == kPagedWideWarps ? launch<DP, HG, true, kPagedWideWarps>(a, ctas, ranks, ctx)
-                                  : launch<DP, HG, true, kPagedWarps>(a, ctas, ranks, ctx);
+int launch_as(const PagedArgs& a, int ctas, int ranks, bool wide, const LaunchCtx& ctx) {
+  if (ranks == 0) return launch<DP, HG, false, kCtaWarps>(a, ctas, ranks, ctx);
+  return wide ? launch<DP, HG, true, kCtaWarps * kCtasPerSm>(a, ctas, ranks, ctx)
+              : launch<DP, HG, true, kCtaWarps>(a, ctas, ranks, ctx);
 }
 
 template <int DP>
-int launch_heads(const PagedArgs& a, int ctas, int ranks, int warps, const LaunchCtx& ctx) {
-  if (a.item_heads == 1) return launch_as<DP, 1>(a, ctas, ranks, warps, ctx);
-  if (a.item_heads <= 4) return launch_as<DP, 4>(a, ctas, ranks, warps, ctx);
-  return launch_as<DP, 8>(a, ctas, ranks, warps, ctx);
+int launch_heads(const PagedArgs& a, int ctas, int ranks, bool wide, const LaunchCtx& ctx) {
+  if (a.item_heads == 1) return launch_as<DP, 1>(a, ctas, ranks, wide, ctx);
+  if (a.item_heads <= 4) return launch_as<DP, 4>(a, ctas, ranks, wide, ctx);
+  return launch_as<DP, 8>(a, ctas, ranks, wide, ctx);
 }
 
 }  // namespace
 
-int paged_f32_ctas_per_sm() { return kCtasPerSm; }
+PagedShape paged_f32_shape() { return PagedShape{kCtasPerSm, kCtaWarps}; }
 
-int launch_paged_f32(const PagedArgs& a, int ctas, int ranks, int warps, const LaunchCtx& ctx) {
-  if (a.head_dim <= 64) return launch_heads<64>(a, ctas, ranks, warps, ctx);
-  if (a.head_dim <= 128) return launch_heads<128>(a, ctas, ranks, warps, ctx);
-  return launch_heads<256>(a, ctas, ranks, warps, ctx);
+int launch_paged_f32(const PagedArgs& a, int ctas, int ranks, bool wide, const LaunchCtx& ctx) {
+  if (a.head_dim <= 64) return launch_heads<64>(a, ctas, ranks, wide, ctx);
+  if (a.head_dim <= 128) return launch_heads<128>(a, ctas, ranks, wide, ctx);
+  return launch_heads<256>(a, ctas, ranks, wide, ctx);
 }
 
 }  // namespace cmpx

@@ -30,6 +30,7 @@ namespace cmpx {
 namespace {
 
 constexpr int kKeys = 16;  // keys per buffer
+constexpr int kCtaWarps = 4;
 
 template <int DP>
 struct MmaCfg {
@@ -39,7 +40,7 @@ struct MmaCfg {
   // fewer buffers each serve better ([8, 16 heads, 4 key heads, 40] fp16 with 39062 keys: 51 us, 59 with two CTAs
   // and six stages); at 128 they do not (3 CTAs and two stages: 39.7 us for 12207 keys, 38.8 so).
   static constexpr int CTAS = DP == 64 ? 4 : DP == 256 ? 1 : 2;
-  using Pipe = KeyPipe<ROW, kKeys, STAGES, true>;
+  using Pipe = KeyPipe<ROW, kKeys, STAGES, 1>;
   static_assert(Pipe::BYTES >= 16 * DP * 4, "the warps' outputs are joined in the buffers");
 };
 
@@ -88,7 +89,7 @@ __device__ __forceinline__ uint32_t cut2(float lo, float hi) {
 }
 
 template <int DT, int DP, bool WHOLE, int kWarps>
-__global__ void __launch_bounds__(32 * kWarps, kWarps == kPagedWarps ? MmaCfg<DP>::CTAS : 1) paged_attn_mma_kernel(const __grid_constant__ PagedArgs a) {
+__global__ void __launch_bounds__(32 * kWarps, kWarps == kCtaWarps ? MmaCfg<DP>::CTAS : 1) paged_attn_mma_kernel(const __grid_constant__ PagedArgs a) {
   using C = MmaCfg<DP>;
   constexpr float kBias = DT == CMPX_F16 ? 14.f : 0.f;
   constexpr float kLeast = DT == CMPX_F16 ? 0x1p-24f : 0x1p-126f;  // the types' smallest (normal) values
@@ -280,29 +281,29 @@ int launch(const PagedArgs& a, int ctas, int ranks, const LaunchCtx& ctx) {
 }
 
 template <int DT, int DP>
-int launch_as(const PagedArgs& a, int ctas, int ranks, int warps, const LaunchCtx& ctx) {
-  if (ranks == 0) return launch<DT, DP, false, kPagedWarps>(a, ctas, ranks, ctx);
+int launch_as(const PagedArgs& a, int ctas, int ranks, bool wide, const LaunchCtx& ctx) {
+  if (ranks == 0) return launch<DT, DP, false, kCtaWarps>(a, ctas, ranks, ctx);
   if constexpr (MmaCfg<DP>::CTAS > 1)
-    if (warps == kPagedWideWarps) return launch<DT, DP, true, kPagedWideWarps>(a, ctas, ranks, ctx);
-  return launch<DT, DP, true, kPagedWarps>(a, ctas, ranks, ctx);
+    if (wide) return launch<DT, DP, true, 2 * kCtaWarps>(a, ctas, ranks, ctx);
+  return launch<DT, DP, true, kCtaWarps>(a, ctas, ranks, ctx);
 }
 
 template <int DT>
-int launch_dt(const PagedArgs& a, int ctas, int ranks, int warps, const LaunchCtx& ctx) {
-  if (a.head_dim <= 64) return launch_as<DT, 64>(a, ctas, ranks, warps, ctx);
-  if (a.head_dim <= 128) return launch_as<DT, 128>(a, ctas, ranks, warps, ctx);
-  if (a.head_dim <= 192) return launch_as<DT, 192>(a, ctas, ranks, warps, ctx);
-  return launch_as<DT, 256>(a, ctas, ranks, warps, ctx);
+int launch_dt(const PagedArgs& a, int ctas, int ranks, bool wide, const LaunchCtx& ctx) {
+  if (a.head_dim <= 64) return launch_as<DT, 64>(a, ctas, ranks, wide, ctx);
+  if (a.head_dim <= 128) return launch_as<DT, 128>(a, ctas, ranks, wide, ctx);
+  if (a.head_dim <= 192) return launch_as<DT, 192>(a, ctas, ranks, wide, ctx);
+  return launch_as<DT, 256>(a, ctas, ranks, wide, ctx);
 }
 
 }  // namespace
 
-int paged_mma_ctas_per_sm(int64_t head_dim) {
-  return head_dim <= 64 ? MmaCfg<64>::CTAS : head_dim <= 192 ? MmaCfg<128>::CTAS : MmaCfg<256>::CTAS;
+PagedShape paged_mma_shape(int64_t head_dim) {
+  return PagedShape{head_dim <= 64 ? MmaCfg<64>::CTAS : head_dim <= 192 ? MmaCfg<128>::CTAS : MmaCfg<256>::CTAS, kCtaWarps};
 }
 
-int launch_paged_mma(const PagedArgs& a, int dtype, int ctas, int ranks, int warps, const LaunchCtx& ctx) {
-  return dtype == CMPX_BF16 ? launch_dt<CMPX_BF16>(a, ctas, ranks, warps, ctx) : launch_dt<CMPX_F16>(a, ctas, ranks, warps, ctx);
+int launch_paged_mma(const PagedArgs& a, int dtype, int ctas, int ranks, bool wide, const LaunchCtx& ctx) {
+  return dtype == CMPX_BF16 ? launch_dt<CMPX_BF16>(a, ctas, ranks, wide, ctx) : launch_dt<CMPX_F16>(a, ctas, ranks, wide, ctx);
 }
 
 }  // namespace cmpx

@@ -201,13 +201,19 @@ __device__ __forceinline__ Stretch whole_item(const PagedArgs& a, int64_t index,
 
 // A warp's pipeline over the keys of a stretch: STAGES buffers of KEYS keys and values in shared memory,
 // ROW bytes each, filled by 16-byte cp.async.  The rows are found through the page table one by one (a page may
-// end inside a buffer).  With SWIZZLE the 16-byte chunks of row r lie at chunk ^ (r % 8).  Keys behind
+// end inside a buffer).  Chunk c (16 bytes) of row r lies at c ^ turn_of(r).  SWIZZLE 1, for ldmatrix: 8 rows' chunks
+// of one column lie in different banks.  2, for a lane's own 16-byte loads: so do 4 neighbouring chunks of rows 2 i and
+// 2 i + 1, and 2 neighbouring chunks of 4 rows of one parity.  Keys behind
 // the stretch, pages that do not exist and columns behind head_dim are filled with zeros.
-template <int ROW, int KEYS, int STAGES, bool SWIZZLE>
+template <int ROW, int KEYS, int STAGES, int SWIZZLE>
 struct KeyPipe {
   static constexpr int CHUNKS = ROW / 16;
   static constexpr int STAGE = 2 * KEYS * ROW;
   static constexpr int BYTES = STAGES * STAGE;  // per warp
+
+  static __device__ __forceinline__ int turn_of(int r) {
+    return SWIZZLE == 0 ? 0 : SWIZZLE == 1 ? r & 7 : (r & 2) | (((r >> 2) ^ r) & 1) << 2;
+  }
 
   const PagedArgs& a;
   const int32_t* table;
@@ -261,7 +267,7 @@ struct KeyPipe {
         for (int j = 0; j < KEYS * CHUNKS / 32; ++j) {
           const int idx = j * 32 + lane, r = idx / CHUNKS, ch = idx % CHUNKS;
           const int bytes = ch < row_chunks ? 16 : 0;
-          const uint32_t dst = base + r * ROW + ((SWIZZLE ? ch ^ (r & 7) : ch) << 4);
+          const uint32_t dst = base + r * ROW + ((ch ^ turn_of(r)) << 4);
           cp_async16(dst, kp + r * a.kc_st + (bytes ? ch * 16 : 0), bytes);
           cp_async16(dst + KEYS * ROW, vp + r * a.vc_st + (bytes ? ch * 16 : 0), bytes);
         }
@@ -273,7 +279,7 @@ struct KeyPipe {
           const int idx = j * 32 + lane, r = idx / CHUNKS, ch = idx % CHUNKS;
           const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
           const bool there = kr >= 0 && ch < row_chunks;
-          const uint32_t dst = base + r * ROW + ((SWIZZLE ? ch ^ (r & 7) : ch) << 4);
+          const uint32_t dst = base + r * ROW + ((ch ^ turn_of(r)) << 4);
           cp_async16(dst, there ? kb + kr + ch * 16 : a.q, there ? 16 : 0);
           cp_async16(dst + KEYS * ROW, there ? vb + vr + ch * 16 : a.q, there ? 16 : 0);
         }
@@ -368,13 +374,17 @@ int launch_whole(Kernel kernel, const PagedArgs& a, int64_t ctas, int ranks, int
 }
 
 // The kernels over the keys: fp16 / bf16 items of up to 16 heads (paged_attn_mma.cu), fp32 items of up to 8
-// (paged_attn_f32.cu).  ranks: CTAs per whole item, 0 for equal shares; warps: 4 per CTA, or 8 (whole items, one
-// CTA per SM; not for 16-bit heads above 192, whose buffers take the SM with 4).
-constexpr int kPagedWarps = 4, kPagedWideWarps = 8;
-int paged_mma_ctas_per_sm(int64_t head_dim);
-int paged_f32_ctas_per_sm();
-int launch_paged_mma(const PagedArgs& a, int dtype, int ctas, int ranks, int warps, const LaunchCtx& ctx);
-int launch_paged_f32(const PagedArgs& a, int ctas, int ranks, int warps, const LaunchCtx& ctx);
+// (paged_attn_f32.cu, paged_attn_f32_mma.cu).  ranks: CTAs per whole item, 0 for equal shares; wide: whole items whose
+// CTAs have an SM each to themselves, with the warps of all that would share it.
+struct PagedShape {
+  int ctas, warps;  // CTAs per SM, warps per CTA
+};
+PagedShape paged_mma_shape(int64_t head_dim);
+PagedShape paged_f32_shape();
+PagedShape paged_f32_mma_shape(int64_t head_dim);
+int launch_paged_mma(const PagedArgs& a, int dtype, int ctas, int ranks, bool wide, const LaunchCtx& ctx);
+int launch_paged_f32(const PagedArgs& a, int ctas, int ranks, bool wide, const LaunchCtx& ctx);
+int launch_paged_f32_mma(const PagedArgs& a, int ctas, int ranks, bool wide, const LaunchCtx& ctx);
 
 // Programmatic dependent launch: the join kernel starts while the main kernel runs, reads the
 // lengths, and waits here for the main kernel's results.
