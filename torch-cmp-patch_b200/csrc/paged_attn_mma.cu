@@ -11,8 +11,8 @@
 //     warps, which met at the end of each item, [32, 32 heads, 8 key heads, 128] bf16 with 64 to 8192 keys took 81 us);
 //   * WHOLE (short caches): a CTA, or a cluster of up to 8, takes an item; the warps share its keys, meet once
 //     and join their results through (distributed) shared memory, without a second kernel;
-//   * rows of a buffer are swizzled in 16-byte chunks (chunk ^ row % 8): ldmatrix reads without bank
-//     conflicts, and nothing is padded.
+//   * rows of a buffer are swizzled in 16-byte chunks: ldmatrix reads without bank conflicts, and nothing is
+//     padded.
 // P is used as the sum of two 16-bit parts (cut off, and the rounded rest), so the weights carry 16 bits
 // and more; a second product of P V costs nothing here, and one part alone would add as much error as the
 // output's rounding does.  The rest is kept above zero, so that an infinite value stays infinite (0 * inf is
@@ -36,10 +36,11 @@ template <int DP>
 struct MmaCfg {
   static constexpr int ROW = DP * 2;                     // bytes of a row
   static constexpr int STAGES = DP == 192 ? 2 : 3;
-  // Per SM: 192 KB of buffers in all.  At 64, where a tile is 4 KB and its products' latency counts, more warps with
+  // Per SM: 192 to 216 KB of buffers in all.  At 64, where a tile is 4 KB and its products' latency counts, more warps with
   // fewer buffers each serve better ([8, 16 heads, 4 key heads, 40] fp16 with 39062 keys: 51 us, 59 with two CTAs
-  // and six stages); at 128 they do not (3 CTAs and two stages: 39.7 us for 12207 keys, 38.8 so).
-  static constexpr int CTAS = DP == 64 ? 4 : DP == 256 ? 1 : 2;
+  // and six stages); at 96 they do a little (80 in tiles of 128: 44.9 us for 19531 keys, of 96 with two CTAs and with
+  // three 41.3; 300 keys of 32 sequences 9.0 and 8.1), at 128 not (39.7 us for 12207 keys; with two CTAs 38.8).
+  static constexpr int CTAS = DP == 64 ? 4 : DP == 96 ? 3 : DP == 256 ? 1 : 2;
   using Pipe = KeyPipe<ROW, kKeys, STAGES, 1>;
   static_assert(Pipe::BYTES >= 16 * DP * 4, "the warps' outputs are joined in the buffers");
 };
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == kCtaWarps ? MmaCfg<DP>:
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks) {
         uint32_t b[4];
-        ldmatrix4<false>(kbuf + k_row * C::ROW + (((2 * ks + k_chunk) ^ (k_row & 7)) << 4), b);
+        ldmatrix4<false>(kbuf + k_row * C::ROW + (((2 * ks + k_chunk) ^ C::Pipe::turn_of(k_row)) << 4), b);
         mma16816<DT>(ks & 1 ? s2[0] : s[0], q[ks], b[0], b[1]);
         mma16816<DT>(ks & 1 ? s2[1] : s[1], q[ks], b[2], b[3]);
       }
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == kCtaWarps ? MmaCfg<DP>:
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i) {
         uint32_t b[4];
-        ldmatrix4<true>(vbuf + v_row * C::ROW + (((2 * i + v_chunk) ^ (v_row & 7)) << 4), b);
+        ldmatrix4<true>(vbuf + v_row * C::ROW + (((2 * i + v_chunk) ^ C::Pipe::turn_of(v_row)) << 4), b);
         mma16816<DT>(o[2 * i], hi, b[0], b[1]);
         mma16816<DT>(o[2 * i + 1], hi, b[2], b[3]);
         mma16816<DT>(o[2 * i], lo, b[0], b[1]);
@@ -291,6 +292,7 @@ int launch_as(const PagedArgs& a, int ctas, int ranks, bool wide, const LaunchCt
 template <int DT>
 int launch_dt(const PagedArgs& a, int ctas, int ranks, bool wide, const LaunchCtx& ctx) {
   if (a.head_dim <= 64) return launch_as<DT, 64>(a, ctas, ranks, wide, ctx);
+  if (a.head_dim <= 96) return launch_as<DT, 96>(a, ctas, ranks, wide, ctx);
   if (a.head_dim <= 128) return launch_as<DT, 128>(a, ctas, ranks, wide, ctx);
   if (a.head_dim <= 192) return launch_as<DT, 192>(a, ctas, ranks, wide, ctx);
   return launch_as<DT, 256>(a, ctas, ranks, wide, ctx);
@@ -299,7 +301,11 @@ int launch_dt(const PagedArgs& a, int ctas, int ranks, bool wide, const LaunchCt
 }  // namespace
 
 PagedShape paged_mma_shape(int64_t head_dim) {
-  return PagedShape{head_dim <= 64 ? MmaCfg<64>::CTAS : head_dim <= 192 ? MmaCfg<128>::CTAS : MmaCfg<256>::CTAS, kCtaWarps};
+  const int ctas = head_dim <= 64    ? MmaCfg<64>::CTAS
+                   : head_dim <= 96  ? MmaCfg<96>::CTAS
+                   : head_dim <= 192 ? MmaCfg<128>::CTAS
+                                     : MmaCfg<256>::CTAS;
+  return PagedShape{ctas, kCtaWarps};
 }
 
 int launch_paged_mma(const PagedArgs& a, int dtype, int ctas, int ranks, bool wide, const LaunchCtx& ctx) {

@@ -212,7 +212,8 @@ struct KeyPipe {
   static constexpr int BYTES = STAGES * STAGE;  // per warp
 
   static __device__ __forceinline__ int turn_of(int r) {
-    return SWIZZLE == 0 ? 0 : SWIZZLE == 1 ? r & 7 : (r & 2) | (((r >> 2) ^ r) & 1) << 2;
+    if (SWIZZLE == 1) return ROW % 128 == 0 ? r & 7 : (r >> 1) & 3;  // (64 bytes over: odd rows begin 4 chunks on)
+    return SWIZZLE == 0 ? 0 : (r & 2) | (((r >> 2) ^ r) & 1) << 2;
   }
 
   const PagedArgs& a;
