@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(32 * W) paged_join_kernel(const __grid_constan
 // ---------------------------------------------------------------------------------------------
 
 // fp32 on the tensor cores: from five heads per item on, where the FMA units bound the other kernel ([8, 32/4, 128],
-// 6103 keys: 42 us, 53 there; four heads: 42 and 35), and from two where that kernel pads the heads to 128 and this
+// 6103 keys: 37 us, 53 there; with four heads the other takes 35), and from two where that kernel pads the heads to 128 and this
 // one to 96 ([8, 16/4, 80], 9765 keys: 42 and 48).  Above 192 the queries do not fit its registers.
 bool f32_mma(int item_heads, int64_t head_dim) {
   return item_heads > 4 ? head_dim <= 192 : item_heads > 1 && head_dim > 64 && head_dim <= 96;
@@ -187,12 +187,12 @@ Schedule schedule(const cmpx_paged_attn_desc* d, int num_sms) {
   const int per_sm = shape.ctas;
   const int64_t slots = static_cast<int64_t>(num_sms) * per_sm;
   // Whole items, by one CTA or a cluster of 2, 4 or 8 (256 keys each): one launch and no join.  The CTAs have to
-  // fit on the GPU at once, and a cluster's into one GPC: 7/8 of the places can be counted on, 3/4 where a cluster
-  // takes 8 SMs.  Where they are few, each has an SM to itself and all its warps, for the loads in
-  // flight ([1, 32/8, 128] bf16, 4096 keys: 10.5 us; equal shares and a join 13.5).  Of many, that lengths differ
+  // fit on the GPU at once, and a cluster's into one GPC: 7/8 of the places can be counted on.
+  // Where they are few, each has an SM to itself and all its warps, for the loads in flight
+  // ([1, 32/8, 128] bf16, 4096 keys: 10.5 us; equal shares and a join 13.5).  Of many, that lengths differ
   // costs less than the join does ([100, 16/4, 64] fp16, 900 keys: 19.4 us; equal shares 23.4; [64, 32/8, 64], 10 to
   // 1000 keys: 15.4 and 14.3).
-  auto fits = [&](int ranks) { return s.items * ranks * 8 <= slots * (per_sm == 1 && ranks == 8 ? 6 : 7); };
+  auto fits = [&](int ranks) { return s.items * ranks * 8 <= slots * 7; };
   int ranks = 1;
   while (ranks < 8 && keys > 256 * ranks && fits(2 * ranks)) ranks *= 2;
   if (keys <= kWholeKeys || (keys <= kClusterKeys * ranks && fits(ranks))) {

@@ -26,8 +26,8 @@ struct F32Cfg {
   static constexpr int STEPS = 4;
   static constexpr int KEYS = GROUPS * STEPS;  // per buffer: 8 KB of keys and values
   static constexpr int ROW = DP * 4;
-  static constexpr int STAGES = 3;
-  using Pipe = KeyPipe<ROW, KEYS, STAGES, 0>;
+  static constexpr int SLOTS = 3;
+  using Pipe = KeyPipe<ROW, KEYS, SLOTS, 0>;
 };
 
 template <int DP, int HG, bool WHOLE, int kWarps>
@@ -59,9 +59,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == kCtaWarps ? kCtasPerSm 
   const int col[2] = {4 * sub, 4 * (sub + LPT)};
 
   while (more) {
-    const int count = pipe.begin(st, first);
-#pragma unroll
-    for (int i = 0; i < C::STAGES - 1; ++i) pipe.issue(first + i * kStep, kStep, count, i);
+    pipe.begin(st, first, kStep);
     float q[HG][8], o[HG][8], m[HG], l[HG];
 #pragma unroll
     for (int h = 0; h < HG; ++h) {
@@ -80,13 +78,8 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == kCtaWarps ? kCtasPerSm 
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[h][e] = 0.f;
     }
-    int stage = 0;
-    for (int at = first; at < count; at += kStep) {
-      cp_async_wait<C::STAGES - 2>();
-      __syncwarp();  // this buffer is filled, and everybody is done with the one before it
-      pipe.issue(at + (C::STAGES - 1) * kStep, kStep, count, stage == 0 ? C::STAGES - 1 : stage - 1);
-      const uint8_t* const kbuf = buffers + stage * C::Pipe::STAGE;
-      stage = stage + 1 == C::STAGES ? 0 : stage + 1;
+    for (int at = first; at < pipe.count; at += kStep) {
+      const uint8_t* const kbuf = buffers + pipe.template take<true>();
       const int left = st.key1 - st.key0 - at * C::KEYS;  // keys of this buffer
 
       float s[STEPS][HG];
@@ -125,9 +118,10 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == kCtaWarps ? kCtasPerSm 
           l[h] += s[u][h];
         }
       }
+      const uint8_t* const vbuf = buffers + pipe.template take<false>();
 #pragma unroll
       for (int u = 0; u < STEPS; ++u) {
-        const uint8_t* const row = kbuf + (C::KEYS + u * C::GROUPS + group) * C::ROW;
+        const uint8_t* const row = vbuf + (u * C::GROUPS + group) * C::ROW;
         const float4 v0 = *reinterpret_cast<const float4*>(row + col[0] * 4);
         const float4 v1 = *reinterpret_cast<const float4*>(row + col[1] * 4);
         const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};

@@ -12,7 +12,7 @@
 // with infinities (whose rest would be NaN) in mind.
 // What bounds it: the two or three warps that a scheduler has, whose registers and buffers leave no more, wait for their
 // own products and shuffles (issue slots 46% used, tensor cores 26% at 64).  [8, 32 heads, 4 key heads] over
-// 200 MB: 52 us at 40, 42 at 64, 43 at 80, 38 at 96, 43 at 128, 51 at 160, 50 at 192 (FMA units: 74, 52, 75, 67,
+// 200 MB: 52 us at 40, 42 at 64, 43 at 80, 38 at 96, 37 at 128, 51 at 160, 50 at 192 (FMA units: 74, 52, 75, 67,
 // 53, 84, 71); at 256 the queries do not fit the registers.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -34,10 +34,10 @@ struct PartsCfg {
   // would leave four warps per SM (192: 80 us instead of 50).
   static constexpr int KEYS = DP <= 128 ? 16 : 8;
   static constexpr int ROW = DP * 4;                       // bytes of a row
-  static constexpr int STAGES = 2;
+  static constexpr int SLOTS = DP == 128 ? 3 : 2;
   static constexpr int CTAS = DP == 64 ? 3 : 2;           // per SM
-  static constexpr int WARPS = DP == 128 ? 3 : 4;         // per CTA
-  using Pipe = KeyPipe<ROW, KEYS, STAGES, 2>;
+  static constexpr int WARPS = 4;         // per CTA
+  using Pipe = KeyPipe<ROW, KEYS, SLOTS, 2, DP == 128>;
   static_assert(Pipe::BYTES >= kHeads * DP * 4, "the warps' outputs are joined in the buffers");
 };
 
@@ -120,9 +120,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == PartsCfg<DP>::WARPS ? P
     float o[DP / 16][4], m[2], l[2];  // m and l of heads 2 tq and 2 tq + 1; l of this lane's keys
     auto walk = [&](auto inf) {       // inf: values may be infinite
       constexpr bool INF = decltype(inf)::value;
-      const int count = pipe.begin(st, first);
-#pragma unroll
-      for (int i = 0; i < C::STAGES - 1; ++i) pipe.issue(first + i * kStep, kStep, count, i);
+      pipe.begin(st, first, kStep);
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
@@ -136,14 +134,8 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == PartsCfg<DP>::WARPS ? P
 #pragma unroll
           for (int i = 0; i < 4; ++i) cut_round<INF>(q[s][i], qp[KEEP_Q ? s : 0][i]);
       }
-      int stage = 0;
-      for (int at = first; at < count; at += kStep) {
-        cp_async_wait<C::STAGES - 2>();
-        __syncwarp();  // this buffer is filled, and everybody is done with the one before it
-        pipe.issue(at + (C::STAGES - 1) * kStep, kStep, count, stage == 0 ? C::STAGES - 1 : stage - 1);
-        const uint8_t* const kbuf = buffers + stage * C::Pipe::STAGE;
-        const uint8_t* const vbuf = kbuf + KEYS * C::ROW;
-        stage = stage + 1 == C::STAGES ? 0 : stage + 1;
+      for (int at = first; at < pipe.count; at += kStep) {
+        const uint8_t* const kbuf = buffers + pipe.template take<true>();
 
         // The products of the leading parts in short chains, added up here: a sum inside the tensor core is cut off,
         // not rounded, which over a long chain shows (4096 keys: 1.7e-6 off, like this).
@@ -222,6 +214,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == PartsCfg<DP>::WARPS ? P
           cut_round<INF>(__uint_as_float(__byte_perm(low, up, 0x5410)), w[h][0]);
           cut_round<INF>(__uint_as_float(__byte_perm(low, up, 0x7632)), w[h][1]);
         }
+        const uint8_t* const vbuf = buffers + pipe.template take<false>();
 #pragma unroll
         for (int blk = 0; blk < DP / 32; ++blk) {
           float t[2][4];

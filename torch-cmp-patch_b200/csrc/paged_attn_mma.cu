@@ -5,7 +5,7 @@
 // at a time, K and V fragments straight from shared memory (ldmatrix, transposed for V).  The
 // products are a few percent of what the tensor cores do even in this form; what bounds the kernel is the
 // one read of K and V, so it is built around loads in flight:
-//   * every warp runs its own pipeline of STAGES buffers of 16 keys (KeyPipe, paged_schedule.cuh) and its own
+//   * every warp runs its own pipeline of buffers of 16 keys (KeyPipe, paged_schedule.cuh) and its own
 //     online softmax over its own share of the keys.  Nothing in a share waits for another warp, so one
 //     warp's first loads of an item hide behind the others' stream (with one share for a CTA's four
 //     warps, which met at the end of each item, [32, 32 heads, 8 key heads, 128] bf16 with 64 to 8192 keys took 81 us);
@@ -35,13 +35,13 @@ constexpr int kCtaWarps = 4;
 template <int DP>
 struct MmaCfg {
   static constexpr int ROW = DP * 2;                     // bytes of a row
-  static constexpr int STAGES = DP == 192 ? 2 : 3;
+  static constexpr int SLOTS = DP == 192 ? 2 : 3;
   // Per SM: 192 to 216 KB of buffers in all.  At 64, where a tile is 4 KB and its products' latency counts, more warps with
   // fewer buffers each serve better ([8, 16 heads, 4 key heads, 40] fp16 with 39062 keys: 51 us, 59 with two CTAs
-  // and six stages); at 96 they do a little (80 in tiles of 128: 44.9 us for 19531 keys, of 96 with two CTAs and with
+  // and six slots); at 96 they do a little (80 in tiles of 128: 44.9 us for 19531 keys, of 96 with two CTAs and with
   // three 41.3; 300 keys of 32 sequences 9.0 and 8.1), at 128 not (39.7 us for 12207 keys; with two CTAs 38.8).
-  static constexpr int CTAS = DP == 64 ? 4 : DP == 96 ? 3 : DP == 256 ? 1 : 2;
-  using Pipe = KeyPipe<ROW, kKeys, STAGES, 1>;
+  static constexpr int CTAS = DP == 64 ? 4 : DP == 96 ? 3 : 2;
+  using Pipe = KeyPipe<ROW, kKeys, SLOTS, 1, DP == 256>;
   static_assert(Pipe::BYTES >= 16 * DP * 4, "the warps' outputs are joined in the buffers");
 };
 
@@ -120,9 +120,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == kCtaWarps ? MmaCfg<DP>:
   const int v_row = (lane & 7) + (((lane >> 3) & 1) << 3), v_chunk = lane >> 4;
 
   while (more) {
-    const int subs = pipe.begin(st, first);
-#pragma unroll
-    for (int i = 0; i < C::STAGES - 1; ++i) pipe.issue(first + i * kStep, kStep, subs, i);
+    pipe.begin(st, first, kStep);
     uint32_t q[DP / 16][4];
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s)
@@ -139,13 +137,8 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == kCtaWarps ? MmaCfg<DP>:
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    int stage = 0;
-    for (int sub = first; sub < subs; sub += kStep) {
-      cp_async_wait<C::STAGES - 2>();
-      __syncwarp();  // this buffer is filled, and everybody is done with the one before it
-      pipe.issue(sub + (C::STAGES - 1) * kStep, kStep, subs, stage == 0 ? C::STAGES - 1 : stage - 1);
-      const uint32_t kbuf = pipe.buf + stage * C::Pipe::STAGE, vbuf = kbuf + kKeys * C::ROW;
-      stage = stage + 1 == C::STAGES ? 0 : stage + 1;
+    for (int sub = first; sub < pipe.count; sub += kStep) {
+      const uint32_t kbuf = pipe.buf + pipe.template take<true>();
 
       // two chains of products for each 8 keys
       float s[2][4], s2[2][4];
@@ -201,6 +194,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == kCtaWarps ? MmaCfg<DP>:
           lo[2 * n + r] = pack2<DT>(fmaxf(p0 - h0, kLeast), fmaxf(p1 - h1, kLeast));
         }
       }
+      const uint32_t vbuf = pipe.buf + pipe.template take<false>();
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i) {
         uint32_t b[4];
@@ -284,8 +278,7 @@ int launch(const PagedArgs& a, int ctas, int ranks, const LaunchCtx& ctx) {
 template <int DT, int DP>
 int launch_as(const PagedArgs& a, int ctas, int ranks, bool wide, const LaunchCtx& ctx) {
   if (ranks == 0) return launch<DT, DP, false, kCtaWarps>(a, ctas, ranks, ctx);
-  if constexpr (MmaCfg<DP>::CTAS > 1)
-    if (wide) return launch<DT, DP, true, 2 * kCtaWarps>(a, ctas, ranks, ctx);
+  if (wide) return launch<DT, DP, true, 2 * kCtaWarps>(a, ctas, ranks, ctx);
   return launch<DT, DP, true, kCtaWarps>(a, ctas, ranks, ctx);
 }
 
@@ -301,10 +294,7 @@ int launch_dt(const PagedArgs& a, int ctas, int ranks, bool wide, const LaunchCt
 }  // namespace
 
 PagedShape paged_mma_shape(int64_t head_dim) {
-  const int ctas = head_dim <= 64    ? MmaCfg<64>::CTAS
-                   : head_dim <= 96  ? MmaCfg<96>::CTAS
-                   : head_dim <= 192 ? MmaCfg<128>::CTAS
-                                     : MmaCfg<256>::CTAS;
+  const int ctas = head_dim <= 64 ? MmaCfg<64>::CTAS : head_dim <= 96 ? MmaCfg<96>::CTAS : MmaCfg<128>::CTAS;
   return PagedShape{ctas, kCtaWarps};
 }
 

@@ -199,17 +199,20 @@ __device__ __forceinline__ Stretch whole_item(const PagedArgs& a, int64_t index,
   return st;
 }
 
-// A warp's pipeline over the keys of a stretch: STAGES buffers of KEYS keys and values in shared memory,
-// ROW bytes each, filled by 16-byte cp.async.  The rows are found through the page table one by one (a page may
-// end inside a buffer).  Chunk c (16 bytes) of row r lies at c ^ turn_of(r).  SWIZZLE 1, for ldmatrix: 8 rows' chunks
-// of one column lie in different banks.  2, for a lane's own 16-byte loads: so do 4 neighbouring chunks of rows 2 i and
-// 2 i + 1, and 2 neighbouring chunks of 4 rows of one parity.  Keys behind
-// the stretch, pages that do not exist and columns behind head_dim are filled with zeros.
-template <int ROW, int KEYS, int STAGES, int SWIZZLE>
+// A warp's pipeline over the keys of a stretch: a ring of SLOTS slots in shared memory with KEYS keys and their values
+// each, ROW bytes a row, filled by 16-byte cp.async.  With HALVES a slot has the keys or the values alone: more
+// instructions, but the ring needs less room for the same loads in flight (fp16 heads of 256, 8 warps per SM
+// instead of 4: 36 us instead of 49 over 200 MB; heads of 128, which have the room, 40 instead of 39).  The rows
+// are found through the page table one by one (a page may end inside a slot).  Chunk c (16 bytes) of row r lies at
+// c ^ turn_of(r).  SWIZZLE 1, for ldmatrix: 8 rows' chunks of one column lie in different banks.  2, for a
+// lane's own 16-byte loads: so do 4 neighbouring chunks of rows 2 i and 2 i + 1, and 2 neighbouring chunks of 4
+// rows of one parity.  Keys behind the stretch, pages that do not exist and columns behind head_dim are filled with zeros.
+template <int ROW, int KEYS, int SLOTS, int SWIZZLE, bool HALVES = false>
 struct KeyPipe {
   static constexpr int CHUNKS = ROW / 16;
-  static constexpr int STAGE = 2 * KEYS * ROW;
-  static constexpr int BYTES = STAGES * STAGE;  // per warp
+  static constexpr int HALF = KEYS * ROW;
+  static constexpr int SLOT = HALVES ? HALF : 2 * HALF;
+  static constexpr int BYTES = SLOTS * SLOT;  // per warp
 
   static __device__ __forceinline__ int turn_of(int r) {
     if (SWIZZLE == 1) return ROW % 128 == 0 ? r & 7 : (r >> 1) & 3;  // (64 bytes over: odd rows begin 4 chunks on)
@@ -221,8 +224,12 @@ struct KeyPipe {
   const uint8_t *kb, *vb;
   int key0, key1, row_chunks;
   uint32_t buf;
-  int id_ahead, row_ahead;  // page and row of this lane's key of the next buffer
-  bool bad;
+  int count, step;          // the stretch's sub-tiles of KEYS keys, and from one of this warp's to its next
+  int next;                 // sub-tile that is loaded next
+  int slot_in, slot_out;    // slots that are filled and read next
+  int id_ahead, row_ahead;  // page and row of this lane's key of the next sub-tile
+  int id, row;              // and of the one that is being loaded
+  bool ok, one_page, bad;   // its page exists; all its keys lie in one page
 
   __device__ __forceinline__ KeyPipe(const PagedArgs& args, uint32_t buffers, int row_bytes)
       : a(args), row_chunks(row_bytes / 16), buf(buffers) {}
@@ -237,31 +244,57 @@ struct KeyPipe {
       id_ahead = __ldg(table + page);
     }
   }
-  // Begins a stretch whose first buffer is `first`; the stretch's count of buffers.
-  __device__ __forceinline__ int begin(const Stretch& st, int first) {
+  // Begins a stretch with this warp's sub-tiles first, first + every, ...: fills all slots but one.
+  __device__ __forceinline__ void begin(const Stretch& st, int first, int every) {
     table = a.table + st.b * a.table_stride;
     kb = a.kc + st.kvh * a.kc_sh;
     vb = a.vc + st.kvh * a.vc_sh;
     key0 = st.key0;
     key1 = st.key1;
     bad = st.bad;
+    count = (key1 - key0 + KEYS - 1) / KEYS;
+    step = every;
+    next = first;
+    slot_in = slot_out = 0;
     look_up(first);
-    return (key1 - key0 + KEYS - 1) / KEYS;
+#pragma unroll
+    for (int j = 0; j < SLOTS - 1; ++j)
+      if (HALVES && j % 2 == 1) load<false, true>();
+      else load<true, !HALVES>();
   }
-  // Starts the loads of buffer i of `count` (nothing behind the last), closes the group, and looks up the
-  // pages of buffer i + step, which is the next one.
-  __device__ __forceinline__ void issue(int i, int step, int count, int stage) {
+  // Waits for the keys (then the values) of a sub-tile, starts the loads that are SLOTS - 1 slots ahead in the place
+  // that was read before, and returns their offset in the warp's buffers.
+  template <bool K>
+  __device__ __forceinline__ int take() {
+    if (!HALVES && !K) return (slot_out == 0 ? SLOTS - 1 : slot_out - 1) * SLOT + HALF;
+    cp_async_wait<SLOTS - 2>();
+    __syncwarp();  // this slot is filled, and everybody is done with the one before it
+    if (HALVES) load<K == (SLOTS % 2 == 1), K != (SLOTS % 2 == 1)>();
+    else load<true, true>();
+    const int at = slot_out * SLOT;
+    slot_out = slot_out + 1 == SLOTS ? 0 : slot_out + 1;
+    return at;
+  }
+  // Starts the loads of the next sub-tile's keys, its values, or both (nothing behind the last); closes the group.
+  template <bool K, bool V>
+  __device__ __forceinline__ void load() {
     const int lane = threadIdx.x & 31;
-    if (i < count) {
-      const int t0 = key0 + i * KEYS, id = id_ahead, row = row_ahead;
-      look_up(i + step);
-      const bool ok = id >= 0 && id < a.num_pages;
-      if (!ok && t0 + lane % KEYS < key1) bad = true;
-      const uint32_t base = buf + stage * STAGE;
-      const int row0 = __shfl_sync(0xffffffffu, row, 0);
-      if (t0 + KEYS <= key1 && row0 + KEYS <= static_cast<int>(a.page.d) && __shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) {
-        // all keys in one page
-        const int id0 = __shfl_sync(0xffffffffu, id, 0);
+    if (next < count) {
+      if (K) {
+        const int t0 = key0 + next * KEYS;
+        id = id_ahead;
+        row = row_ahead;
+        look_up(next + step);
+        const bool there = t0 + lane % KEYS < key1;
+        ok = id >= 0 && id < a.num_pages;
+        if (!ok && there) bad = true;
+        ok = ok && there;
+        one_page = t0 + KEYS <= key1 && __shfl_sync(0xffffffffu, row + KEYS <= static_cast<int>(a.page.d) && ok ? 1 : 0, 0);
+      }
+      const uint32_t base = buf + slot_in * SLOT;
+      constexpr int V_AT = K ? HALF : 0;
+      if (one_page) {
+        const int id0 = __shfl_sync(0xffffffffu, id, 0), row0 = __shfl_sync(0xffffffffu, row, 0);
         const uint8_t* const kp = kb + id0 * a.kc_sp + row0 * a.kc_st;
         const uint8_t* const vp = vb + id0 * a.vc_sp + row0 * a.vc_st;
 #pragma unroll
@@ -269,23 +302,30 @@ struct KeyPipe {
           const int idx = j * 32 + lane, r = idx / CHUNKS, ch = idx % CHUNKS;
           const int bytes = ch < row_chunks ? 16 : 0;
           const uint32_t dst = base + r * ROW + ((ch ^ turn_of(r)) << 4);
-          cp_async16(dst, kp + r * a.kc_st + (bytes ? ch * 16 : 0), bytes);
-          cp_async16(dst + KEYS * ROW, vp + r * a.vc_st + (bytes ? ch * 16 : 0), bytes);
+          if (K) cp_async16(dst, kp + r * a.kc_st + (bytes ? ch * 16 : 0), bytes);
+          if (V) cp_async16(dst + V_AT, vp + r * a.vc_st + (bytes ? ch * 16 : 0), bytes);
         }
       } else {
-        const bool mine = ok && t0 + lane % KEYS < key1;
-        const int64_t ko = mine ? id * a.kc_sp + row * a.kc_st : -1, vo = mine ? id * a.vc_sp + row * a.vc_st : -1;
+        const int64_t ko = ok ? id * a.kc_sp + row * a.kc_st : -1, vo = ok ? id * a.vc_sp + row * a.vc_st : -1;
 #pragma unroll
         for (int j = 0; j < KEYS * CHUNKS / 32; ++j) {
           const int idx = j * 32 + lane, r = idx / CHUNKS, ch = idx % CHUNKS;
-          const int64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
-          const bool there = kr >= 0 && ch < row_chunks;
           const uint32_t dst = base + r * ROW + ((ch ^ turn_of(r)) << 4);
-          cp_async16(dst, there ? kb + kr + ch * 16 : a.q, there ? 16 : 0);
-          cp_async16(dst + KEYS * ROW, there ? vb + vr + ch * 16 : a.q, there ? 16 : 0);
+          if (K) {
+            const int64_t kr = __shfl_sync(0xffffffffu, ko, r);
+            const bool there = kr >= 0 && ch < row_chunks;
+            cp_async16(dst, there ? kb + kr + ch * 16 : a.q, there ? 16 : 0);
+          }
+          if (V) {
+            const int64_t vr = __shfl_sync(0xffffffffu, vo, r);
+            const bool there = vr >= 0 && ch < row_chunks;
+            cp_async16(dst + V_AT, there ? vb + vr + ch * 16 : a.q, there ? 16 : 0);
+          }
         }
       }
     }
+    if (V) next += step;
+    slot_in = slot_in + 1 == SLOTS ? 0 : slot_in + 1;
     cp_async_commit();
   }
 };
