@@ -1,0 +1,54 @@
+"""Calls of the serving operators at the edges of what they take (needs a B200; marked gpu): special values, views with
+odd strides, far positions, kept signatures that meet other pointers."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import cmpext3
+from cmpext3 import _native as N
+from tests.test_paged_attention_gpu import DTYPES, IDS
+
+pytestmark = pytest.mark.gpu
+
+SCHEDULES = [(40, "one CTA"), (3000, "cluster"), (9500, "equal shares")]
+
+
+def _cache(n, heads_kv, dim, dtype, dev, page=16):
+    """Caches of one sequence of n tokens (zeros) whose pages lie in order, its page table and its length."""
+    pages = -(-n // page)
+    k, v = (torch.zeros(pages, heads_kv, page, dim, dtype=dtype, device=dev) for _ in range(2))
+    return (k, v, torch.arange(pages, dtype=torch.int32, device=dev)[None], torch.tensor([n], dtype=torch.int32, device=dev))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("n,schedule", SCHEDULES)
+@pytest.mark.parametrize("gap", [20, 40, 80])
+def test_an_infinite_value_stays_infinite_under_a_small_weight(cuda_device, dtype, n, schedule, gap):
+    # one key's score is `gap` above all the others', whose weights, exp(-gap), are above 2^-126 of the largest
+    k, v, table, length = _cache(n, 1, 64, dtype, cuda_device)
+    q = torch.zeros(1, 2, 1, 64, dtype=dtype, device=cuda_device)
+    q[..., 0] = 8.0
+    v.fill_(1.0)
+    for top, at in ((0, n - 1), (n - 1, 0), (n // 2, n // 2 + 1)):
+        k.zero_()
+        k[top // 16, 0, top % 16, 0] = gap
+        v[at // 16, 0, at % 16, 3], v[at // 16, 0, at % 16, 6] = float("inf"), -float("inf")
+        assert schedule in N.paged_attention_plan(q, k, v, table, length)
+        out = cmpext3.ops.paged_attention(q, k, v, table, length)[0, :, 0].cpu()
+        v[at // 16, 0, at % 16] = 1.0
+        assert (out[:, 3] == float("inf")).all() and (out[:, 6] == -float("inf")).all()
+        rest = out[:, [d for d in range(64) if d not in (3, 6)]].double()
+        # values that are all 1: the weights' parts add up to the sum, but for the least parts of fp16's tiny weights
+        # (2^-37 of the largest each, below 2^-23 for 9500 keys), two roundings of 2^-24 a tile or part (700) and one
+        assert (rest - 1).abs().max() <= torch.finfo(dtype).eps / 2 + 1400 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_an_infinite_value_without_weight_has_no_product(cuda_device, dtype):
+    # a score of -inf: 0 * inf, in the definition too
+    k, v, table, length = _cache(40, 1, 64, dtype, cuda_device)
+    q = torch.ones(1, 2, 1, 64, dtype=dtype, device=cuda_device)
+    k[0, 0, 7, 5], v[0, 0, 7, 3] = -float("inf"), float("inf")
+    out = cmpext3.ops.paged_attention(q, k, v, table, length)[0, :, 0]
+    assert torch.isnan(out[:, 3]).all() and (out[:, :3] == 0).all() and (out[:, 4:] == 0).all()

@@ -15,9 +15,10 @@
 //     padded.
 // P is used as the sum of two 16-bit parts (cut off, and the rounded rest), so the weights carry 16 bits
 // and more; a second product of P V costs nothing here, and one part alone would add as much error as the
-// output's rounding does.  The rest is kept above zero, so that an infinite value stays infinite (0 * inf is
-// not).  fp16 weights are exp2(s - m + 14): without the factor, which cancels, the rest of a weight below
-// 2^-14 would fall into fp16's subnormal steps.
+// output's rounding does.  Both parts of a weight above zero are kept above zero, so that an infinite value stays
+// infinite (0 * inf is not) as long as its weight is 2^-126 of the largest or more.  fp16 weights are exp2(s - m + 14):
+// without the factor, which cancels, the rest of a weight below 2^-14 would fall into fp16's subnormal steps.  Those
+// below 2^-24 then count as 2^-23, 2^-37 of the largest: less than a thousandth of the output's rounding for 2^16 such keys.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -87,6 +88,12 @@ __device__ __forceinline__ uint32_t cut2(float lo, float hi) {
   else
     asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// A weight as its leading part is cut from: in fp16 at least the least that the type has, unless there is no weight.
+template <int DT>
+__device__ __forceinline__ float kept(float p) {
+  return DT == CMPX_F16 && p != 0.f ? fmaxf(p, 0x1p-24f) : p;
 }
 
 template <int DT, int DP, bool WHOLE, int kWarps>
@@ -187,7 +194,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == kCtaWarps ? MmaCfg<DP>:
         for (int n = 0; n < 2; ++n) {
           const float p0 = ex2_approx(s[n][2 * r] - base + kBias), p1 = ex2_approx(s[n][2 * r + 1] - base + kBias);
           l[r] += p0 + p1;
-          const uint32_t w = cut2<DT>(p0, p1);
+          const uint32_t w = cut2<DT>(kept<DT>(p0), kept<DT>(p1));
           float h0, h1;
           unpack2<DT>(w, h0, h1);
           hi[2 * n + r] = w;
