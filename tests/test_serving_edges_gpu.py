@@ -52,3 +52,23 @@ def test_an_infinite_value_without_weight_has_no_product(cuda_device, dtype):
     k[0, 0, 7, 5], v[0, 0, 7, 3] = -float("inf"), float("inf")
     out = cmpext3.ops.paged_attention(q, k, v, table, length)[0, :, 0]
     assert torch.isnan(out[:, 3]).all() and (out[:, :3] == 0).all() and (out[:, 4:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_queries_with_odd_strides_along_dimensions_of_one(cuda_device, dtype):
+    g = torch.Generator().manual_seed(30)
+    k, v, table, length = _cache(300, 2, 64, dtype, cuda_device)
+    for c in (k, v):
+        c.copy_(torch.randn(c.shape, generator=g))
+    wide = torch.randn(4, 515, generator=g).to(dtype).to(cuda_device)
+    row = wide[:, :512].unflatten(1, (8, 64)).unsqueeze(2)[0:1]      # [1, 8, 1, 64], batch stride 515
+    want = cmpext3.ops.paged_attention(row.clone(memory_format=torch.contiguous_format).view(1, 8, 1, 64), k, v, table, length)
+    for _ in range(2):                                               # the second call has a kept signature
+        assert torch.equal(cmpext3.ops.paged_attention(row, k, v, table, length), want)
+    turned = cmpext3.ops.kv_append(k[:1, :, :1].clone(), v[:1, :, :1].clone(), k, v, table, length, query=row)
+    assert torch.equal(turned, row)
+    assert cmpext3.ops.paged_attention(turned, k, v, table, length).shape == row.shape
+    one = torch.randn(3 * 64 + 515, generator=g).to(dtype).to(cuda_device).as_strided((3, 1, 1, 64), (64, 515, 64, 1))
+    table, length = table.expand(3, -1), torch.tensor([300, 17, 0], dtype=torch.int32, device=cuda_device)
+    want = cmpext3.ops.paged_attention(one.reshape(3, 64).clone().view(3, 1, 1, 64), k[:, :1], v[:, :1], table, length)
+    assert torch.equal(cmpext3.ops.paged_attention(one, k[:, :1], v[:, :1], table, length), want)

@@ -522,7 +522,7 @@ def _paged_attn_desc(query, k_cache, v_cache, page_table, lengths, scale):
         raise RuntimeError("scale must be finite")
     st = query.stride()
     unit = 16 // query.element_size()
-    if st[3] != 1 or st[0] % unit or st[1] % unit or query.data_ptr() % 16:
+    if st[3] != 1 or b > 1 and st[0] % unit or heads > 1 and st[1] % unit or query.data_ptr() % 16:
         query = query.contiguous()
         if query.data_ptr() % 16:
             query = query.clone()

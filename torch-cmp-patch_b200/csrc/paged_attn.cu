@@ -251,8 +251,9 @@ const char* paged_attn_plan(const cmpx_paged_attn_desc* d, int* status) {
   const int64_t es = elt_size(d->dtype);
   *status = CMPX_ERR_MISALIGNED;
   if (reinterpret_cast<uintptr_t>(d->q) % 16 || reinterpret_cast<uintptr_t>(d->o) % 16) return "none";
-  for (int i = 0; i < 2; ++i)
-    if ((d->q_stride[i] * es) % 16 || (d->o_stride[i] * es) % 16) return "none";
+  const int64_t extent[2] = {d->batch, d->heads};
+  for (int i = 0; i < 2; ++i)  // (a single one's stride is never stepped)
+    if (extent[i] > 1 && ((d->q_stride[i] * es) % 16 || (d->o_stride[i] * es) % 16)) return "none";
   *status = CMPX_ERR_UNSUPPORTED_SHAPE;
   if (d->heads > (1 << 20) || d->batch > (1 << 20) || d->batch * d->heads > (1ll << 31) - 65536) return "none";
   *status = CMPX_OK;
