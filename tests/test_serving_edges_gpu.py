@@ -72,3 +72,30 @@ def test_queries_with_odd_strides_along_dimensions_of_one(cuda_device, dtype):
     table, length = table.expand(3, -1), torch.tensor([300, 17, 0], dtype=torch.int32, device=cuda_device)
     want = cmpext3.ops.paged_attention(one.reshape(3, 64).clone().view(3, 1, 1, 64), k[:, :1], v[:, :1], table, length)
     assert torch.equal(cmpext3.ops.paged_attention(one, k[:, :1], v[:, :1], table, length), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_caches_and_rows_with_odd_strides_along_dimensions_of_one(cuda_device, dtype):
+    g = torch.Generator().manual_seed(31)
+    i32 = dict(dtype=torch.int32, device=cuda_device)
+    freqs = (10000.0 ** (-torch.arange(32, dtype=torch.float64) / 32)).float().to(cuda_device)
+    for shape, at, tokens in (((1, 2, 16, 64), 0, 3), ((4, 1, 16, 64), 1, 20), ((4, 2, 1, 64), 2, 3)):
+        pages, heads, page, dim = shape
+        k, v = (torch.randn(shape, generator=g).to(dtype).to(cuda_device) for _ in range(2))
+        stride = list(k.stride())
+        stride[at] = 12345
+        table = torch.arange(pages, **i32)[None]
+        length = torch.tensor([tokens], **i32)
+        new, query = (torch.randn(1, h, 1, dim, generator=g).to(dtype).to(cuda_device) for h in (heads, 2 * heads))
+        seen = []
+        for odd in (False, True):
+            kc, vc = k.clone(), v.clone()
+            if odd:
+                kc, vc = (c.as_strided(shape, stride) for c in (kc, vc))
+            turned = cmpext3.ops.kv_append(new, new, kc, vc, table, length, query=query, freqs=freqs)
+            seen.append((kc, vc, turned, cmpext3.ops.paged_attention(turned, kc, vc, table, length)))
+        assert all(torch.equal(a, b) for a, b in zip(*seen))
+    x = torch.randn(1, 3, 5, 64, generator=g).to(dtype).to(cuda_device)
+    y = cmpext3.ops.rope(x, torch.arange(5, device=cuda_device), freqs)
+    odd = x.as_strided(x.shape, (12345, *x.stride()[1:]))
+    assert torch.equal(cmpext3.ops.rope(odd, torch.arange(5, device=cuda_device), freqs), y)

@@ -230,21 +230,29 @@ bool rotation_ok(const cmpx_rotation& r, int64_t head_dim, bool place_allowed) {
   return at == r.pairs;
 }
 
-bool rows_aligned(const void* p, const int64_t* st, int es, int unit) {
-  if (reinterpret_cast<uintptr_t>(p) % unit != 0) return false;
+// Rows of head_dim values: where they begin, how far apart they are along three dimensions, and how many there are.
+struct RowLayout {
+  const void* p;
+  const int64_t* stride;  // elements
+  int64_t extent[3];
+};
+
+// Whether all rows begin at multiples of unit bytes.  The stride of a dimension of one is never stepped: it may be odd.
+bool rows_aligned(const RowLayout& r, int es, int unit) {
+  if (reinterpret_cast<uintptr_t>(r.p) % unit != 0) return false;
   for (int i = 0; i < 3; ++i)
-    if ((st[i] * es) % unit != 0) return false;
+    if (r.extent[i] > 1 && (r.stride[i] * es) % unit != 0) return false;
   return true;
 }
 
 // The widest vector (16, 4 bytes, or one element) that every row, the head and the two halves of the turned part
 // allow.  Between them only the count of memory instructions differs: one 16-byte access against four or eight.
-int pick_vec(int es, int64_t head_dim, int pairs, const void* const* ptrs, const int64_t* const* strides, int n) {
+int pick_vec(int es, int64_t head_dim, int pairs, const RowLayout* rows, int n) {
   for (int unit : {16, 4}) {
     if (unit < es) continue;
     bool ok = (head_dim * es) % unit == 0 && (static_cast<int64_t>(pairs) * es) % unit == 0;
     for (int i = 0; i < n && ok; ++i)
-      if (ptrs[i]) ok = rows_aligned(ptrs[i], strides[i], es, unit);
+      if (rows[i].p) ok = rows_aligned(rows[i], es, unit);
     if (ok) return unit;
   }
   return es;
@@ -300,16 +308,20 @@ int launch(RopeArgs& a, int dt, int vec_bytes, const LaunchCtx& ctx) {
 bool dtype_ok(int dt) { return dt == CMPX_F32 || dt == CMPX_F16 || dt == CMPX_BF16; }
 
 int rope_vec(const cmpx_rope_desc* d) {
-  const void* ptrs[2] = {d->x, d->y};
-  const int64_t* strides[2] = {d->x_stride, d->y_stride};
-  return pick_vec(elt_size(d->dtype), d->head_dim, d->rot.pairs, ptrs, strides, 2);
+  const RowLayout rows[2] = {{d->x, d->x_stride, {d->batch, d->heads, d->len}},
+                             {d->y, d->y_stride, {d->batch, d->heads, d->len}}};
+  return pick_vec(elt_size(d->dtype), d->head_dim, d->rot.pairs, rows, 2);
 }
 
 int append_vec(const cmpx_kv_append_desc* d) {
-  const void* ptrs[6] = {d->k, d->v, d->q, d->q_out, d->cache.k, d->cache.v};
-  const int64_t* strides[6] = {d->k_in_stride, d->v_in_stride, d->q_stride, d->q_out_stride, d->cache.k_stride,
-                               d->cache.v_stride};
-  return pick_vec(elt_size(d->dtype), d->cache.head_dim, d->rot.pairs, ptrs, strides, 6);
+  const cmpx_paged_cache& c = d->cache;
+  const RowLayout rows[6] = {{d->k, d->k_in_stride, {d->batch, c.heads_kv, d->len}},
+                             {d->v, d->v_in_stride, {d->batch, c.heads_kv, d->len}},
+                             {d->q, d->q_stride, {d->batch, d->heads, d->len}},
+                             {d->q_out, d->q_out_stride, {d->batch, d->heads, d->len}},
+                             {c.k, c.k_stride, {c.num_pages, c.heads_kv, c.page_size}},
+                             {c.v, c.v_stride, {c.num_pages, c.heads_kv, c.page_size}}};
+  return pick_vec(elt_size(d->dtype), c.head_dim, d->rot.pairs, rows, 6);
 }
 
 }  // namespace
@@ -333,7 +345,9 @@ int paged_cache_limits(const cmpx_paged_cache& c, int dtype) {
   if (c.num_pages > most || c.page_size > most || c.heads_kv > 65535 || c.table_width > most ||
       c.table_width > most / c.page_size)
     return CMPX_ERR_UNSUPPORTED_SHAPE;
-  if (!rows_aligned(c.k, c.k_stride, es, 16) || !rows_aligned(c.v, c.v_stride, es, 16)) return CMPX_ERR_MISALIGNED;
+  for (const RowLayout& rows : {RowLayout{c.k, c.k_stride, {c.num_pages, c.heads_kv, c.page_size}},
+                                RowLayout{c.v, c.v_stride, {c.num_pages, c.heads_kv, c.page_size}}})
+    if (!rows_aligned(rows, es, 16)) return CMPX_ERR_MISALIGNED;
   return CMPX_OK;
 }
 
