@@ -416,7 +416,8 @@ CMPX_API int cmpx_paged_attn_plan(const cmpx_paged_attn_desc* desc, char* buf, s
  * x's type; zeros [n, k / group] bytes (0..15) or NULL (8).  group is a multiple of 32 and
  * divides k.  The differences code - zero are exact in every type, their products with x are summed
  * in fp32 and multiplied by the fp32 value of the scale group by group; the bias is added before the
- * one rounding.  Rows of x and w start on 16-byte boundaries; w's row stride is at most 2^27 bytes. */
+ * one rounding.  Rows of x and w start on 16-byte boundaries; w's row stride, if it
+ * has several, is at most 2^27 bytes. */
 typedef struct cmpx_linear_w4_desc {
   const void* x;
   const uint8_t* w;

@@ -49,3 +49,10 @@ def test_strides_along_dimensions_of_one_do_not_narrow_the_vectors_or_refuse_a_c
     assert N.rope_plan(wide, torch.arange(4), freqs) == "rope<single values>"
     with pytest.raises(N.CmpxError):
         N.paged_attention_plan(torch.zeros(1, 2, 1, 64, dtype=dtype), wide, wide, torch.zeros(1, 2, **i32), torch.ones(1, **i32))
+
+
+def test_a_single_row_of_4_bit_weights_may_have_any_stride():
+    from tests.test_serving_host import _linear, _status
+    assert _status(N.lib.cmpx_linear_w4_plan, _linear(n=1, ws=(1 << 27) + 3))[0] == N.OK
+    assert _status(N.lib.cmpx_linear_w4_plan, _linear(m=1, xs=257))[0] == N.OK
+    assert _status(N.lib.cmpx_linear_w4_plan, _linear(n=2, ws=(1 << 27) + 16))[0] == N.ERR_UNSUPPORTED_SHAPE

@@ -555,7 +555,7 @@ const char* linear_w4_plan(const cmpx_linear_w4_desc* d, int* status) {
   *status = CMPX_ERR_UNSUPPORTED_SHAPE;
   if (d->group % 32 != 0 || d->k > (1 << 24) || d->n > ((1ll << 38) / d->k) || d->n > (1ll << 31) - 65536 || d->m > 65535ll * 8) return "none";
   // (the kernel counts 12 rows of W in 32 bits)
-  if (d->x_row_stride < 0 || d->w_row_stride < 0 || d->w_row_stride > (1 << 27) || d->scales_row_stride < 0 || d->zeros_row_stride < 0 ||
+  if (d->x_row_stride < 0 || d->w_row_stride < 0 || (d->n > 1 && d->w_row_stride > (1 << 27)) || d->scales_row_stride < 0 || d->zeros_row_stride < 0 ||
       d->y_row_stride < d->n)
     return "none";
   *status = CMPX_ERR_MISALIGNED;
