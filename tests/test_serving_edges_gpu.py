@@ -99,3 +99,17 @@ def test_caches_and_rows_with_odd_strides_along_dimensions_of_one(cuda_device, d
     y = cmpext3.ops.rope(x, torch.arange(5, device=cuda_device), freqs)
     odd = x.as_strided(x.shape, (12345, *x.stride()[1:]))
     assert torch.equal(cmpext3.ops.rope(odd, torch.arange(5, device=cuda_device), freqs), y)
+
+
+def test_dual_tensors_are_refused_with_a_kept_signature_too(cuda_device):
+    from torch.autograd import forward_ad as fa
+    x = torch.randn(1, 2, 3, 16, device=cuda_device)
+    positions, freqs = torch.arange(3, device=cuda_device), torch.ones(8, device=cuda_device)
+    want = cmpext3.ops.rope(x, positions, freqs)
+    with fa.dual_level():
+        assert torch.equal(cmpext3.ops.rope(x, positions, freqs), want)    # a level without duals changes nothing
+        dual = fa.make_dual(x, x.clone())
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            cmpext3.ops.rope(dual, positions, freqs)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            cmpext3.ops.rope(fa.make_dual(x.clone().requires_grad_(), x.clone()), positions, freqs)

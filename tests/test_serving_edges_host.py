@@ -56,3 +56,43 @@ def test_a_single_row_of_4_bit_weights_may_have_any_stride():
     assert _status(N.lib.cmpx_linear_w4_plan, _linear(n=1, ws=(1 << 27) + 3))[0] == N.OK
     assert _status(N.lib.cmpx_linear_w4_plan, _linear(m=1, xs=257))[0] == N.OK
     assert _status(N.lib.cmpx_linear_w4_plan, _linear(n=2, ws=(1 << 27) + 16))[0] == N.ERR_UNSUPPORTED_SHAPE
+
+
+# ---- derivatives -------------------------------------------------------------------------------
+
+def test_dual_tensors_are_refused(cpu):
+    # their tangents would be lost: in each differentiable argument, with autograd on and off
+    from torch.autograd import forward_ad as fa
+    ops = cmpext3.ops
+    x, p, f = torch.randn(2, 2, 3, 16), torch.arange(3.0), torch.ones(8)
+    k, v, table, lengths = _cache_args()
+    one = torch.randn(2, 4, 1, 16)
+    w, act, scale, bias = torch.zeros(5, 32, dtype=torch.uint8), torch.randn(3, 64), torch.ones(5, 2), torch.ones(5)
+    calls = [(ops.rope, (x, p, f), (0, 1, 2)),
+             (lambda *a: ops.kv_append(*a[:6], query=a[6], positions=a[7], freqs=a[8]),
+              (x, x.clone(), k, v, table, lengths, x.clone(), p, f), (0, 1, 2, 3, 6, 7, 8)),
+             (ops.paged_attention, (one, k, v, table, lengths), (0, 1, 2)),
+             (lambda *a: ops.linear_w4(*a[:3], None, a[3]), (act, w, scale, bias), (0, 2, 3))]
+    with fa.dual_level():
+        for call, args, wheres in calls:
+            for i in wheres:
+                dual = list(args)
+                dual[i] = fa.make_dual(args[i].clone(), torch.ones_like(args[i]))
+                refused("no forward-mode derivative", call, *dual)
+                with torch.no_grad():
+                    refused("no forward-mode derivative", call, *dual)
+                dual[i] = dual[i].detach()
+                with pytest.raises(BaseException) as e:   # detached it goes on to the device check or the launch
+                    call(*dual)
+                assert "forward-mode" not in str(e.value)
+
+
+def test_a_gradient_with_a_tangent_is_refused_in_the_backward_pass(cpu, monkeypatch):
+    from torch.autograd import forward_ad as fa
+    monkeypatch.setattr(S, "_run", lambda *a: None)
+    monkeypatch.setattr(S, "_note_leaf", lambda *a: None)
+    x, p, f = torch.randn(1, 2, 3, 16, requires_grad=True), torch.arange(3), torch.ones(8)
+    y = cmpext3.ops.rope(x, p, f)
+    with fa.dual_level():
+        grad = fa.make_dual(torch.ones_like(y), torch.ones_like(y))
+        refused("no forward-mode derivative", torch.autograd.grad, y, x, grad)

@@ -12,7 +12,7 @@ weights.  ``cmpext3.ops`` offers them beside ``attention`` and ``linear``:
 As in the rest of the binding: arguments are checked here, outputs and scratch come from torch's
 caching allocator, work goes to the current stream of the tensors' device, and what the kernels do not
 cover raises ``RuntimeError`` / ``TypeError``.  ``rope`` has a gradient; the others are for inference
-and refuse tensors that autograd is recording.
+and refuse tensors that autograd is recording.  All refuse dual tensors (forward-mode derivatives).
 """
 from __future__ import annotations
 
@@ -21,6 +21,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad as _forward
 
 from ._native import _CHECK, _DTYPE, OK, CmpxError, _post_check, _stream_handle, _traced, lib
 
@@ -187,6 +188,14 @@ def _no_grad_only(what: str, *tensors) -> None:
                 raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
+def _no_tangent(what: str, *tensors) -> None:
+    """Refuses dual tensors, whose tangents the kernels would drop; only called within a dual level."""
+    if torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and _forward.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative: call it on detached tensors")
+
+
 def _unit(t: torch.Tensor) -> torch.Tensor:
     """t with a contiguous last dimension (a copy where it has none)."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
@@ -271,6 +280,8 @@ def _rope_desc(x, positions, freqs, sections, interleaved, inverse):
 
 
 def _rope_call(x, positions, freqs, sections, interleaved, inverse):
+    if _forward._current_level >= 0:
+        _no_tangent("rope", x, positions, freqs)
     try:
         key = ("rope", x.shape, x.stride(), x.dtype, x.device, positions.shape, positions.stride(), positions.dtype,
                positions.device, freqs.shape, freqs.stride(), freqs.dtype, freqs.device, sections, interleaved, inverse)
@@ -342,7 +353,7 @@ def rope(input, positions, freqs, sections=None, interleaved=False):
     ...): the first sections[0] pairs turn by positions[0], the next by positions[1], and so on.
     Angles are computed in 64 bits (good below 2^50 radians); the result, a new tensor laid out as
     input, is rounded once.
-    Differentiable in ``input``; positions and freqs have no gradient.  A capture of forward and backward pass
+    Differentiable in ``input`` (backward passes; forward mode is refused); positions and freqs have no gradient.  A capture of forward and backward pass
     into a CUDA graph needs its leaves free of eager graphs from the default stream (RuntimeError).
     head_dim <= 256."""
     sections, interleaved = None if sections is None else tuple(sections), bool(interleaved)
@@ -460,6 +471,8 @@ def kv_append(key, value, k_cache, v_cache, page_table, lengths, new_lengths=Non
     sections, interleaved = None if sections is None else tuple(sections), bool(interleaved)
     if torch.is_grad_enabled():
         _no_grad_only("kv_append", key, value, k_cache, v_cache, query, positions, freqs)
+    if _forward._current_level >= 0:
+        _no_tangent("kv_append", key, value, k_cache, v_cache, query, positions, freqs)
     try:
         sig = ("kv_append", key.shape, key.stride(), key.dtype, key.device, value.shape, value.stride(), value.dtype,
                value.device, k_cache.shape, k_cache.stride(), k_cache.dtype, k_cache.device, v_cache.shape,
@@ -547,6 +560,8 @@ def paged_attention(query, k_cache, v_cache, page_table, lengths, scale=None):
     scale = None if scale is None else float(scale)
     if torch.is_grad_enabled():
         _no_grad_only("paged_attention", query, k_cache, v_cache)
+    if _forward._current_level >= 0:
+        _no_tangent("paged_attention", query, k_cache, v_cache)
     try:
         sig = ("paged_attention", query.shape, query.stride(), query.dtype, query.device, k_cache.shape, k_cache.stride(),
                k_cache.dtype, k_cache.device, v_cache.shape, v_cache.stride(), v_cache.dtype, v_cache.device,
@@ -644,6 +659,8 @@ def linear_w4(input, weight, scales, zeros=None, bias=None):
     dequantised weight and ``linear`` are the faster way."""
     if torch.is_grad_enabled():
         _no_grad_only("linear_w4", input, scales, bias)
+    if _forward._current_level >= 0:
+        _no_tangent("linear_w4", input, scales, bias)
     try:
         sig = ("linear_w4", input.shape, input.stride(), input.dtype, input.device, weight.shape, weight.stride(),
                weight.dtype, weight.device, scales.shape, scales.stride(), scales.dtype, scales.device)
