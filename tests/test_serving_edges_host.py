@@ -96,3 +96,20 @@ def test_a_gradient_with_a_tangent_is_refused_in_the_backward_pass(cpu, monkeypa
     with fa.dual_level():
         grad = fa.make_dual(torch.ones_like(y), torch.ones_like(y))
         refused("no forward-mode derivative", torch.autograd.grad, y, x, grad)
+
+
+# ---- kept signatures ---------------------------------------------------------------------------
+
+def test_sections_that_equal_kept_ones_are_refused_all_the_same(cpu, monkeypatch):
+    class Kept(dict):
+        def get(self, key, default=None):
+            return (b"", b"", 0) if key[0] == "kv_append" else (b"", 0)
+    monkeypatch.setattr(S, "_SIGNATURES", Kept())
+    monkeypatch.setattr(S, "_direct", lambda *a: N.OK)
+    x, f = torch.randn(2, 2, 3, 16), torch.ones(8)
+    positions, cache = torch.zeros(2, 3), _cache_args()
+    cmpext3.ops.rope(x, positions, f, (4, 4))
+    for sections in ((4.0, 4.0), [4, 4.0], (True, 7), (torch.tensor(4), 4)):
+        refused("whole numbers", cmpext3.ops.rope, x, positions, f, sections, error=TypeError)
+        refused("whole numbers", cmpext3.ops.kv_append, x, x, *cache, positions=positions, freqs=f, sections=sections,
+                error=TypeError)

@@ -218,6 +218,14 @@ def _is_like(out: torch.Tensor, t: torch.Tensor) -> bool:
 # rotary positions
 # ---------------------------------------------------------------------------------------------
 
+def _whole(sections) -> tuple:
+    # before a kept signature is looked up, where 8.0 would pass for 8
+    sections = tuple(sections)
+    if not all(type(n) is int for n in sections):
+        raise TypeError("sections must be whole numbers")
+    return sections
+
+
 def _rotation(positions, freqs, sections, interleaved, batch: int, tokens: int, head_dim: int,
               device: torch.device) -> tuple[Rotation, tuple]:
     """The descriptor of a rotation, and the tensors it points into."""
@@ -229,8 +237,7 @@ def _rotation(positions, freqs, sections, interleaved, batch: int, tokens: int, 
     axes = 1
     ends = (pairs, 0, 0, 0)
     if sections is not None:
-        if not all(type(n) is int for n in sections):
-            raise TypeError("sections must be whole numbers")
+        sections = _whole(sections)
         axes = len(sections)
         if not 1 <= axes <= _MAX_AXES or min(sections) < 0 or sum(sections) != pairs:
             raise RuntimeError(f"sections must be 1 to {_MAX_AXES} counts of pairs that add up to {pairs}, got {sections}")
@@ -356,7 +363,7 @@ def rope(input, positions, freqs, sections=None, interleaved=False):
     Differentiable in ``input`` (backward passes; forward mode is refused); positions and freqs have no gradient.  A capture of forward and backward pass
     into a CUDA graph needs its leaves free of eager graphs from the default stream (RuntimeError).
     head_dim <= 256."""
-    sections, interleaved = None if sections is None else tuple(sections), bool(interleaved)
+    sections, interleaved = None if sections is None else _whole(sections), bool(interleaved)
     if torch.is_grad_enabled():
         _no_grad_only("rope in positions and freqs", positions, freqs)
         if isinstance(input, torch.Tensor) and input.requires_grad:
@@ -468,7 +475,7 @@ def kv_append(key, value, k_cache, v_cache, page_table, lengths, new_lengths=Non
     A token whose place is negative, behind the table or in a page that does not exist is not stored and
     sets a bit of ``device_status()``.  Which of two tokens that share a slot stays is not defined; key and
     value must not lie in the caches' memory."""
-    sections, interleaved = None if sections is None else tuple(sections), bool(interleaved)
+    sections, interleaved = None if sections is None else _whole(sections), bool(interleaved)
     if torch.is_grad_enabled():
         _no_grad_only("kv_append", key, value, k_cache, v_cache, query, positions, freqs)
     if _forward._current_level >= 0:
