@@ -287,8 +287,6 @@ def _rope_desc(x, positions, freqs, sections, interleaved, inverse):
 
 
 def _rope_call(x, positions, freqs, sections, interleaved, inverse):
-    if _forward._current_level >= 0:
-        _no_tangent("rope", x, positions, freqs)
     try:
         key = ("rope", x.shape, x.stride(), x.dtype, x.device, positions.shape, positions.stride(), positions.dtype,
                positions.device, freqs.shape, freqs.stride(), freqs.dtype, freqs.device, sections, interleaved, inverse)
@@ -341,6 +339,8 @@ class _Rope(torch.autograd.Function):
     def backward(ctx, grad):
         positions, freqs = ctx.saved_tensors
         sections, interleaved, inverse = ctx.how
+        if _forward._current_level >= 0:
+            _no_tangent("rope's gradient", grad)
         if torch.is_grad_enabled() and grad.requires_grad:
             gx = _Rope.apply(grad, positions, freqs, sections, interleaved, not inverse)
         else:
@@ -364,6 +364,8 @@ def rope(input, positions, freqs, sections=None, interleaved=False):
     into a CUDA graph needs its leaves free of eager graphs from the default stream (RuntimeError).
     head_dim <= 256."""
     sections, interleaved = None if sections is None else _whole(sections), bool(interleaved)
+    if _forward._current_level >= 0:
+        _no_tangent("rope", input, positions, freqs)
     if torch.is_grad_enabled():
         _no_grad_only("rope in positions and freqs", positions, freqs)
         if isinstance(input, torch.Tensor) and input.requires_grad:
