@@ -307,8 +307,9 @@ typedef enum cmpx_pos_kind {
  * The pair is (x[j], x[j + pairs]), or (x[2j], x[2j + 1]) where interleaved is 1; values behind the
  * first 2 * pairs of a row pass through.  Axis a takes the pairs section_end[a - 1] <= j <
  * section_end[a] (section_end[axes - 1] == pairs).  positions holds one value per axis, batch item
- * and token, pos_stride elements apart (0 = broadcast).  The angle is computed in 64 bits, so far
- * positions keep their full precision; the products and the sum are fp32, rounded once. */
+ * and token, pos_stride elements apart (0 = broadcast).  The angle is reduced in 64 bits with the rest of
+ * its product, so that it is exact to fp32 below 2^50 radians (positions of up to 2^53); the products and the
+ * sum are fp32, rounded once. */
 typedef struct cmpx_rotation {
   const void* positions;
   const float* freqs;    /* [pairs] radians per position */

@@ -113,3 +113,33 @@ def test_dual_tensors_are_refused_with_a_kept_signature_too(cuda_device):
             cmpext3.ops.rope(dual, positions, freqs)
         with pytest.raises(RuntimeError, match="forward-mode"):
             cmpext3.ops.rope(fa.make_dual(x.clone().requires_grad_(), x.clone()), positions, freqs)
+
+
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64, torch.float32])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_far_angles_are_exact_to_fp32(cuda_device, kind, interleaved):
+    # angles up to 2^50 radians, reduced here in 80 decimal digits
+    import math
+    from decimal import Decimal, localcontext
+    places = [2 ** 28 + 32, 2 ** 31 - 128, -(2 ** 31)]
+    if kind != torch.int32:
+        places += [2 ** 40 + 2 ** 17, 2 ** 49 - 2 ** 25, -(2 ** 49) - 2 ** 30]
+    if kind == torch.int64:
+        places += [2 ** 31 - 1, 2 ** 40 + 3, 2 ** 49 - 1, 10 ** 14 + 7]
+    positions, freqs = torch.tensor(places).to(kind), torch.tensor([1.0, 0.3, 1e-3, 1.7])
+    assert [int(p) for p in positions.tolist()] == places
+    x = torch.randn(1, 2, len(places), 10, generator=torch.Generator().manual_seed(32))
+    y = cmpext3.ops.rope(x.to(cuda_device), positions.to(cuda_device), freqs.to(cuda_device), interleaved=interleaved).cpu().double()
+    with localcontext() as ctx:
+        ctx.prec = 80
+        turn = 2 * Decimal("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899")
+        rest = torch.tensor([[float(Decimal(p) * Decimal(f) % turn) for f in freqs.tolist()] for p in places], dtype=torch.float64)
+    cos, sin = torch.cos(rest), torch.sin(rest)
+    re, im = (slice(0, 8, 2), slice(1, 8, 2)) if interleaved else (slice(0, 4), slice(4, 8))
+    u, w = x[..., re].double(), x[..., im].double()
+    # cos and sin are off by at most 2^-23 (half a step of the fp32 remainder, and their polynomials' own), the two products
+    # and the sum by 2^-24 each of at most |u| + |w|, the result by its rounding
+    bound = (u.abs() + w.abs()) * 2.0 ** -21
+    for got, want in ((y[..., re], u * cos - w * sin), (y[..., im], u * sin + w * cos)):
+        assert ((got - want).abs() - bound).max() <= 0, (got - want).abs().amax((0, 1, 3))
+    assert torch.equal(y[..., 8:], x[..., 8:].double()) and math.isfinite(y.sum())

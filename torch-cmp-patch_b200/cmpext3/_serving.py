@@ -358,8 +358,8 @@ def rope(input, positions, freqs, sections=None, interleaved=False):
     ``positions`` (int32, int64 or float32) is [tokens] or [batch, tokens].  With ``sections``, up to
     four counts that add up to pairs, positions has a leading axis of that many (time, height, width,
     ...): the first sections[0] pairs turn by positions[0], the next by positions[1], and so on.
-    Angles are computed in 64 bits (good below 2^50 radians); the result, a new tensor laid out as
-    input, is rounded once.
+    Angles are exact to fp32 below 2^50 radians (positions of up to 2^53); the result, a new tensor laid out
+    as input, is rounded once.
     Differentiable in ``input`` (backward passes; forward mode is refused); positions and freqs have no gradient.  A capture of forward and backward pass
     into a CUDA graph needs its leaves free of eager graphs from the default stream (RuntimeError).
     head_dim <= 256."""

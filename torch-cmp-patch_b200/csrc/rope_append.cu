@@ -13,7 +13,7 @@
 // addresses take more registers, with four heads and two blocks (4 x 2048 tokens, 16 heads of 64, fp16, 71 MB:
 // 16.6 us; 18.9 with two and four).
 // The angle is reduced in fp64 (1e6 radians in fp32 are off by 0.06) to within an eighth of a turn, where
-// short Taylor sums of sine and cosine are exact to fp32.
+// short Taylor sums of sine and cosine are exact to fp32 (below 2^50 radians: turn()).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -65,16 +65,18 @@ __device__ __forceinline__ double load_pos(const RopeArgs& a, int axis, int b, i
   return static_cast<double>(static_cast<const float*>(a.pos)[i]);
 }
 
-// cos and sin of pos * freq, given quarters = pos * 2 / pi.  quarters * freq is the angle in quarter turns: adding
-// 1.5 * 2^52 rounds it to a whole number, whose last two bits, now the sum's, are the quadrant; the
-// rest, at most half a quarter turn, goes to the Taylor sums up to x^9 / 9! and x^10 / 10! (the next
-// terms are below 2^-29 there).  Good for angles below 2^50.
-__device__ __forceinline__ void turn(double quarters, float freq, float& c, float& s) {
-  constexpr double kRound = 6755399441055744.0;
+// cos and sin of pos * freq.  pos * 2 / pi, times freq, is the angle in quarter turns: adding 1.5 * 2^52 rounds it to
+// a whole number, whose last two bits, now the sum's, are the quadrant; the rest, at most half a quarter turn, goes to
+// the Taylor sums up to x^9 / 9! and x^10 / 10! (the next terms are below 2^-29 there).  2 / pi and the product
+// with it are the sums of two doubles each: what the first leaves over, 2^-53 of the angle, passes an fp32 step from 2^28
+// radians on.  With it the angle is exact to fp32 below 2^50, where the rounding ends.
+__device__ __forceinline__ void turn(double pos, float freq, float& c, float& s) {
+  constexpr double kRound = 6755399441055744.0, kTwoOverPi = 0.6366197723675814, kTwoOverPiRest = -3.935735335036497e-17;
   const double f = static_cast<double>(freq);
+  const double quarters = pos * kTwoOverPi, over = fma(pos, kTwoOverPiRest, fma(pos, kTwoOverPi, -quarters));
   const double sum = fma(quarters, f, kRound);
   const int quad = __double2loint(sum) & 3;
-  const float x = static_cast<float>(fma(quarters, f, -(sum - kRound)) * 1.57079632679489661923);
+  const float x = static_cast<float>(fma(over, f, fma(quarters, f, -(sum - kRound))) * 1.57079632679489661923);
   const float x2 = x * x;
   const float sine = fmaf(x * x2, fmaf(x2, fmaf(x2, fmaf(x2, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f), x);
   const float cosine =
@@ -135,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(APPEND)) rope_append_k
   if (turned && there) {
     double pos[CMPX_ROPE_MAX_AXES];
 #pragma unroll
-    for (int x = 0; x < CMPX_ROPE_MAX_AXES; ++x) pos[x] = x < a.axes ? load_pos(a, x, b, l, place) * 0.63661977236758134308 : 0.0;
+    for (int x = 0; x < CMPX_ROPE_MAX_AXES; ++x) pos[x] = x < a.axes ? load_pos(a, x, b, l, place) : 0.0;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const int j = c * VEC + i;
