@@ -402,7 +402,7 @@ typedef struct cmpx_paged_attn_desc {
   int64_t batch, heads;
   int64_t q_stride[2]; /* batch, head (elements) */
   int64_t o_stride[2];
-  double scale;
+  double scale;  /* scale * log2(e) is finite in fp32 */
   int32_t dtype; /* cmpx_dtype */
   int32_t reserved;
 } cmpx_paged_attn_desc;

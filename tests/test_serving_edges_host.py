@@ -113,3 +113,15 @@ def test_sections_that_equal_kept_ones_are_refused_all_the_same(cpu, monkeypatch
         refused("whole numbers", cmpext3.ops.rope, x, positions, f, sections, error=TypeError)
         refused("whole numbers", cmpext3.ops.kv_append, x, x, *cache, positions=positions, freqs=f, sections=sections,
                 error=TypeError)
+
+
+# ---- the scale ---------------------------------------------------------------------------------
+
+def test_a_scale_that_is_infinite_in_fp32_is_refused(cpu):
+    from tests.test_serving_host import _attn, _status
+    q, args = torch.randn(2, 4, 1, 16), _cache_args()
+    for scale in (1e300, -1e39, 3e38, float("nan"), float("-inf")):
+        refused("scale must be finite", cmpext3.ops.paged_attention, q, *args, scale)
+        assert _status(N.lib.cmpx_paged_attn_plan, _attn(scale=scale))[0] == N.ERR_INVALID_ARGUMENT
+    for scale in (2.3e38, -1e30, 0.0):
+        assert "paged_attn" in N.paged_attention_plan(q, *args, scale)

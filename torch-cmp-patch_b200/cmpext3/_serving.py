@@ -540,8 +540,8 @@ def _paged_attn_desc(query, k_cache, v_cache, page_table, lengths, scale):
     if cache.head_dim != d or heads % cache.heads_kv:
         raise RuntimeError(f"k_cache {tuple(k_cache.shape)} does not match query {tuple(query.shape)}")
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise RuntimeError("scale must be finite")
+    if not abs(scale) * math.log2(math.e) <= torch.finfo(torch.float32).max:  # the kernels' factor, of scores in log2 units
+        raise RuntimeError("scale must be finite (in fp32)")
     st = query.stride()
     unit = 16 // query.element_size()
     if st[3] != 1 or b > 1 and st[0] % unit or heads > 1 and st[1] % unit or query.data_ptr() % 16:

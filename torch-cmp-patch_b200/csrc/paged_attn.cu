@@ -151,6 +151,8 @@ __global__ void __launch_bounds__(32 * W) paged_join_kernel(const __grid_constan
 // host
 // ---------------------------------------------------------------------------------------------
 
+float scale_log2(const cmpx_paged_attn_desc* d) { return static_cast<float>(d->scale * 1.4426950408889634074); }
+
 // fp32 on the tensor cores: from five heads per item on, where the FMA units bound the other kernel ([8, 32/4, 128],
 // 6103 keys: 37 us, 53 there; with four heads the other takes 35), and from two where that kernel pads the heads to 128 and this
 // one to 96 ([8, 16/4, 80], 9765 keys: 42 and 48).  Above 192 the queries do not fit its registers.
@@ -242,7 +244,7 @@ int launch_join_dim(const PagedArgs& a, int64_t most_parts, const LaunchCtx& ctx
 
 const char* paged_attn_plan(const cmpx_paged_attn_desc* d, int* status) {
   *status = CMPX_ERR_INVALID_ARGUMENT;
-  if (!d || !d->q || !d->o || d->batch < 0 || d->heads < 0 || !std::isfinite(d->scale)) return "none";
+  if (!d || !d->q || !d->o || d->batch < 0 || d->heads < 0 || !std::isfinite(scale_log2(d))) return "none";
   if (!paged_cache_ok(d->cache, d->batch) || d->heads % d->cache.heads_kv != 0) return "none";
   *status = CMPX_ERR_UNSUPPORTED_DTYPE;
   if (d->dtype != CMPX_F32 && d->dtype != CMPX_F16 && d->dtype != CMPX_BF16) return "none";
@@ -307,7 +309,7 @@ int launch_paged_attn(const cmpx_paged_attn_desc* d, const LaunchCtx& ctx) {
   a.item_heads = s.item_heads;
   a.items_per_head = s.items_per_head;
   a.head_dim = static_cast<int>(c.head_dim);
-  a.scale_log2 = static_cast<float>(d->scale * 1.4426950408889634074);
+  a.scale_log2 = scale_log2(d);
   a.workers = s.workers;
   a.flags = ctx.dev_flags;
   if (floats) {
