@@ -143,3 +143,67 @@ def test_far_angles_are_exact_to_fp32(cuda_device, kind, interleaved):
     for got, want in ((y[..., re], u * cos - w * sin), (y[..., im], u * sin + w * cos)):
         assert ((got - want).abs() - bound).max() <= 0, (got - want).abs().amax((0, 1, 3))
     assert torch.equal(y[..., 8:], x[..., 8:].double()) and math.isfinite(y.sum())
+
+
+# ---- a kept signature meets other pointers -----------------------------------------------------
+
+def _shifted(t):
+    """Copies of t, contiguous: at a new allocation's begin, and one element behind it."""
+    return [torch.zeros(t.numel() + 1, dtype=t.dtype, device=t.device)[at:at + t.numel()].view(t.shape).copy_(t) for at in (0, 1)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_a_kept_signature_with_misaligned_tensors(cuda_device, dtype):
+    g = torch.Generator().manual_seed(33)
+    dev, ops = cuda_device, cmpext3.ops
+
+    def randn(*shape):
+        return torch.randn(shape, generator=g).to(dtype).to(dev)
+
+    def both(call, *tensors):
+        """call(*tensors), aligned, a second time with its kept signature, then with each tensor misaligned in turn."""
+        pairs = [_shifted(t) for t in tensors]
+        first = [p[0] for p in pairs]
+        want = call(*first)
+        assert torch.equal(call(*first), want)
+        for i, (_, off) in enumerate(pairs):
+            assert off.data_ptr() % 16 and off.stride() == first[i].stride()
+            assert torch.equal(call(*first[:i], off, *first[i + 1:]), want), i
+        assert torch.equal(call(*first), want)
+    freqs = (10000.0 ** (-torch.arange(32, dtype=torch.float64) / 32)).float().to(dev)
+    both(ops.rope, randn(2, 3, 5, 64), torch.arange(5, device=dev), freqs)
+    k, v, table, length = _cache(300, 2, 64, dtype, dev)
+    k.copy_(randn(*k.shape)), v.copy_(randn(*v.shape))
+    both(lambda q, t, n: ops.paged_attention(q, k, v, t, n), randn(1, 8, 1, 64), table, length)
+
+    def append(key, value, t, n, new, query, f):
+        kc, vc = k.clone(), v.clone()
+        out = ops.kv_append(key, value, kc, vc, t, n, new, query, freqs=f)
+        return torch.cat((kc.flatten(), vc.flatten(), out.flatten()))
+    both(append, randn(1, 2, 3, 64), randn(1, 2, 3, 64), table, length, torch.tensor([2], dtype=torch.int32, device=dev),
+         randn(1, 4, 3, 64), freqs)
+    w = torch.randint(0, 256, (40, 128), generator=g, dtype=torch.uint8).to(dev)
+    zeros = torch.randint(0, 16, (40, 4), generator=g, dtype=torch.uint8).to(dev)
+    both(ops.linear_w4, randn(3, 256), w, randn(40, 4), zeros, randn(40))
+    # a cache off its 16-byte boundaries has no other way: refused, kept signature or not
+    off = _shifted(k)[1]
+    for _ in range(2):
+        with pytest.raises(N.CmpxError, match="aligned"):
+            ops.paged_attention(randn(1, 8, 1, 64), off, v, table, length)
+        with pytest.raises(N.CmpxError, match="aligned"):
+            ops.kv_append(randn(1, 2, 3, 64), randn(1, 2, 3, 64), off, v, table, length)
+    assert N.device_status() == 0
+
+
+def test_more_signatures_than_are_kept(cuda_device, monkeypatch):
+    from cmpext3 import _serving as S
+    monkeypatch.setattr(S, "_SIGNATURES", {})
+    monkeypatch.setattr(S, "_SIGNATURES_MOST", 5)
+    freqs = torch.ones(8, device=cuda_device)
+    xs = [torch.randn(1, 2, n, 16, device=cuda_device) for n in range(1, 14)]
+    want = [cmpext3.ops.rope(x, torch.arange(x.shape[2], device=cuda_device), freqs) for x in xs]
+    assert 1 <= len(S._SIGNATURES) <= 5
+    for _ in range(2):
+        for x, y in zip(xs, want):
+            assert torch.equal(cmpext3.ops.rope(x, torch.arange(x.shape[2], device=cuda_device), freqs), y)
+            assert len(S._SIGNATURES) <= 5
