@@ -207,3 +207,23 @@ def test_more_signatures_than_are_kept(cuda_device, monkeypatch):
         for x, y in zip(xs, want):
             assert torch.equal(cmpext3.ops.rope(x, torch.arange(x.shape[2], device=cuda_device), freqs), y)
             assert len(S._SIGNATURES) <= 5
+
+
+# ---- linear_w4: all three parts of fp32 activations ----------------------------------------------
+
+@pytest.mark.parametrize("m", [1, 8, 9, 16])
+@pytest.mark.parametrize("k,group", [(64, 64), (96, 32), (160, 32), (256, 128), (4096, 32), (4096, 64), (4096, 128), (16384, 128)])
+def test_low_parts_of_full_precision_activations(cuda_device, m, k, group):
+    # x = 1 + a 2^-12 + b 2^-22, a < 16, b < 4: a value in each part of 8 bits.  Weights are +1 for k % 8 < 4 and -1 else, so that the
+    # ones cancel in every product of 16 k; what is left are multiples of 2^-22, below 2 in all partial sums: exact in fp32
+    g = torch.Generator().manual_seed(m + k + group)
+    a, b = torch.randint(0, 16, (m, k), generator=g), torch.randint(0, 4, (m, k), generator=g)
+    x = (1 + a * 2.0 ** -12 + b * 2.0 ** -22).float()
+    assert torch.equal(x.double(), 1 + a * 2.0 ** -12 + b * 2.0 ** -22)
+    sign = torch.where(torch.arange(k) % 8 < 4, 1, -1)
+    codes = (8 + sign).to(torch.uint8).expand(24, k)
+    w = codes[:, 0::2] | (codes[:, 1::2] << 4)
+    want = (x.double() * sign).sum(1)
+    assert want.abs().max() < 2
+    y = cmpext3.ops.linear_w4(x.to(cuda_device), w.to(cuda_device), torch.ones(24, k // group, device=cuda_device))
+    assert torch.equal(y.cpu().double(), want[:, None].expand(m, 24))
