@@ -360,8 +360,10 @@ def rope(input, positions, freqs, sections=None, interleaved=False):
     ...): the first sections[0] pairs turn by positions[0], the next by positions[1], and so on.
     Angles are exact to fp32 below 2^50 radians (positions of up to 2^53); the result, a new tensor laid out
     as input, is rounded once.
-    Differentiable in ``input`` (backward passes; forward mode is refused); positions and freqs have no gradient.  A capture of forward and backward pass
-    into a CUDA graph needs its leaves free of eager graphs from the default stream (RuntimeError).
+    Differentiable in ``input`` (backward passes; forward mode is refused); positions and freqs have no gradient.
+    A capture of forward and backward pass into a CUDA graph needs its leaves free of eager graphs from the
+    default stream: RuntimeError where rope recorded them; those of other ops are not seen here, and end the
+    process in autograd's thread as they do with any op.
     head_dim <= 256."""
     sections, interleaved = None if sections is None else _whole(sections), bool(interleaved)
     if _forward._current_level >= 0:

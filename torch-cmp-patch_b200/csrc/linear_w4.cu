@@ -18,12 +18,16 @@
 // parts 6) are laid out in that order in shared memory once per CTA; others follow it with one byte
 // permutation a register, and fp32's are cut again for every tile (1 x 16384 x 4096 fp32: 18 us from
 // shared memory, 26 without).
-// What bounds it beside the bytes: first the lines that its loads touch (one a cycle), which is why eight lanes load
+// What bounds it beside the bytes: the lines that its loads touch (one a cycle), which is why eight lanes load
 // 128 bytes of a row together and scales and zero points come for sets of turns, through a table in shared
-// memory; then the half-rate units: for eight weights 3 shifts and 4 masks beside 4 subtractions (fp16: 1,
-// 4, 4).  Measured from a graph: 8 x 16384 x 4096 fp16, groups of 64: 15 us for 37 MB (5.7 at the
-// copy rate; 8 x 131072 x 4096: 72 us, 4.1 TB/s); 1 x 4096 x 4096 bf16: 5.9 us, most of it the launch and one pass
-// through the pipeline.
+// memory; then latency, at the four warps per scheduler that its registers leave.  Counted for 8 x 16384 x 4096 fp16, groups
+// of 64: 32 instructions per 32 words of weights, of which 9 widen (1 shift, 4 masks, 4 subtractions; bf16: 3, 4, 4), 1
+// multiplies and 3 load or store; the others are addresses, moves, selects and the scales' sums.  They take 54% of the issue
+// slots of the 14.2 us that the SMs are busy, no unit more than 42% (ALU); a warp waits longest for its loads (a fifth
+// of its cycles).  Starting and ending take 4.5 us more with cold caches.  Measured from a graph: that case 15.0 us (15.8 with a
+// bias) for 37 MB (5.7 at the copy rate; 8 x 131072 x 4096: 72 us, 4.1 TB/s); 1 x 4096 x 4096 bf16: 6.1 us, most of it
+// the launch and one pass through the pipeline.  16 x 16384 x 4096: 22.7 us; from the 17th token on the weights are read
+// and widened again for every 16 (32: 42 us, 64: 79).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -178,9 +182,10 @@ template <int DT, int NT, int GK, bool XS>
 __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_constant__ W4Args a) {
   using C = W4Cfg<DT, NT, GK, XS>;
   constexpr int ES = elt_size(DT), GROUPS = C::GROUPS, COLS = C::COLS;
-  // Where registers allow it (a spill costs more than either gives: 8 x 16384 x 4096 with groups of 64 takes 16.4
-  // us with 20 bytes of them, 14.7 with none), the two words of a quarter turn have sums of their own, and
-  // activations that are not in shared memory are loaded a quarter turn ahead.
+  // Where registers allow it, the two words of a quarter turn have sums of their own, and activations that are not in
+  // shared memory are loaded a quarter turn ahead.  8 x 16384 x 4096 fp16 with groups of 64 spills 20 bytes with them and is
+  // slower by 1.7 us of 15.  Without them, too, 29 of the 36 variants spill 4 to 120 bytes at the 128 registers that 16 warps
+  // leave a thread: all but one for 9 to 16 tokens, all for groups of 32, and most of fp32's.
   constexpr bool TWO = DT != CMPX_F32 && NT == 1 && GK == kGroup128;
   constexpr bool AHEAD = TWO && !XS;
   extern __shared__ __align__(128) uint8_t smem[];
