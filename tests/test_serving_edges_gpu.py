@@ -227,3 +227,19 @@ def test_low_parts_of_full_precision_activations(cuda_device, m, k, group):
     assert want.abs().max() < 2
     y = cmpext3.ops.linear_w4(x.to(cuda_device), w.to(cuda_device), torch.ones(24, k // group, device=cuda_device))
     assert torch.equal(y.cpu().double(), want[:, None].expand(m, 24))
+
+
+@pytest.mark.parametrize("m,k,group", [(1, 384, 128), (1, 4096, 128), (8, 4096, 128), (16, 4096, 128), (8, 4096, 64), (3, 2560, 32)])
+def test_full_precision_sums_are_fp32_sums(cuda_device, m, k, group):
+    from tests import serving_oracle as O
+    from tests.test_linear_w4_gpu import _make
+    x, w, s, z, _ = args = _make(torch.float32, m, 1001, k, group, True, False, k + group)
+    y = cmpext3.ops.linear_w4(*(None if t is None else t.to(cuda_device) for t in args)).cpu().double()
+    want = O.linear_w4(*args)[0]
+    codes = torch.stack((w & 15, w >> 4), -1).reshape(1001, -1, group).double()
+    weights = ((codes - z.double()[..., None]) * s.double()[..., None]).reshape(1001, k)
+    root = ((x.double() ** 2) @ (weights ** 2).t()).sqrt()          # of an output's squared products: about its size
+    # For every 32 k two sums are cut off at 2^-23 of a partial sum about as large as the root of its products' squares, with
+    # the sign of that sum, 2 * 2^-23 of the whole's; up to 24 fp32 sums of 2^-24 (8 words a warp, 16 warps), and a rounding
+    off = ((2 * 2.0 ** -23) ** 2 + 24 * (2.0 ** -24) ** 2) ** 0.5 + 2.0 ** -24
+    assert (y - want).norm() <= off * root.norm()

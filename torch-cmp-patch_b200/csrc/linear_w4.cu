@@ -5,7 +5,7 @@
 // code - zero is a whole number of at most 4 bits and a sign, exact in fp16 and bf16; the sums are
 // fp32 and the scale multiplies a group's fp32 sum, so no weight is ever rounded.  fp32 activations
 // go in as three bf16 parts (the leading, next and last 8 bits of the fraction: an exact sum), three
-// products each.
+// products each, and their sums leave the tensor core every 32 k.
 //
 // The weights are read once, n k / 2 bytes, and that read bounds it while the tokens are few.  One CTA per SM
 // has a run of tiles of 16 rows of W, and its warps have equal runs of the tiles' turns of 256 k laid
@@ -16,7 +16,7 @@
 // of it: word j of the lanes tq = 0..3 holds k = 16 tq + 8 j .. + 7, and nibbles e and e + 4 of a word, which
 // one mask isolates as the halves of a register, are a pair.  Activations of up to 64 KB (2 bytes a value, fp32's
 // parts 6) are laid out in that order in shared memory once per CTA; others follow it with one byte
-// permutation a register, and fp32's are cut again for every tile (1 x 16384 x 4096 fp32: 18 us from
+// permutation a register, and fp32's are cut again for every tile (1 x 16384 x 4096 fp32: 18.6 us from
 // shared memory, 26 without).
 // What bounds it beside the bytes: the lines that its loads touch (one a cycle), which is why eight lanes load
 // 128 bytes of a row together and scales and zero points come for sets of turns, through a table in shared
@@ -184,10 +184,16 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
   constexpr int ES = elt_size(DT), GROUPS = C::GROUPS, COLS = C::COLS;
   // Where registers allow it, the two words of a quarter turn have sums of their own, and activations that are not in
   // shared memory are loaded a quarter turn ahead.  8 x 16384 x 4096 fp16 with groups of 64 spills 20 bytes with them and is
-  // slower by 1.7 us of 15.  Without them, too, 29 of the 36 variants spill 4 to 120 bytes at the 128 registers that 16 warps
-  // leave a thread: all but one for 9 to 16 tokens, all for groups of 32, and most of fp32's.
+  // slower by 1.7 us of 15.  Without them, too, 26 of the 36 variants spill 4 to 80 bytes at the 128 registers that 16 warps
+  // leave a thread: all for 9 to 16 tokens, and for 8 all for groups of 32 and three of the six for groups of 64.
   constexpr bool TWO = DT != CMPX_F32 && NT == 1 && GK == kGroup128;
   constexpr bool AHEAD = TWO && !XS;
+  // fp32's sums leave the tensor core after every word (32 k), the low parts' added first: a sum in there is cut off,
+  // not rounded, which over a group of 128 times three parts shows (8 x 1001 x 4096: 5.0e-7 off; like this 9.4e-8, plain fp32 sums
+  // 2.6e-7; for 0 to 7% of the time).  One quarter turn at a time, where more would spill: none of its variants for 8
+  // tokens does but one, of 4 bytes (16 x 16384 x 4096, groups of 128: 49 us, 54 with the four quarters unrolled).
+  constexpr bool SHORT = DT == CMPX_F32;
+  constexpr int kAtOnce = SHORT ? 1 : kChunk / 64;  // quarter turns
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, tq = lane & 3;
   const int m0 = blockIdx.y * (8 * NT);
@@ -283,7 +289,20 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
     constexpr int CHAINS = TWO ? 2 : 1;
     float part[CHAINS][SETS][NT][4];
     float2 col[2], other[2];  // this lane's k's column, and (groups of 32) the quad's other one
+    auto add_scaled = [&](int t) {
 #pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float s = col[e >> 1].x;
+        if (GK == kGroup32) {
+          const float o = other[e >> 1].x;
+          acc[t][e] = fmaf(tq < 2 ? s : o, part[0][0][t][e], acc[t][e]);
+          acc[t][e] = fmaf(tq < 2 ? o : s, part[0][SETS - 1][t][e], acc[t][e]);
+        } else {
+          acc[t][e] = fmaf(s, TWO ? part[0][0][t][e] + part[CHAINS - 1][0][t][e] : part[0][0][t][e], acc[t][e]);
+        }
+      }
+    };
+#pragma unroll(kAtOnce)
     for (int h = 0; h < kChunk / 64; ++h) {
       const int k = c * kChunk + h * 64;
       if (!FULL && k >= a.k) break;
@@ -311,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
 #pragma unroll
       for (int r = 0; r < 2; ++r)
         w[r] = *reinterpret_cast<const uint2*>(stage + (8 * r + gr) * (kChunk / 2) + ((h ^ (gr & 3)) << 5) + tq * 8);
-      const bool first = GK != kGroup128 || (h & 1) == 0;  // of the products that share a scale
+      const bool first = SHORT || GK != kGroup128 || (h & 1) == 0;  // of the products that share a scale
       if (first) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -342,36 +361,26 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
             x[j][t].pairs(p);
           }
 #pragma unroll
-          for (int y = 0; y < PARTS; ++y) {
+          for (int y = PARTS - 1; y >= 0; --y) {
 #pragma unroll
             for (int set = 0; set < SETS; ++set) {
               // groups of 32: the quad's first two lanes are in one group, its last two in the next
               const bool in = SETS == 1 || (tq >> 1) == set;
               const uint32_t b0 = in ? p[y][0] : 0, b1 = in ? p[y][1] : 0, b2 = in ? p[y][2] : 0, b3 = in ? p[y][3] : 0;
               float(&sum)[4] = part[j % CHAINS][set][t];
-              if (first && j < CHAINS && y == 0)
+              if (SHORT ? y == PARTS - 1 : first && j < CHAINS)
                 mma_w4<DT, true>(sum, d0[0], d1[0], d0[1], d1[1], b0, b1);
               else
                 mma_w4<DT, false>(sum, d0[0], d1[0], d0[1], d1[1], b0, b1);
               mma_w4<DT, false>(sum, d0[2], d1[2], d0[3], d1[3], b2, b3);
             }
           }
+          if (SHORT) add_scaled(t);
         }
       }
-      if (GK == kGroup128 && first && (FULL || k + 64 < a.k)) continue;  // the next quarter has the same scale
+      if (SHORT || GK == kGroup128 && first && (FULL || k + 64 < a.k)) continue;  // the next quarter has the same scale
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float s = col[e >> 1].x;
-          if (GK == kGroup32) {
-            const float o = other[e >> 1].x;
-            acc[t][e] = fmaf(tq < 2 ? s : o, part[0][0][t][e], acc[t][e]);
-            acc[t][e] = fmaf(tq < 2 ? o : s, part[0][SETS - 1][t][e], acc[t][e]);
-          } else {
-            acc[t][e] = fmaf(s, TWO ? part[0][0][t][e] + part[CHAINS - 1][0][t][e] : part[0][0][t][e], acc[t][e]);
-          }
-        }
+      for (int t = 0; t < NT; ++t) add_scaled(t);
     }
   };
   auto write = [&](int m, int n, float s) {
