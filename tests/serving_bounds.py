@@ -25,8 +25,8 @@ def attention(q, k, v, scale):
     s = (qq @ kk.transpose(1, 2)) * scale                                            # [H, 1, n]
     p = torch.softmax(s, -1)
     out = (p @ vv)[:, 0]
-    # A score's products are off by 1.25 * 2^-20 each at most (two tf32 parts a value: the product of the rests, 2^-21, what
-    # a cut rest loses, 1.5 * 2^-22, and a rounded one, 2^-23; less in the other kernels), with the signs of q and k; its 24
+    # A score's products are off by 1.25 * 2^-20 each at most (two tf32 parts a value, rounded or cut: the product of the rests,
+    # 2^-21, and what two rests lose, 2 * 1.5 * 2^-22; less in the other kernels), with the signs of q and k; its 24
     # additions at most (chains of 16 products, of 8 per lane) by 2^-23 of a partial sum, on average of the size below, the
     # maximum's subtraction and the scale's product by 2^-23 of the score.
     size = ((qq ** 2) @ (kk ** 2).transpose(1, 2)).sqrt() * abs(scale) + s.abs()
@@ -110,9 +110,7 @@ def low_parts_want(which, q, k, v, scale, tensor_cores=True):
     return out, bound
 
 
-def one_part(x, which):
-    """x cut off (keys, values) or rounded (queries, weights) to 11 bits, in fp32."""
-    bits = x.float().view(torch.int32)
-    if which in ("queries", "weights"):
-        bits = bits + 0x1000
+def one_part(x, rounded):
+    """x rounded, or cut off, to 11 bits, in fp32."""
+    bits = x.float().view(torch.int32) + (0x1000 if rounded else 0)
     return (bits & ~0x1FFF).view(torch.float32)

@@ -97,3 +97,33 @@ def test_low_parts_in_full_precision(cuda_device, part, n, heads, D):
     for h, c in enumerate(cases):
         want, bound = B.low_parts_want(part, *c, tensor_cores=D <= 192 and (heads > 4 or heads > 1 and 64 < D <= 96))
         O.assert_within(out[h * heads:(h + 1) * heads], want, bound, f"key head {h}")
+
+
+@pytest.mark.parametrize("D", [40, 64, 80, 96, 128, 160, 192, 256])
+def test_one_key_gives_its_value_in_full_precision(cuda_device, D):
+    # a weight of one: a value's leading 11 bits are rounded, and of the rest, at most 2^-11 of it, 11 bits are left: within
+    # 2^-23 of the value; one key in each of 50 sequences, in pages of one
+    g = torch.Generator().manual_seed(D)
+    k, v = (torch.randn(50, 2, 1, D, generator=g).to(cuda_device) for _ in range(2))
+    q = torch.randn(50, 16, 1, D, generator=g).to(cuda_device)
+    table = torch.arange(50, dtype=torch.int32, device=cuda_device)[:, None]
+    out = cmpext3.ops.paged_attention(q, k, v, table, torch.ones(50, dtype=torch.int32, device=cuda_device))
+    want = v.double().repeat_interleave(8, 1)
+    assert ((out.double() - want).abs() <= 2.0 ** -23 * want.abs()).all()
+
+
+@pytest.mark.parametrize("D", [40, 64, 96, 128, 160, 192])
+def test_the_largest_values_stay_finite_in_full_precision(cuda_device, D):
+    # rounded to 11 bits they would be infinite; the second of two keys has a weight of exp(-30) and a small value
+    top = torch.finfo(torch.float32).max
+    k, v = (torch.zeros(1, 1, 16, D, device=cuda_device) for _ in range(2))
+    k[0, 0, 0, 0], v[0, 0, 0], v[0, 0, 1] = 30.0, top, 1.0
+    v[0, 0, 0, 1::2] = -top
+    q = torch.zeros(1, 8, 1, D, device=cuda_device)
+    q[..., 0] = 1.0
+    table = torch.zeros(1, 1, dtype=torch.int32, device=cuda_device)
+    for n in (1, 2):
+        out = cmpext3.ops.paged_attention(q, k, v, table, torch.tensor([n], dtype=torch.int32, device=cuda_device), 1.0)[0, :, 0]
+        want = v[0, 0, 0].double() / (1 + (n - 1) * torch.exp(torch.tensor(-30.0, dtype=torch.float64)).item())
+        # two parts cut off: 3 * 2^-23, and the sums and the quotient 2^-22
+        assert torch.isfinite(out).all() and ((out.double() - want).abs() <= 5 * 2.0 ** -23 * want.abs()).all()

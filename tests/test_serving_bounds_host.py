@@ -12,15 +12,15 @@ def _random(n, d, dtype, heads=1, seed=0):
     return tuple(torch.randn(s, generator=g).to(dtype) for s in ((heads, d), (1, n, d), (1, n, d)))
 
 
-def _attend(q, k, v, scale, keep=None, tf32=()):
+def _attend(q, k, v, scale, keep=None, tf32=(), rounded=True):
     """The definition over the keys `keep`, with the operands named in tf32 as one part of 11 bits."""
     if keep is not None:
         k, v = k[:, keep], v[:, keep]
-    q, k, v = (B.one_part(t, w).double() if w in tf32 else t.double() for t, w in ((q, "queries"), (k[0], "keys"), (v[0], "values")))
+    q, k, v = (B.one_part(t, rounded).double() if w in tf32 else t.double() for t, w in ((q, "queries"), (k[0], "keys"), (v[0], "values")))
     p = torch.softmax(q @ k.t() * scale, -1)
     if "weights" in tf32:
         top = p.amax(-1, keepdim=True)                      # the kernels' weights are at most 1
-        p = B.one_part(p / top, "weights").double() * top
+        p = B.one_part(p / top, rounded).double() * top
     return p @ v
 
 
@@ -52,7 +52,8 @@ def test_operands_of_one_part_are_seen_in_full_precision(n, d, part):
     q, k, v = _random(n, d, torch.float32, heads=8, seed=d)
     want, bound = B.attention(q, k, v, d ** -0.5)
     assert not _seen(_attend(q, k, v, d ** -0.5).float().double(), want, bound)
-    assert _seen(_attend(q, k, v, d ** -0.5, tf32=(part,)), want, bound)
+    for rounded in (False, True):
+        assert _seen(_attend(q, k, v, d ** -0.5, tf32=(part,), rounded=rounded), want, bound)
 
 
 @pytest.mark.parametrize("n", [40, 3000, 9500])

@@ -7,16 +7,16 @@
 //   S^T = K Q^T (keys x heads),  O^T += V^T P^T (dims x heads),
 // sums and softmax in fp32.  The order of a product's k, and of the rows of the other side, is free as long as
 // both sides share it: a lane takes 16 bytes of a row at a time, and P^T's fragments are S^T's, turned by movmatrix.
-// K and V are cut with an AND and a subtraction each, always towards zero; Q and P, whose values are used many times, are
-// rounded.  If a result is not finite, the warp walks its keys once more with infinities (whose rest would be NaN) in mind.
-// What that is off by, of a product: the two rests' product, which is left out, is below 2^-21 (a cut rest is below 2^-10, a
-// rounded one 2^-11), a cut rest loses up to 1.5 * 2^-22, a rounded one 2^-23.  Against 64 bits, norm of the
-// difference over the result's, random inputs of 300 to 30000 keys, by head size (this kernel; FMA units on the same inputs; plain
-// fp32 products): 40: 4.1e-7, 2.4e-7, 4.1e-7; 64: 4.5, 2.3, 4.4; 80: 4.0, 2.7, 4.8; 96: 4.2, 2.7, 5.2; 128: 4.1, 2.4, 5.2;
-// 160: 3.6, 2.8, 5.5; 192: 3.6, 2.9, 6.0 (the largest of three lengths).
+// K and V are cut with an addition, an AND and a subtraction each.  If a result is not finite, the warp walks its keys
+// once more with infinities (whose rest would be NaN) in mind.
+// What that is off by, of a product: the two rests' product, which is left out, is at most 2^-22 (a rest is at most 2^-11), and
+// each rest loses up to 2^-23.  Against 64 bits, norm of the difference over the result's, random inputs of 300 to
+// 30000 keys, by head size (this kernel; FMA units on the same inputs; plain fp32 products): 40: 2.9e-7, 2.4e-7, 4.1e-7;
+// 64: 3.0, 2.3, 4.4; 80: 2.9, 2.7, 4.8; 96: 2.8, 2.7, 5.2; 128: 2.8, 2.4, 5.2; 160: 2.4, 2.8, 5.5; 192: 2.6, 2.9, 6.0
+// (the largest of three lengths).  With the leading parts of K and V cut towards zero it was 3.6 to 4.5, in the same time.
 // What bounds it: the two or three warps that a scheduler has, whose registers and buffers leave no more, wait for their
 // own products and shuffles (issue slots 46% used, tensor cores 26% at 64).  [8, 32 heads, 4 key heads] over
-// 200 MB: 53 us at 40, 43 at 64, 44 at 80, 38 at 96, 37 at 128, 51 at 160, 50 at 192 (FMA units: 74, 52, 75, 67,
+// 200 MB: 52 us at 40, 42 at 64, 43 at 80, 37 at 96, 37 at 128, 50 at 160, 49 at 192 (FMA units: 74, 52, 75, 67,
 // 53, 84, 71); at 256 the queries do not fit the registers.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -45,11 +45,11 @@ struct PartsCfg {
   static_assert(Pipe::BYTES >= kHeads * DP * 4, "the warps' outputs are joined in the buffers");
 };
 
-// The parts of a value: the upper 11 bits of its fraction, and the rest, of which the tensor cores take 11 more.  An
-// infinite value has no rest; without INF its rest is NaN.
+// The parts of a value: the upper 11 bits of its fraction, rounded, and the rest, of which the tensor cores take 11 of its
+// 12 bits.  An infinite value (and one that is rounded to it) has no rest; without INF its rest is NaN.
 template <bool INF>
 __device__ __forceinline__ void cut(float x, uint32_t (&p)[2]) {
-  p[0] = __float_as_uint(x) & 0xFFFFE000u;
+  p[0] = (INF ? __float_as_uint(x) : __float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
   float rest = x - __uint_as_float(p[0]);
   if (INF && fabsf(x) == INFINITY) rest = 0.f;
   p[1] = __float_as_uint(rest);
