@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_w4_kernel(const __grid_con
   // Where registers allow it, the two words of a quarter turn have sums of their own, and activations that are not in
   // shared memory are loaded a quarter turn ahead.  8 x 16384 x 4096 fp16 with groups of 64 spills 20 bytes with them and is
   // slower by 1.7 us of 15.  Without them, too, 26 of the 36 variants spill 4 to 80 bytes at the 128 registers that 16 warps
-  // leave a thread: all for 9 to 16 tokens, and for 8 all for groups of 32 and three of the six for groups of 64.
+  // leave a thread: all for 9 to 16 tokens, and for 8 all but one for groups of 32 and three of the six for groups of 64.
   constexpr bool TWO = DT != CMPX_F32 && NT == 1 && GK == kGroup128;
   constexpr bool AHEAD = TWO && !XS;
   // fp32's sums leave the tensor core after every word (32 k), the low parts' added first: a sum in there is cut off,
